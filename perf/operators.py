@@ -1,0 +1,537 @@
+"""What the batch operators over a shared paged cache are measured on.
+
+Three operators serve the rows of many sequences in one call, each sequence with
+its own page table over one pool of int8 K/V pages:
+
+- ``append``: per-head norm and rotary positions of new Q/K rows, their int8
+  quantisation, and K/V written into the sequences' pages; with ``bounds`` also
+  the channel bounds of the pages that were written;
+- ``attention``: attention of every sequence's new rows (one token, a chunk or a
+  whole prompt, mixed in one call) over its cached keys;
+- ``sparse``: for each new row and KV head the pages whose bounds promise the
+  largest scores, and attention over those pages alone.
+
+A case is a dict of plain values; ``draw`` gives more of the same ranges.  The
+lengths of a case's sequences follow from its ``lens`` alone, the values from the
+seed.  K/V rows and queries are unit-variance heads quantised to int8.
+"""
+from __future__ import annotations
+
+import math
+import random
+import sys
+from pathlib import Path
+
+import numpy as np
+import torch
+
+own = False
+
+HD = 128
+QK_SCALE = float(np.float32(1.0 / math.sqrt(HD)))
+INV_HD = 1.0 / HD
+INV127 = float(np.float32(1.0) / np.float32(127.0))
+THETA = 1e6
+
+
+def listed():
+    return [
+        # one decoding token's Q/K/V rows into the cache: the smallest call
+        {"name": "append_1", "kind": "append", "lens": 1, "n": 1, "rows_lo": 1, "rows_hi": 1, "ctx_lo": 4000, "ctx_hi": 4000,
+         "heads": 16, "kv_heads": 8, "page": 32, "rot": 128, "interleaved": False, "norm": True, "bounds": False},
+        # a decoding batch of another head layout, half of each head rotated in pairs
+        {"name": "append_48", "kind": "append", "lens": 2, "n": 48, "rows_lo": 1, "rows_hi": 1, "ctx_lo": 100, "ctx_hi": 4000,
+         "heads": 32, "kv_heads": 8, "page": 64, "rot": 64, "interleaved": True, "norm": False, "bounds": True},
+        # a continuous batch: prompt chunks and decoding rows together
+        {"name": "append_ragged", "kind": "append", "lens": 3, "n": 7, "rows_lo": 1, "rows_hi": 500, "ctx_lo": 1, "ctx_hi": 3000,
+         "heads": 16, "kv_heads": 8, "page": 32, "rot": 128, "interleaved": False, "norm": True, "bounds": True},
+        # a long prompt's rows at once
+        {"name": "append_2048", "kind": "append", "lens": 4, "n": 1, "rows_lo": 2048, "rows_hi": 2048, "ctx_lo": 0, "ctx_hi": 0,
+         "heads": 16, "kv_heads": 8, "page": 32, "rot": 128, "interleaved": False, "norm": True, "bounds": False},
+        # one token of a chat at a short context
+        {"name": "attention_1_at_543", "kind": "attention", "lens": 5, "n": 1, "rows_lo": 1, "rows_hi": 1, "ctx_lo": 543, "ctx_hi": 543,
+         "heads": 16, "kv_heads": 8, "page": 32},
+        # one token late in a very long context
+        {"name": "attention_1_at_131071", "kind": "attention", "lens": 6, "n": 1, "rows_lo": 1, "rows_hi": 1, "ctx_lo": 131071,
+         "ctx_hi": 131071, "heads": 16, "kv_heads": 8, "page": 64},
+        # a serving batch decoding at contexts of very different lengths
+        {"name": "attention_64", "kind": "attention", "lens": 7, "n": 64, "rows_lo": 1, "rows_hi": 1, "ctx_lo": 500, "ctx_hi": 4000,
+         "heads": 16, "kv_heads": 8, "page": 32},
+        # prompt chunks of some requests beside decoding rows of others
+        {"name": "attention_mixed", "kind": "attention", "lens": 8, "n": 20, "rows_lo": 1, "rows_hi": 300, "ctx_lo": 1, "ctx_hi": 3000,
+         "heads": 16, "kv_heads": 8, "page": 32},
+        # three whole prompts in one call
+        {"name": "attention_prompts", "kind": "attention", "lens": 9, "n": 3, "rows_lo": 1500, "rows_hi": 2500, "ctx_lo": 0, "ctx_hi": 0,
+         "heads": 32, "kv_heads": 8, "page": 128},
+        # one token at a long context, a sixteenth of its pages read
+        {"name": "sparse_1_at_32767", "kind": "sparse", "lens": 10, "n": 1, "rows_lo": 1, "rows_hi": 1, "ctx_lo": 32767, "ctx_hi": 32767,
+         "heads": 16, "kv_heads": 8, "page": 32, "select": 64},
+        # a decoding batch at long contexts, eight query heads to a KV head
+        {"name": "sparse_24", "kind": "sparse", "lens": 11, "n": 24, "rows_lo": 1, "rows_hi": 1, "ctx_lo": 4000, "ctx_hi": 20000,
+         "heads": 64, "kv_heads": 8, "page": 64, "select": 33},
+        # short chunks (verified drafts, late prompt chunks) at long contexts
+        {"name": "sparse_chunks", "kind": "sparse", "lens": 12, "n": 3, "rows_lo": 16, "rows_hi": 70, "ctx_lo": 5000, "ctx_hi": 8000,
+         "heads": 16, "kv_heads": 8, "page": 32, "select": 48},
+    ]
+
+
+def _size(rng, lo, hi):
+    """A size between lo and hi, spread over its logarithm (0 as likely as 1)."""
+    return max(lo, min(hi, round(math.exp(rng.uniform(math.log(lo + 1), math.log(hi + 2))) - 1)))
+
+
+def draw(rng):
+    most = {k: max(_cost(c) for c in listed() if c["kind"] == k) for k in ("append", "attention", "sparse")}
+    while True:
+        heads, kv_heads = rng.choice([(16, 8), (16, 8), (32, 8), (64, 8), (12, 4), (8, 8), (20, 4), (16, 1)])
+        c = {"kind": rng.choice(["append", "attention", "attention", "sparse"]), "lens": rng.randrange(1 << 20), "n": _size(rng, 1, 64),
+             "heads": heads, "kv_heads": kv_heads, "page": rng.choice([32, 32, 64, 96, 128, 256])}
+        rows, ctx = _size(rng, 1, 2500), _size(rng, 0, 131071)
+        if rng.random() < 0.5:
+            rows = 1
+        if c["kind"] == "append":
+            ctx = min(ctx, 6000)
+            c.update(rot=rng.choice([128, 128, 64, 32, 96, 2]), interleaved=rng.random() < 0.5, norm=rng.random() < 0.5, bounds=rng.random() < 0.5)
+        if c["kind"] == "sparse":
+            rows = min(rows, 100)
+            c.update(select=_size(rng, 1, 128))
+        c.update(rows_lo=rng.choice([1, rows]), rows_hi=rows, ctx_lo=rng.choice([0, ctx // 4, ctx]), ctx_hi=ctx)
+        pages = sum(_pages(c, r + x) for r, x in _lens(c))
+        dense = c["n"] * c["heads"] * c["rows_hi"] * (c["rows_hi"] + c["ctx_hi"])  # the plain form's padded scores
+        if pages < 65536 and pages * c["page"] <= 400000 and dense <= 1 << 30 and _cost(c) <= most[c["kind"]]:
+            return c
+
+
+def _lens(case):
+    """(new rows, keys before them) of each sequence."""
+    r = random.Random(case["lens"])
+    return [(_size(r, case["rows_lo"], case["rows_hi"]), _size(r, case["ctx_lo"], case["ctx_hi"])) for _ in range(case["n"])]
+
+
+def _pages(case, tokens):
+    return -(-tokens // case["page"])
+
+
+def work(case):
+    lens, H, KV = _lens(case), case["heads"], case["kv_heads"]
+    rows, keys = sum(r for r, _ in lens), sum(r + c for r, c in lens)
+    if case["kind"] == "append":
+        # f32 rows read, int8 rows and scales written, a row of angles per new row
+        b = rows * (H + 2 * KV) * (4 * HD + HD + 4) + rows * 4 * case["rot"]
+        f = rows * (H + KV) * 6 * HD + rows * (H + 2 * KV) * 3 * HD
+        if case["bounds"]:
+            touched = sum(_pages(case, c + r) - c // case["page"] for r, c in lens)
+            b += touched * KV * (2 * HD + 4) + sum(c % case["page"] for _, c in lens) * KV * (HD + 4)
+            f += touched * KV * case["page"] * 3 * HD
+        return {"bytes": b, "flops": f}
+    b = rows * H * (HD + 4 + 4 * HD)
+    if case["kind"] == "attention":
+        pairs = sum(r * c + r * (r + 1) // 2 for r, c in lens)
+        return {"bytes": b + keys * KV * 2 * (HD + 4), "flops": 4 * HD * H * pairs}
+    f = 0
+    for r, c in lens:
+        pages = _pages(case, c + r)
+        read = min(pages, case["select"]) * case["page"]
+        b += pages * KV * (2 * HD + 4) + min(r * read, c + r) * KV * 2 * (HD + 4) + r * KV * 4 * case["select"]
+        f += r * H * (2 * 2 * HD * pages + 4 * HD * min(read, c + r))
+    return {"bytes": b, "flops": f}
+
+
+def _cost(case):
+    w = work(case)
+    return max(w["bytes"], w["flops"] / 50)
+
+
+# ---- inputs -----------------------------------------------------------------
+
+
+def _int8(g, *shape, sigma=42.0):
+    x = torch.empty(shape, dtype=torch.int8, device="cuda")
+    flat = x.view(-1)
+    for i in range(0, flat.numel(), 1 << 27):  # the f32 values of a large pool in pieces
+        n = min(1 << 27, flat.numel() - i)
+        flat[i:i + n] = torch.randn(n, device="cuda", generator=g).mul_(sigma).round_().clamp_(-127, 127).to(torch.int8)
+    return x
+
+
+def _uniform(g, lo, hi, *shape):
+    return torch.rand(*shape, device="cuda", generator=g).mul_(hi - lo).add_(lo)
+
+
+def prepare(case, seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed & 0x7FFFFFFFFFFF)
+    lens, H, KV, page = _lens(case), case["heads"], case["kv_heads"], case["page"]
+    n, rows = len(lens), sum(r for r, _ in lens)
+    per = [_pages(case, r + c) for r, c in lens]
+    n_pages, ld = sum(per), max(per)
+    order = np.random.default_rng([seed & 0x7FFFFFFF, 1]).permutation(n_pages)
+    tables = np.zeros((n, ld), np.uint16)
+    for i, p in enumerate(per):
+        tables[i, :p] = order[sum(per[:i]):sum(per[:i + 1])]
+    start = np.cumsum([0] + [r for r, _ in lens])
+    s = {
+        "case": dict(case), "rows": rows, "max_rows": max(r for r, _ in lens), "max_kv": max(r + c for r, c in lens), "n_pages": n_pages,
+        "tables": torch.from_numpy(tables.view(np.int16)).cuda(),
+        "row_start": torch.from_numpy(start.astype(np.int32)).cuda(),
+        "kv_len": torch.tensor([r + c for r, c in lens], dtype=torch.int32, device="cuda"),
+        # the pool: K/V rows of every page and one scale for each token and head
+        "k": _int8(g, n_pages, page, KV * HD), "ks": _uniform(g, 0.018, 0.03, n_pages, page, KV),
+        "v": _int8(g, n_pages, page, KV * HD), "vs": _uniform(g, 0.018, 0.03, n_pages, page, KV),
+    }
+    if case["kind"] == "append":
+        qkv = torch.randn(rows, (H + 2 * KV) * HD, device="cuda", generator=g)  # one fused projection's rows
+        s["xq"], s["xk"], s["xv"] = qkv[:, :H * HD], qkv[:, H * HD:(H + KV) * HD], qkv[:, (H + KV) * HD:]
+        s["nq"], s["nk"] = (torch.randn(HD, device="cuda", generator=g).mul_(0.05).add_(1.0) for _ in range(2))
+        half = case["rot"] // 2
+        inv = THETA ** (-torch.arange(half, dtype=torch.float64, device="cuda") / half)
+        a = torch.arange(s["max_kv"], dtype=torch.float64, device="cuda")[:, None] * inv
+        s["cos"], s["sin"] = a.cos().float(), a.sin().float()
+        s["q8"] = torch.empty(rows, H * HD, dtype=torch.int8, device="cuda")
+        s["qs"] = torch.empty(rows, H, device="cuda")
+        if case["bounds"]:
+            s["bounds"] = torch.zeros(n_pages * KV, 2 * HD, dtype=torch.int8, device="cuda")
+            s["bscale"] = torch.zeros(n_pages, KV, device="cuda")
+        return s
+    s["q8"], s["qs"] = _int8(g, rows, H * HD), _uniform(g, 0.018, 0.03, rows, H)
+    s["out"] = torch.empty(rows, H * HD, device="cuda")
+    if case["kind"] == "sparse":
+        # keys of one page lie near each other, as neighbouring tokens' do
+        s["k"].copy_((s["k"].float() * 0.6 + _int8(g, n_pages, 1, KV * HD).float() * 0.7).round_().clamp_(-127, 127).to(torch.int8))
+        s["bounds"], s["bscale"] = (t.contiguous() for t in _page_bounds(s, torch.arange(n_pages, device="cuda"), None))
+        s["ids"] = torch.empty(rows, KV * case["select"], dtype=torch.int32, device="cuda")
+    return s
+
+
+# ---- the framework's operators ------------------------------------------------
+
+
+def _run_own(s):
+    pkg = str(Path.cwd() / "qwen3-tile-ops_amd")
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
+    from q3ops import ops
+
+    c = s["case"]
+    if "pool" not in s:  # the handle of the pool, made once
+        s["pool"] = ops.kv_pool(s["k"], s["v"], s["ks"], s["vs"])
+    pool = s["pool"]
+    seqs = ops.sequences(pool, s["tables"], s["row_start"], s["kv_len"], s["max_rows"], s["max_kv"])
+    if c["kind"] == "append":
+        ops.rope_append_paged(s["xq"], s["xk"], s["xv"], pool, seqs, s["q8"], s["qs"], nwq=s["nq"] if c["norm"] else None,
+                              nwk=s["nk"] if c["norm"] else None, inv_hd=INV_HD, cos=s["cos"], sin=s["sin"], rot_dim=c["rot"],
+                              interleaved=c["interleaved"])
+        if c["bounds"]:
+            ops.page_bounds(pool, seqs, s["bounds"], s["bscale"])
+        return [s[k] for k in ("q8", "qs", "k", "ks", "v", "vs") + (("bounds", "bscale") if c["bounds"] else ())]
+    if c["kind"] == "attention":
+        ops.attention_varlen_paged(s["q8"], s["qs"], pool, seqs, s["out"], qk_scale=QK_SCALE)
+        return s["out"]
+    ops.select_pages(s["q8"], s["qs"], pool, seqs, s["bounds"], s["bscale"], s["ids"], c["select"])
+    ops.attention_pages(s["q8"], s["qs"], pool, seqs, s["ids"], c["select"], s["out"], qk_scale=QK_SCALE)
+    return s["ids"], s["out"]
+
+
+def run(state):
+    if own:
+        return _run_own(state)
+    return {"append": _append, "attention": _attention, "sparse": _sparse}[state["case"]["kind"]](state)
+
+
+# ---- plain forms ----------------------------------------------------------------
+
+
+def _rows_of(s):
+    """Sequence and position of each new row."""
+    start, kv = s["row_start"].long(), s["kv_len"].long()
+    r = torch.arange(s["rows"], device="cuda")
+    seq = torch.searchsorted(start, r, right=True) - 1
+    return seq, kv[seq] - start[seq + 1] + r
+
+
+def _tables(s):
+    return s["tables"].long() & 0xFFFF
+
+
+def _head_norm(x, w):
+    """x / sqrt(mean x^2 + eps) * w of 128-wide heads, the squares added in the
+    order of the framework's head norm (pairs within 32 columns, then the four
+    sums), so that the int8 values behind it are the same."""
+    q = (x * x).view(*x.shape[:-1], 4, 32)
+    q = q[..., 0::2] + q[..., 1::2]
+    q = q[..., 0::2] + q[..., 1::2]
+    q = q[..., 0::2] + q[..., 1::2]
+    q = q[..., 0::2] + q[..., 1::2]
+    q = q[..., 0] + q[..., 1]
+    m = (((q[..., 0] + q[..., 1]) + q[..., 2]) + q[..., 3]) * INV_HD + 1e-6
+    r = (1.0 / m.double().sqrt().float().double()).float()
+    return (x * r[..., None]) * w
+
+
+def _rotate(x, cos, sin, rot, interleaved):
+    """Rotary positions of the first `rot` columns of x [rows][heads][128]."""
+    cos, sin = cos[:, None, :], sin[:, None, :]
+    h = rot // 2
+    a, b = (x[..., 0:rot:2], x[..., 1:rot:2]) if interleaved else (x[..., :h], x[..., h:rot])
+    ra, rb = a * cos - b * sin, a * sin + b * cos
+    y = torch.stack((ra, rb), -1).flatten(-2) if interleaved else torch.cat((ra, rb), -1)
+    return torch.cat((y, x[..., rot:]), -1)
+
+
+def _quantise(x):
+    """int8 of x [...][128] and its scales absmax / 127: the f32 quotient,
+    rounded to the nearest integer (64 bits, then 32, is the f32 quotient)."""
+    scale = x.abs().amax(-1) * INV127
+    q = (x.double() / scale.double()[..., None]).float()
+    return torch.nan_to_num(q, nan=0.0).round().clamp(-127, 127).to(torch.int8), scale
+
+
+def _page_bounds(s, pages, tokens):
+    """Channel-wise least and largest key of the given pages (their first
+    `tokens` tokens; all where None), rounded outwards to int8 with one scale."""
+    KV = s["case"]["kv_heads"]
+    k = s["k"][pages].view(len(pages), -1, KV, HD).float() * s["ks"][pages][..., None]
+    lo, hi = k, k
+    if tokens is not None:
+        dead = (torch.arange(k.shape[1], device="cuda")[None] >= tokens[:, None])[..., None, None]
+        lo, hi = k.masked_fill(dead, math.inf), k.masked_fill(dead, -math.inf)
+    lo, hi = lo.amin(1), hi.amax(1)
+    scale = torch.maximum(lo.abs(), hi.abs()).amax(-1) * INV127
+    d = scale.double()[..., None]
+    lo = torch.nan_to_num((lo.double() / d).float(), nan=0.0).floor().clamp(-127, 127)
+    hi = torch.nan_to_num((hi.double() / d).float(), nan=0.0).ceil().clamp(-127, 127)
+    return torch.cat((lo, hi), -1).to(torch.int8).view(-1, 2 * HD), scale
+
+
+def _append(s):
+    c = s["case"]
+    H, KV, page, rows = c["heads"], c["kv_heads"], c["page"], s["rows"]
+    seq, pos = _rows_of(s)
+    q, k, v = s["xq"].reshape(rows, H, HD), s["xk"].reshape(rows, KV, HD), s["xv"].reshape(rows, KV, HD)
+    if c["norm"]:
+        q, k = _head_norm(q, s["nq"]), _head_norm(k, s["nk"])
+    cos, sin = s["cos"][pos], s["sin"][pos]
+    q8, qs = _quantise(_rotate(q, cos, sin, c["rot"], c["interleaved"]))
+    k8, ks = _quantise(_rotate(k, cos, sin, c["rot"], c["interleaved"]))
+    v8, vs = _quantise(v)
+    tables = _tables(s)
+    at, slot = tables[seq, pos // page], pos % page
+    s["k"][at, slot], s["ks"][at, slot] = k8.view(rows, -1), ks
+    s["v"][at, slot], s["vs"][at, slot] = v8.view(rows, -1), vs
+    out = [q8.view(rows, -1), qs, s["k"], s["ks"], s["v"], s["vs"]]
+    if c["bounds"]:
+        # the pages that got rows: one row of each is enough to name it
+        logical, kv = pos // page, s["kv_len"].long()[seq]
+        pages = at.unique()
+        tokens = torch.zeros(s["n_pages"], dtype=torch.int64, device="cuda")
+        tokens[at] = torch.minimum(kv - logical * page, torch.full_like(kv, page))
+        b, bs = _page_bounds(s, pages, tokens[pages])
+        s["bounds"].view(s["n_pages"], -1)[pages] = b.view(len(pages), -1)
+        s["bscale"][pages] = bs
+        out += [s["bounds"], s["bscale"]]
+    return out
+
+
+def _gathered(s, dtype):
+    """K, V as [sequence][KV head][key][128] over each sequence's pages, padded
+    to the longest; the values of padded keys are finite and masked later."""
+    KV = s["case"]["kv_heads"]
+    t = _tables(s)
+    both = []
+    for x, xs in ((s["k"], s["ks"]), (s["v"], s["vs"])):
+        rows = x[t].view(len(t), -1, KV, HD)[:, :s["max_kv"]].to(dtype) * xs[t].view(len(t), -1, KV)[:, :s["max_kv"], :, None].to(dtype)
+        both.append(rows.transpose(1, 2).contiguous())
+    return both
+
+
+def _padded_queries(s, dtype):
+    """Queries as [sequence][KV head][row x group][128], the last real rows'
+    positions [sequence][row], and where each row came from."""
+    c = s["case"]
+    H, KV = c["heads"], c["kv_heads"]
+    start, kv = s["row_start"].long(), s["kv_len"].long()
+    n = start[1:] - start[:-1]
+    i = torch.arange(s["max_rows"], device="cuda")
+    pos = kv[:, None] - n[:, None] + i
+    at = (start[:-1, None] + i).clamp(max=s["rows"] - 1)
+    q = s["q8"].to(dtype).view(s["rows"], H, HD) * s["qs"].to(dtype)[..., None]
+    q = q[at].view(len(n), len(i), KV, H // KV, HD).permute(0, 2, 1, 3, 4).reshape(len(n), KV, len(i) * (H // KV), HD)
+    return q, pos.masked_fill(i >= n[:, None], 0), i < n[:, None]
+
+
+def _softmax_times(x, v):
+    """softmax(x) . v along the last axis of x, rows whose x is all -inf as 0."""
+    m = x.amax(-1, keepdim=True)
+    p = (x - m.masked_fill(m == -math.inf, 0)).exp_()
+    return torch.matmul(p, v) / p.sum(-1, keepdim=True).clamp(min=1e-30)
+
+
+def _attend(s, dtype):
+    c = s["case"]
+    H, KV = c["heads"], c["kv_heads"]
+    G = H // KV
+    k, v = _gathered(s, dtype)
+    q, pos, real = _padded_queries(s, dtype)
+    x = torch.matmul(q, k.transpose(-1, -2)).mul_(QK_SCALE)
+    hidden = torch.arange(s["max_kv"], device="cuda") > pos.repeat_interleave(G, 1)[:, None, :, None]
+    o = _softmax_times(x.masked_fill_(hidden, -math.inf), v)
+    o = o.view(len(pos), KV, -1, G, HD).permute(0, 2, 1, 3, 4).reshape(len(pos), -1, H * HD)
+    return o[real]
+
+
+def _attention(s):
+    return _attend(s, torch.float32)
+
+
+def _select(s):
+    """The `select` pages of each row and KV head with the largest bounds of a
+    score, the row's own page among them: [rows][KV][select], ascending, -1 behind
+    the last.  The sums are of whole numbers below 2^24, exact in f32."""
+    c = s["case"]
+    H, KV, page, rows, n_sel = c["heads"], c["kv_heads"], c["page"], s["rows"], c["select"]
+    seq, pos = _rows_of(s)
+    t = _tables(s)
+    b = s["bounds"].view(-1, KV, 2 * HD)[t].transpose(1, 2).float()  # [seq][KV][page][256]
+    bs = s["bscale"][t].transpose(1, 2)
+    q = s["q8"].float().view(rows, KV, H // KV, HD)
+    q = torch.cat((q.clamp(max=0), q.clamp(min=0)), -1)
+    x = torch.matmul(q[:, :, :, None], b.transpose(-1, -2).contiguous()[seq][:, :, None]).squeeze(-2)  # [rows][KV][G][page]
+    x = (x * bs[seq][:, :, None]) * s["qs"].view(rows, KV, -1)[..., None]
+    x = x.amax(2)
+    last = (pos // page)[:, None, None]
+    i = torch.arange(t.shape[1], device="cuda")
+    x = x.masked_fill(i > last, -math.inf).masked_fill(i == last, math.inf)
+    order = torch.sort(x, dim=-1, descending=True, stable=True).indices[..., :n_sel]
+    order = order.masked_fill(order > last, 1 << 30).sort(-1).values
+    ids = torch.full((rows, KV, n_sel), 1 << 30, device="cuda")
+    ids[..., :order.shape[-1]] = order
+    return ids.masked_fill(ids == 1 << 30, -1), seq, pos
+
+
+def _attend_pages(s, ids, seq, pos, dtype):
+    c = s["case"]
+    H, KV, page, rows = c["heads"], c["kv_heads"], c["page"], s["rows"]
+    key = (ids[..., None] * page + torch.arange(page, device="cuda")).flatten(-2)  # [rows][KV][keys]
+    hidden = ((key < 0) | (key > pos[:, None, None]))[:, :, None]
+    key = key.clamp(min=0)
+    at = _tables(s)[seq[:, None, None], (key // page).clamp(max=s["tables"].shape[1] - 1)]
+    head = torch.arange(KV, device="cuda")[None, :, None]
+    k = s["k"].view(-1, page, KV, HD)[at, key % page, head].to(dtype) * s["ks"][at, key % page, head][..., None].to(dtype)
+    v = s["v"].view(-1, page, KV, HD)[at, key % page, head].to(dtype) * s["vs"][at, key % page, head][..., None].to(dtype)
+    q = s["q8"].to(dtype).view(rows, KV, H // KV, HD) * s["qs"].to(dtype).view(rows, KV, H // KV, 1)
+    x = torch.matmul(q, k.transpose(-1, -2)).mul_(QK_SCALE)
+    return _softmax_times(x.masked_fill_(hidden, -math.inf), v).reshape(rows, H * HD)
+
+
+def _sparse(s):
+    ids, seq, pos = _select(s)
+    return ids.to(torch.int32).view(s["rows"], -1), _attend_pages(s, ids, seq, pos, torch.float32)
+
+
+# ---- the definitions in 64 bits -----------------------------------------------------
+
+
+def exact(case, seed):
+    if case["kind"] == "sparse" and sum(r for r, _ in _lens(case)) > 2000:
+        return None  # row by row: too long
+    s = prepare(case, seed)
+    return {"append": _exact_append, "attention": _exact_attention, "sparse": _exact_sparse}[case["kind"]](s)
+
+
+def _host_rows(s):
+    """(sequence, row, position) of each new row."""
+    start, kv = s["row_start"].tolist(), s["kv_len"].tolist()
+    return [(i, r, kv[i] - start[i + 1] + r) for i in range(len(kv)) for r in range(start[i], start[i + 1])]
+
+
+def _exact_append(s):
+    """The scales in 64 bits; the int8 values hang on f32 roundings and have no
+    such value."""
+    c = s["case"]
+    H, KV, page, h = c["heads"], c["kv_heads"], c["page"], c["rot"] // 2
+    where = _host_rows(s)
+    pos = torch.tensor([p for _, _, p in where], device="cuda")
+    t = s["tables"].cpu().numpy().view(np.uint16)
+    at = torch.tensor([int(t[i, p // page]) for i, _, p in where], device="cuda")
+    first = torch.arange(h, device="cuda") * (2 if c["interleaved"] else 1)
+    second = first + (1 if c["interleaved"] else h)
+    cos, sin = s["cos"].double()[pos][:, None], s["sin"].double()[pos][:, None]
+    scales = []
+    for x, w, heads in ((s["xq"], s["nq"], H), (s["xk"], s["nk"], KV), (s["xv"], None, KV)):
+        x = x.double().reshape(-1, heads, HD)
+        if w is not None:
+            if c["norm"]:
+                x = x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + 1e-6) * w.double()
+            a, b = x[..., first], x[..., second]
+            x = x.clone()
+            x[..., first], x[..., second] = a * cos - b * sin, b * cos + a * sin
+        scales.append(x.abs().amax(-1) / 127)
+    ks, vs = s["ks"].double(), s["vs"].double()
+    ks[at, pos % page], vs[at, pos % page] = scales[1], scales[2]
+    out = [None, scales[0], None, ks, None, vs]
+    return out + [None, None] if c["bounds"] else out
+
+
+def _exact_keys(s, seq, n):
+    """K and V of a sequence's first n tokens in 64 bits, [KV][n][128]."""
+    KV, page = s["case"]["kv_heads"], s["case"]["page"]
+    at = torch.from_numpy(s["tables"][seq].cpu().numpy().view(np.uint16).astype(np.int64)).cuda()[:-(-n // page)]
+    deq = lambda x, xs: (x[at].double().view(-1, KV, HD) * xs[at].double().view(-1, KV, 1))[:n].transpose(0, 1).contiguous()  # noqa: E731
+    return deq(s["k"], s["ks"]), deq(s["v"], s["vs"])
+
+
+def _exact_rows(s, i, a, b):
+    KV = s["case"]["kv_heads"]
+    G = s["case"]["heads"] // KV
+    q = s["q8"][a:b].double().view(b - a, KV, G, HD) * s["qs"][a:b].double().view(b - a, KV, G, 1)
+    return q.permute(1, 2, 0, 3).contiguous()  # [KV][G][row][128]
+
+
+def _exact_attention(s):
+    start, kv, out = s["row_start"].tolist(), s["kv_len"].tolist(), []
+    for i in range(len(kv)):
+        n = start[i + 1] - start[i]
+        k, v = _exact_keys(s, i, kv[i])
+        for a in range(start[i], start[i + 1], 512):
+            b = min(a + 512, start[i + 1])
+            pos = kv[i] - n + torch.arange(a - start[i], b - start[i], device="cuda")
+            x = (_exact_rows(s, i, a, b) @ k.transpose(1, 2).contiguous()[:, None]) * QK_SCALE
+            x[..., torch.arange(kv[i], device="cuda")[None] > pos[:, None]] = -math.inf
+            o = torch.softmax(x, -1) @ v[:, None]  # [KV][G][row][128]
+            out.append(o.permute(2, 0, 1, 3).reshape(b - a, -1))
+    return torch.cat(out)
+
+
+def _exact_sparse(s):
+    """Which pages are chosen goes by scores with two f32 roundings, as the
+    operator defines them; what is read there is exact."""
+    c = s["case"]
+    KV, page, n_sel = c["kv_heads"], c["page"], c["select"]
+    G = c["heads"] // KV
+    t = s["tables"].cpu().numpy().view(np.uint16).astype(np.int64)
+    ids, out, have = [], [], {}
+    for i, r, pos in _host_rows(s):
+        if i not in have:
+            have.clear()
+            have[i] = _exact_keys(s, i, int(s["kv_len"][i]))
+            at = torch.from_numpy(t[i]).cuda()
+            have["b"] = s["bounds"].view(-1, KV, 2, HD)[at].double(), s["bscale"][at]
+        (k, v), (b, bs) = have[i], have["b"]
+        last = pos // page
+        q = s["q8"][r].double().view(KV, G, 1, HD)
+        lo, hi = (b[:last + 1, :, j].transpose(0, 1)[:, None] for j in (0, 1))
+        whole = (torch.where(q > 0, hi, lo) * q).sum(-1).float()  # [KV][G][page]
+        score = ((whole * bs[:last + 1].t()[:, None]) * s["qs"][r].view(KV, G, 1)).amax(1)
+        score[:, last] = math.inf
+        pick = torch.argsort(score, dim=-1, descending=True, stable=True)[:, :n_sel].sort(-1).values  # [KV][<= select]
+        row = torch.full((KV, n_sel), -1, device="cuda")
+        row[:, :pick.shape[1]] = pick
+        ids.append(row.flatten())
+        key = (pick[..., None] * page + torch.arange(page, device="cuda")).flatten(1)
+        dead = key > pos
+        key = key.clamp(max=pos)[..., None].expand(-1, -1, HD)
+        qd = (s["q8"][r].double().view(KV, G, HD) * s["qs"][r].double().view(KV, G, 1))
+        x = (qd[:, :, None] * k.gather(1, key)[:, None]).sum(-1) * QK_SCALE
+        p = torch.softmax(x.masked_fill(dead[:, None], -math.inf), -1)
+        out.append((p[..., None] * v.gather(1, key)[:, None]).sum(2).flatten())
+    return torch.stack(ids).to(torch.int32), torch.stack(out)
