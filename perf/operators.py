@@ -222,7 +222,7 @@ def _run_own(s):
                               nwk=s["nk"] if c["norm"] else None, inv_hd=INV_HD, cos=s["cos"], sin=s["sin"], rot_dim=c["rot"],
                               interleaved=c["interleaved"])
         if c["bounds"]:
-            ops.page_bounds(pool, seqs, s["bounds"], s["bscale"])
+            ops.page_bounds(pool, seqs, s["bounds"], s["bscale"], s["rows"])
         return [s[k] for k in ("q8", "qs", "k", "ks", "v", "vs") + (("bounds", "bscale") if c["bounds"] else ())]
     if c["kind"] == "attention":
         ops.attention_varlen_paged(s["q8"], s["qs"], pool, seqs, s["out"], qk_scale=QK_SCALE)
