@@ -239,6 +239,110 @@ int q3_gemm_nt_group_argmax_noalloc(const q3_view *a, const q3_view *a_scale,
 int q3_argmax_logits(const q3_view *logits, int32_t *out_id, void *stream);
 
 /* ------------------------------------------------------------------------ */
+/* Batches of sequences over one paged cache                                */
+/* ------------------------------------------------------------------------ */
+
+/* The operators below serve the new rows of many sequences in one call: one
+ * decoding token, a chunk or a whole prompt each, in any mix.  The reference has
+ * their pieces for one sequence (kernels/norm_rope_quant.h, kernels/kv_pages.h,
+ * kernels/attention_gqa.h).  They share the conventions of the operators above;
+ * head_dim is 128; unlike those they take their tables from q3_seqs, and the
+ * q3_paged_kv's own `table` is not read and may be NULL.
+ *
+ * The rows of sequence s are row_start[s] .. row_start[s + 1] - 1 of the call's
+ * row arrays, its last new row is token kv_len[s] - 1, and tables[s] maps its
+ * logical pages to the pool's.  All three arrays lie on the device and are read
+ * by the kernels alone, so a call may be captured into a graph and replayed on
+ * other lengths, within max_rows and max_kv.  Rows before row_start[0] and from
+ * row_start[n_seq] on are left as they are.  What the arrays may hold wrongly is
+ * clamped: a sequence's rows to max_rows, kv_len to [0, max_kv]; a page id
+ * outside the pool is a page whose keys are never attended to or written.
+ * row_start must not decrease. */
+typedef struct q3_seqs {
+  const int32_t *row_start; /* device [n_seq + 1]                            */
+  const int32_t *kv_len;    /* device [n_seq]: cached tokens, new ones included */
+  const uint16_t *tables;   /* device [n_seq][ld_table]                      */
+  uint32_t n_seq;           /* at most 65535                                 */
+  uint32_t ld_table;        /* logical pages of a table row                  */
+  uint32_t n_pages;         /* pages in the pool                             */
+  uint32_t max_rows;        /* no sequence has more new rows (<= rows)       */
+  uint32_t max_kv;          /* no kv_len is larger (<= ld_table * page_tokens) */
+} q3_seqs;
+
+/* Q, K and V rows of one layer into the cache: per-head RMSNorm of Q and K
+ * (gains nwq / nwk [128], factor inv_hd; NULL: none), rotary positions, int8
+ * quantisation per head; K and V go to the pages of their tokens, Q to q8 / qs.
+ * One f32 operation at a time as q3_norm_rope_quant_heads, and bit-equal to it.
+ * q f32 [rows][heads * 128] (NULL with heads 0: K and V alone), k, v f32
+ * [rows][kv_heads * 128], cos / sin f32 [>= max_kv][rot_dim / 2] indexed by
+ * position.  The first rot_dim columns (even, <= 128) of a head are rotated, as
+ * pairs (i, i + rot_dim / 2), or (2 i, 2 i + 1) if interleaved; rot_dim 0 with
+ * NULL cos / sin: no rotation.  A row whose position would be negative is left
+ * out.  Two sequences must not write the same page. */
+int q3_rope_append_paged(const q3_view *q, const q3_view *k, const q3_view *v,
+                         const q3_view *nwq, const q3_view *nwk, float inv_hd,
+                         const q3_view *cos, const q3_view *sin,
+                         uint32_t rot_dim, int interleaved, const q3_view *q8,
+                         const q3_view *qs, const q3_paged_kv *kv,
+                         const q3_seqs *seqs, int heads, int kv_heads,
+                         void *stream);
+
+/* Channel bounds of the pages that hold the sequences' new rows (rows: the row
+ * count of the call that wrote them), from all of the pages' cached keys: with
+ * lo_d / hi_d the least / largest RN(k_d * ks) of the page and KV head and
+ * b = RN(absmax * RN(1/127)), bounds row [page * kv_heads + head] is
+ * floor(RN(lo / b)) of the 128 channels, then ceil(RN(hi / b)), clamped to
+ * +-127, and bscale [page][head] is b.  A NaN value does not count. */
+int q3_page_bounds(const q3_paged_kv *kv, const q3_seqs *seqs, uint32_t rows,
+                   int kv_heads, const q3_view *bounds, const q3_view *bscale,
+                   void *stream);
+
+/* Attention of every sequence's rows over its cached keys, those at or before
+ * the row's position if causal: softmax(RN-f32 of q . k * ks * (qs * qk_scale))
+ * . (vs * v) with f32 maxima, sums and products (no int8 P, unlike
+ * q3_attention_heads_gqa_tokscale_paged).  A row without any key gets zeros.
+ * The result goes to out f32 [rows][heads * 128], or quantised per head as by
+ * q3_quant_rows_heads to o8 i8 [rows][heads * 128] / os f32 [rows][heads]; the
+ * other form is NULL.  ws: device memory of q3_seqs_workspace's size, 16-byte
+ * aligned, not used by other work until this call's is done. */
+int q3_attention_varlen_paged(const q3_view *q8, const q3_view *q_scale,
+                              const q3_paged_kv *kv, const q3_seqs *seqs,
+                              const q3_view *out, const q3_view *o8,
+                              const q3_view *os, int heads, int kv_heads,
+                              int head_dim, int causal, float qk_scale,
+                              void *ws, uint64_t ws_bytes, void *stream);
+
+/* For each row and KV head the n_sel logical pages, up to the row's own, whose
+ * bounds promise the largest scores: ids i32 [rows][kv_heads * n_sel],
+ * ascending, -1 behind the last.  A page's score is the largest over the KV
+ * head's query heads of RN(RN(f32(sum_d q_d * (q_d > 0 ? hi_d : lo_d)) * b) *
+ * qs), the sum exact; ties go to the lowest page, a NaN counts as the largest, a
+ * page id outside the pool as the least.  The row's own page is always among
+ * them.  heads / kv_heads <= 16. */
+int q3_select_pages(const q3_view *q8, const q3_view *q_scale,
+                    const q3_paged_kv *kv, const q3_seqs *seqs,
+                    const q3_view *bounds, const q3_view *bscale,
+                    const q3_view *ids, uint32_t n_sel, int heads, int kv_heads,
+                    void *ws, uint64_t ws_bytes, void *stream);
+
+/* q3_attention_varlen_paged (causal) over the keys of each row's listed pages
+ * alone.  Ids outside the row's pages are passed over; a page listed twice
+ * counts twice. */
+int q3_attention_pages(const q3_view *q8, const q3_view *q_scale,
+                       const q3_paged_kv *kv, const q3_seqs *seqs,
+                       const q3_view *ids, uint32_t n_sel, const q3_view *out,
+                       const q3_view *o8, const q3_view *os, int heads,
+                       int kv_heads, int head_dim, float qk_scale, void *ws,
+                       uint64_t ws_bytes, void *stream);
+
+/* Bytes of workspace that q3_attention_varlen_paged and, with n_sel > 0,
+ * q3_select_pages and q3_attention_pages need for calls of these sizes: one
+ * buffer serves them all in stream order.  Host only; of seqs the counts and
+ * limits are read, not the arrays. */
+int q3_seqs_workspace(const q3_seqs *seqs, uint32_t rows, uint32_t page_tokens,
+                      int heads, int kv_heads, uint32_t n_sel, uint64_t *bytes);
+
+/* ------------------------------------------------------------------------ */
 /* Blob layout (tools/pqwf.py:95-273) and random-init writer                */
 /* ------------------------------------------------------------------------ */
 

@@ -1,0 +1,148 @@
+// The operators on the rows of many sequences over one pool of K/V pages
+// (include/q3ops.h, "Batches of sequences"): kernel arguments, the lookups that
+// their kernels share, and the launchers.
+//
+// Row starts, lengths and page tables are read on the device, so nothing on the
+// host vouches for them.  Every lookup below clamps what it reads: a start or a
+// length to what the host was told, a page id to the pool.  Whatever the arrays
+// hold, no kernel reads or writes outside its operands.
+#pragma once
+
+#include "q3_device.h"
+
+namespace q3 {
+
+// The pool (q3_paged_kv without its table), strides in elements.
+struct Pool {
+  int8_t *k, *v;
+  float *ks, *vs;
+  int64_t page_bytes, row_bytes;    // of K and V rows
+  int64_t spage, srow;              // of their scales, in floats
+  int page_tokens, n_pages;
+};
+
+// q3_seqs with the call's row count.
+struct Seqs {
+  const int32_t *start, *kv_len;
+  const uint16_t *tables;
+  int64_t ld_table;
+  int n_seq, rows, max_rows, max_kv;
+};
+
+#if defined(__HIPCC__)
+
+// A sequence's rows [r0, r0 + n) and its cached keys.
+struct SeqSpan {
+  int r0, n, kv;
+  __device__ int pos(int row) const { return kv - n + (row - r0); }
+};
+
+__device__ __forceinline__ int clampi(int x, int lo, int hi) { return max(lo, min(x, hi)); }
+
+__device__ __forceinline__ SeqSpan seq_span(const Seqs &q, int s) {
+  SeqSpan o;
+  o.r0 = clampi(q.start[s], 0, q.rows);
+  o.n = clampi(clampi(q.start[s + 1], 0, q.rows) - o.r0, 0, q.max_rows);
+  o.kv = clampi(q.kv_len[s], 0, q.max_kv);
+  return o;
+}
+
+// The sequence that holds a wave-uniform row: as many sequences end at or
+// before it (64 ends a step, one per lane).  n_seq: behind the last one.
+__device__ __forceinline__ int seq_of_row(const Seqs &q, int row) {
+  const int lane = threadIdx.x & 63;
+  int s = 0;
+#pragma unroll 4
+  for (int b = 0; b < q.n_seq; b += 64) {
+    const int j = b + lane;
+    const bool before = j < q.n_seq && q.start[min(j, q.n_seq - 1) + 1] <= row;
+    s += __popcll(__ballot(before));
+  }
+  return s;
+}
+
+// Physical page of a sequence's logical page (0 <= logical * page_tokens <
+// max_kv), -1 if the table names none of the pool's.
+__device__ __forceinline__ int seq_page(const Seqs &q, const Pool &p, int s, int logical) {
+  const int id = q.tables[s * q.ld_table + logical];
+  return id < p.n_pages ? id : -1;
+}
+
+#endif  // __HIPCC__
+
+// ---- new rows into the cache (k_seq_append.hip) ------------------------------
+struct SeqAppendArgs {
+  const float *q, *k, *v;
+  int64_t ldq, ldk, ldv;
+  const float *nwq, *nwk;  // per-head norm gains (null: no norm)
+  int64_t nwq_stride, nwk_stride;
+  float inv_hd;
+  const float *cos_t, *sin_t;  // [position][rot / 2]
+  int64_t ld_cs;
+  int rot, interleaved;
+  int8_t *q8;
+  int64_t ldq8;
+  float *qs;
+  int64_t ldqs, qs_col;
+  int heads, kv_heads;
+  Pool pool;
+  Seqs seqs;
+};
+hipError_t launch_seq_append(const SeqAppendArgs &a, hipStream_t s);
+
+struct PageBoundsArgs {
+  int8_t *bounds;  // [page * kv_heads + head][256]: least, then largest
+  int64_t ldb;
+  float *scale;    // [page][head]
+  int64_t lds;
+  int kv_heads;
+  Pool pool;
+  Seqs seqs;
+};
+hipError_t launch_page_bounds(const PageBoundsArgs &a, hipStream_t s);
+
+// ---- attention (k_seq_attn.hip) ----------------------------------------------
+struct SeqAttnArgs {
+  const int8_t *q8;
+  int64_t ldq;
+  const float *qs;
+  int64_t ldqs, qs_col;
+  int heads, kv_heads, causal;
+  float qk_scale;
+  const int32_t *ids;  // [row][kv_heads * n_sel] logical pages; null: all keys
+  int64_t ld_ids;
+  int n_sel;
+  float *out;          // f32 rows, or
+  int64_t ldo;
+  int8_t *o8;          // int8 rows with one scale per head
+  int64_t ldo8;
+  float *os;
+  int64_t ldos, os_col;
+  void *ws;
+  Pool pool;
+  Seqs seqs;
+};
+uint64_t seq_attn_ws_bytes(const SeqAttnArgs &a);
+hipError_t launch_seq_attn(const SeqAttnArgs &a, hipStream_t s);
+
+// ---- page selection (k_seq_select.hip) ----------------------------------------
+struct SelectArgs {
+  const int8_t *q8;
+  int64_t ldq;
+  const float *qs;
+  int64_t ldqs, qs_col;
+  const int8_t *bounds;
+  int64_t ldb;
+  const float *scale;
+  int64_t lds;
+  int heads, kv_heads, n_sel;
+  int32_t *ids;
+  int64_t ld_ids;
+  uint32_t *keys;  // workspace: [row * kv_heads + head][ld_keys]
+  int64_t ld_keys;
+  Pool pool;
+  Seqs seqs;
+};
+hipError_t launch_select_pages(const SelectArgs &a, hipStream_t s);
+
+}  // namespace q3

@@ -43,6 +43,13 @@ class PagedKV(C.Structure):
                 ("scale_row_bytes", C.c_uint32)]
 
 
+class Seqs(C.Structure):
+    """q3_seqs: the new rows, lengths and page tables of a batch of sequences."""
+    _fields_ = [("row_start", C.c_void_p), ("kv_len", C.c_void_p), ("tables", C.c_void_p),
+                ("n_seq", C.c_uint32), ("ld_table", C.c_uint32), ("n_pages", C.c_uint32),
+                ("max_rows", C.c_uint32), ("max_kv", C.c_uint32)]
+
+
 LAYOUT_DIMS = ["hidden", "layers", "heads", "kv_heads", "head_dim", "inter", "vocab", "seq",
                "max_seq", "half"]
 LAYOUT_OFFSETS = [
@@ -73,6 +80,8 @@ class InitParams(C.Structure):
 _VP, _I, _U, _F = C.c_void_p, C.c_int, C.c_uint32, C.c_float
 _PV = C.POINTER(View)
 _PK = C.POINTER(PagedKV)
+_PS = C.POINTER(Seqs)
+_U64 = C.c_uint64
 SIGNATURES = {
     "q3_set_silent_unsupported": (_I, [_I]),
     "q3_status_str": (C.c_char_p, [_I]),
@@ -90,6 +99,15 @@ SIGNATURES = {
     "q3_gemm_nt_group_argmax": (_I, [_PV, _PV, _PV, _PV, _PV, _PV, _U, _VP]),
     "q3_gemm_nt_group_argmax_noalloc": (_I, [_PV, _PV, _PV, _PV, _PV, _PV, _U, _VP]),
     "q3_argmax_logits": (_I, [_PV, _VP, _VP]),
+    "q3_rope_append_paged": (_I, [_PV, _PV, _PV, _PV, _PV, _F, _PV, _PV, _U, _I, _PV, _PV, _PK, _PS,
+                                  _I, _I, _VP]),
+    "q3_page_bounds": (_I, [_PK, _PS, _U, _I, _PV, _PV, _VP]),
+    "q3_attention_varlen_paged": (_I, [_PV, _PV, _PK, _PS, _PV, _PV, _PV, _I, _I, _I, _I, _F, _VP,
+                                       _U64, _VP]),
+    "q3_select_pages": (_I, [_PV, _PV, _PK, _PS, _PV, _PV, _PV, _U, _I, _I, _VP, _U64, _VP]),
+    "q3_attention_pages": (_I, [_PV, _PV, _PK, _PS, _PV, _U, _PV, _PV, _PV, _I, _I, _I, _F, _VP,
+                                _U64, _VP]),
+    "q3_seqs_workspace": (_I, [_PS, _U, _U, _I, _I, _U, C.POINTER(C.c_uint64)]),
     "q3_layout_compute": (_I, [_U] * 9 + [C.POINTER(CLayout)]),
     "q3_layout_header_text": (_I, [C.POINTER(CLayout), C.c_char_p, C.c_size_t]),
     "q3_init_random_blob": (_I, [C.POINTER(CLayout), C.POINTER(InitParams), _VP, _I]),

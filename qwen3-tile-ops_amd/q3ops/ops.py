@@ -15,7 +15,7 @@ from ctypes import byref
 
 import torch
 
-from ._lib import DT_F32, DT_I8, DT_I32, LM_ARGMAX, PagedKV, View, check, lib
+from ._lib import DT_F32, DT_I8, DT_I32, LM_ARGMAX, PagedKV, Q3Error, Seqs, View, check, lib
 
 # element size and dtype code of the view dtypes
 _DT = {torch.int8: (1, DT_I8), torch.float32: (4, DT_F32), torch.int32: (4, DT_I32)}
@@ -186,7 +186,155 @@ def argmax_logits(logits, out_id, stream=None):
           "argmax_logits")
 
 
-__all__ = ["view", "paged_kv", "embedding_rmsnorm_rows", "rmsnorm_rows", "quant_rows_heads",
+# ---- batches of sequences over one paged cache ------------------------------
+
+
+def kv_pool(k: torch.Tensor, v: torch.Tensor, ks: torch.Tensor, vs: torch.Tensor) -> PagedKV:
+    """The pool of K/V pages that the batch operators below share: k/v
+    [pages, page_tokens, kv_heads * 128] int8, ks/vs [pages, page_tokens,
+    kv_heads] f32, contiguous.  Unlike paged_kv it holds no table (each call's
+    tables come with its sequences), so making it reads nothing back."""
+    if k.dim() != 3 or ks.dim() != 3 or v.shape != k.shape or vs.shape != ks.shape or ks.shape[:2] != k.shape[:2]:
+        raise ValueError("k/v are [pages, page_tokens, kv_heads * 128], ks/vs [pages, page_tokens, kv_heads]")
+    n_pages, page_tokens, kv_dim = k.shape
+    kv_heads = ks.shape[2]
+    if kv_dim != kv_heads * 128:
+        raise ValueError(f"rows of {kv_dim} columns for {kv_heads} heads of 128")
+    for t, dt in ((k, torch.int8), (v, torch.int8), (ks, torch.float32), (vs, torch.float32)):
+        if t.dtype != dt:
+            raise TypeError(f"unsupported dtype {t.dtype}")
+        if not t.is_contiguous():
+            raise ValueError("the pool's tensors must be contiguous")
+        _on_device(t, k)
+    kv = PagedKV(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), None, page_tokens,
+                 page_tokens * kv_dim, kv_dim, page_tokens * kv_heads * 4, kv_heads * 4)
+    kv._keep = (k, v, ks, vs)
+    kv.n_pages, kv.kv_heads, kv.device = n_pages, kv_heads, k.device
+    return kv
+
+
+def sequences(pool: PagedKV, tables, row_start, kv_len, max_rows: int, max_kv: int) -> Seqs:
+    """The batch of one call (q3_seqs): tables [n_seq, pages] int16/uint16
+    logical -> physical pages, row_start [n_seq + 1] and kv_len [n_seq] int32, on
+    the pool's device; max_rows and max_kv are the host's limits of the new rows
+    and of the cached tokens of a sequence.  The arrays' contents may change
+    between calls (or replays of a captured one) within these limits."""
+    if tables.dtype not in (torch.int16, torch.uint16) or row_start.dtype != torch.int32 or kv_len.dtype != torch.int32:
+        raise TypeError("tables are int16 or uint16, row_start and kv_len int32")
+    n_seq = kv_len.shape[0]
+    if kv_len.dim() != 1 or tables.dim() != 2 or tables.shape[0] != n_seq or row_start.shape != (n_seq + 1,):
+        raise ValueError("tables are [n_seq, pages], row_start [n_seq + 1], kv_len [n_seq]")
+    for t in (tables, row_start, kv_len):
+        if not t.is_contiguous():
+            raise ValueError("tables, row_start and kv_len must be contiguous")
+        _on_device(t, pool)
+    s = Seqs(row_start.data_ptr(), kv_len.data_ptr(), tables.data_ptr(), n_seq, tables.shape[1],
+             pool.n_pages, max_rows, max_kv)
+    s._keep = (tables, row_start, kv_len)
+    return s
+
+
+def _on_device(t, like) -> None:
+    if not t.is_cuda:
+        raise ValueError("operator views must point at device memory")
+    if t.device != like.device:
+        raise ValueError(f"tensors on {t.device} and {like.device}")
+
+
+def _launch_stream(pool: PagedKV, stream, *tensors) -> int:
+    """The stream of a call on the pool's device, which has to be the current
+    one (kernels launch there) and to hold every tensor."""
+    dev = pool.device
+    if dev.index != torch.cuda.current_device():
+        raise ValueError(f"the pool is on {dev}, the current device is cuda:{torch.cuda.current_device()}")
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors on {t.device} and {dev}")
+    if stream is not None and stream.device != dev:
+        raise ValueError(f"a stream of {stream.device} for a pool on {dev}")
+    return _stream(stream)
+
+
+def rope_append_paged(q, k, v, pool: PagedKV, seqs: Seqs, q8=None, qs=None, nwq=None, nwk=None, inv_hd=0.0,
+                      cos=None, sin=None, rot_dim=128, interleaved=False, stream=None):
+    """q3_rope_append_paged: new Q/K/V rows (f32 [rows, heads * 128]) of every
+    sequence, normed (gains nwq / nwk), rotated at their positions (cos / sin
+    [position, rot_dim / 2], e.g. rope_tables'; None: not rotated), quantised; K
+    and V into their pages, Q into q8 / qs (q None: K and V alone)."""
+    check(lib().q3_rope_append_paged(view(q), view(k), view(v), view(nwq), view(nwk), inv_hd, view(cos), view(sin),
+                                     rot_dim if cos is not None else 0, int(interleaved), view(q8), view(qs),
+                                     byref(pool), byref(seqs), 0 if q is None else q.shape[1] // 128, pool.kv_heads,
+                                     _launch_stream(pool, stream, q, k, v, nwq, nwk, cos, sin, q8, qs)),
+          "rope_append_paged")
+
+
+def page_bounds(pool: PagedKV, seqs: Seqs, bounds, bscale, rows: int | None = None, stream=None):
+    """q3_page_bounds: channel bounds (int8 [pages * kv_heads, 256], least then
+    largest; f32 [pages, kv_heads]) of the pages that the sequences' new rows lie
+    in (rows: the call's row count, n_seq * max_rows if not given)."""
+    rows = seqs.n_seq * seqs.max_rows if rows is None else rows
+    check(lib().q3_page_bounds(byref(pool), byref(seqs), rows, pool.kv_heads, view(bounds), view(bscale),
+                               _launch_stream(pool, stream, bounds, bscale)), "page_bounds")
+
+
+def seqs_workspace_bytes(pool: PagedKV, seqs: Seqs, rows: int, heads: int, n_sel: int = 0) -> int:
+    """q3_seqs_workspace: bytes for attention_varlen_paged and, with n_sel,
+    select_pages and attention_pages on these sizes."""
+    n = C.c_uint64()
+    check(lib().q3_seqs_workspace(byref(seqs), rows, pool.page_tokens, heads, pool.kv_heads, n_sel, byref(n)),
+          "seqs_workspace")
+    return n.value
+
+
+def _workspace_on(ws, stream, pool, seqs, q8, n_sel):
+    """The caller's workspace tensor, or a new one (torch's allocator hands its
+    memory out again in the order of the current stream)."""
+    if ws is None:
+        n = seqs_workspace_bytes(pool, seqs, q8.shape[0], q8.shape[1] // 128, n_sel)
+        if n and stream is not None and stream != torch.cuda.current_stream(pool.device):
+            raise ValueError("a call on a stream that is not the current one needs its workspace given")
+        ws = torch.empty(n, dtype=torch.uint8, device=pool.device) if n else None
+    elif not ws.is_contiguous():
+        raise ValueError("the workspace must be contiguous")
+    return (ws, None, 0) if ws is None else (ws, ws.data_ptr(), ws.numel() * ws.element_size())
+
+
+def attention_varlen_paged(q8, q_scale, pool: PagedKV, seqs: Seqs, out=None, o8=None, os=None, causal=True,
+                           qk_scale=128 ** -0.5, workspace=None, stream=None):
+    """q3_attention_varlen_paged: attention of every sequence's rows over its
+    cached keys; the result in f32 (out) or int8 with a scale per head (o8, os).
+    workspace: a device tensor of seqs_workspace_bytes, needed on a stream that
+    is not the current one; otherwise one is allocated."""
+    st = _launch_stream(pool, stream, q8, q_scale, out, o8, os, workspace)
+    keep, ws, n = _workspace_on(workspace, stream, pool, seqs, q8, 0)
+    check(lib().q3_attention_varlen_paged(view(q8), view(q_scale), byref(pool), byref(seqs), view(out), view(o8),
+                                          view(os), q8.shape[1] // 128, pool.kv_heads, 128, int(causal), qk_scale,
+                                          ws, n, st), "attention_varlen_paged")
+
+
+def select_pages(q8, q_scale, pool: PagedKV, seqs: Seqs, bounds, bscale, ids, n_sel, workspace=None, stream=None):
+    """q3_select_pages: the n_sel pages of each row and KV head with the largest
+    bounds of a score, into ids (int32 [rows, kv_heads * n_sel])."""
+    st = _launch_stream(pool, stream, q8, q_scale, bounds, bscale, ids, workspace)
+    keep, ws, n = _workspace_on(workspace, stream, pool, seqs, q8, n_sel)
+    check(lib().q3_select_pages(view(q8), view(q_scale), byref(pool), byref(seqs), view(bounds), view(bscale),
+                                view(ids), n_sel, q8.shape[1] // 128, pool.kv_heads, ws, n, st), "select_pages")
+
+
+def attention_pages(q8, q_scale, pool: PagedKV, seqs: Seqs, ids, n_sel, out=None, o8=None, os=None,
+                    qk_scale=128 ** -0.5, workspace=None, stream=None):
+    """q3_attention_pages: attention_varlen_paged over the keys of each row's
+    listed pages (select_pages' ids, or the caller's own)."""
+    st = _launch_stream(pool, stream, q8, q_scale, ids, out, o8, os, workspace)
+    keep, ws, n = _workspace_on(workspace, stream, pool, seqs, q8, n_sel)
+    check(lib().q3_attention_pages(view(q8), view(q_scale), byref(pool), byref(seqs), view(ids), n_sel, view(out),
+                                   view(o8), view(os), q8.shape[1] // 128, pool.kv_heads, 128, qk_scale, ws, n, st),
+          "attention_pages")
+
+
+__all__ = ["Q3Error", "view", "paged_kv", "embedding_rmsnorm_rows", "rmsnorm_rows", "quant_rows_heads",
            "gemm_nt_group_store", "gemm_nt_group_kv_paged", "norm_rope_quant_heads",
            "attention_heads_gqa_tokscale_paged", "gemm_gate_up_swiglu_quant",
-           "gemm_nt_group_argmax", "gemm_nt_group_argmax_noalloc", "argmax_logits", "LM_ARGMAX"]
+           "gemm_nt_group_argmax", "gemm_nt_group_argmax_noalloc", "argmax_logits", "LM_ARGMAX",
+           "kv_pool", "sequences", "rope_append_paged", "page_bounds", "seqs_workspace_bytes",
+           "attention_varlen_paged", "select_pages", "attention_pages"]

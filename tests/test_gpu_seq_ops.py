@@ -1,0 +1,582 @@
+"""The batch operators over one paged cache against their plain forms."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import seqref
+from conftest import bits_equal, describe_diff
+from seqref import F, Batch, attend, attend_bound, quantise, queries
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+from q3ops import ops  # noqa: E402
+from q3ops.rope import rope_tables  # noqa: E402
+
+QK = float(F(128 ** -0.5))
+
+
+def dev(a):
+    a = np.ascontiguousarray(a)
+    return torch.from_numpy(a.view(np.int16) if a.dtype == np.uint16 else a).cuda()
+
+
+def on_device(b: Batch, max_rows=None, max_kv=None):
+    kv = b.kv_heads
+    pool = ops.kv_pool(dev(b.k.reshape(b.n_pages, b.page, kv * 128)), dev(b.v.reshape(b.n_pages, b.page, kv * 128)),
+                       dev(b.ks), dev(b.vs))
+    seqs = ops.sequences(pool, dev(b.tables), dev(b.start), dev(b.kv_len), b.max_rows if max_rows is None else max_rows,
+                         b.max_kv if max_kv is None else max_kv)
+    return pool, seqs
+
+
+def check_attention(b, heads, causal=True, ids=None, n_sel=0, seed=1):
+    rng = np.random.default_rng(seed)
+    q8, qs = queries(rng, b.rows, heads)
+    pool, seqs = on_device(b)
+    tq, ts = dev(q8), dev(qs)
+    out = torch.full((b.rows, heads * 128), 7.5, device="cuda")
+    o8 = torch.full((b.rows, heads * 128), 99, dtype=torch.int8, device="cuda")
+    os_ = torch.full((b.rows, heads), 7.5, device="cuda")
+    if ids is None:
+        call = lambda **kw: ops.attention_varlen_paged(tq, ts, pool, seqs, causal=causal, qk_scale=QK, **kw)  # noqa: E731
+    else:
+        ti = dev(ids)
+        call = lambda **kw: ops.attention_pages(tq, ts, pool, seqs, ti, n_sel, qk_scale=QK, **kw)  # noqa: E731
+    call(out=out)
+    call(o8=o8, os=os_)
+    got = out.cpu().numpy()
+    want, mag, top = attend(b, q8, qs, heads, QK, causal, ids, n_sel)
+    mine = np.zeros(b.rows, bool)
+    mine[[r for r, _, _ in b.row_positions()]] = True
+    assert (got[~mine] == 7.5).all() and (o8.cpu().numpy()[~mine] == 99).all() and (os_.cpu().numpy()[~mine] == 7.5).all()
+    err, bound = np.abs(got - want)[mine], attend_bound(mag, top, max(b.max_kv, n_sel * b.page))[mine]
+    assert np.isfinite(got).all()
+    assert (err <= bound).all(), (float((err / bound).max()), np.argwhere(err > bound)[:4].tolist())
+    r8, rs = quantise(got[mine])  # the int8 form rounds the f32 form's values
+    assert bits_equal(os_.cpu().numpy()[mine], rs), describe_diff(os_.cpu().numpy()[mine], rs)
+    assert bits_equal(o8.cpu().numpy()[mine], r8), describe_diff(o8.cpu().numpy()[mine], r8)
+    again = torch.empty_like(out)
+    call(out=again)
+    assert torch.equal(again[dev(mine)], out[dev(mine)])
+
+
+LENS = {
+    "one": [(1, 0)],
+    "two_keys": [(1, 1)],
+    "page_edges": [(1, 31), (1, 32), (1, 33), (1, 63), (1, 64)],
+    "decode": [(1, 700), (1, 5), (1, 1300), (1, 95), (1, 0)],
+    "prompt": [(97, 0)],
+    "chunks": [(3, 40), (33, 100), (64, 64), (130, 17)],
+    "empty_ones": [(0, 50), (1, 20), (0, 0), (5, 3), (0, 9)],
+    "none_before": [(4, -2), (3, -3), (2, 10), (40, -38)],  # rows at negative positions see nothing
+    "long": [(2, 3000), (1, 4500)],
+}
+
+
+@pytest.mark.parametrize("lens", LENS)
+@pytest.mark.parametrize("heads,kv_heads,page", [(16, 8, 32), (6, 2, 96)])
+def test_attention(cuda, lens, heads, kv_heads, page):
+    check_attention(Batch(LENS[lens], kv_heads, page, seed=len(lens)), heads)
+
+
+@pytest.mark.parametrize("heads,kv_heads,page", [(8, 8, 64), (20, 4, 32), (16, 1, 128), (33, 1, 32), (64, 2, 256), (24, 2, 32)])
+@pytest.mark.parametrize("lens", ["decode", "chunks"])
+def test_attention_head_layouts(cuda, heads, kv_heads, page, lens):
+    check_attention(Batch(LENS[lens], kv_heads, page, seed=heads), heads)
+
+
+@pytest.mark.parametrize("lens", ["decode", "chunks", "empty_ones", "none_before", "prompt"])
+def test_attention_not_causal(cuda, lens):
+    check_attention(Batch(LENS[lens], 4, 32, seed=5), 8, causal=False)
+
+
+def test_attention_rows_around_the_sequences(cuda):
+    check_attention(Batch([(3, 100), (1, 50), (40, 8)], 8, 32, before=5, behind=9), 16)
+    check_attention(Batch([(1, 100), (1, 50)], 8, 32, before=2, behind=3), 16)
+
+
+@pytest.mark.parametrize("rows", [1, 70])
+def test_attention_bad_pages(cuda, rows):
+    """A page id outside the pool hides its keys, whichever it is."""
+    b = Batch([(rows, 500), (rows, 300)], 2, 32, seed=rows)
+    b.tables[0, [0, 3, 9]] = [b.n_pages, 65535, b.n_pages + 7]
+    b.tables[1, :4] = 65535
+    check_attention(b, 4)
+
+
+def test_attention_every_page_bad(cuda):
+    b = Batch([(1, 200), (40, 200)], 2, 32)
+    b.tables[:] = 65535
+    check_attention(b, 4)
+
+
+@pytest.mark.parametrize("rows", [1, 70])
+def test_attention_bad_lengths(cuda, rows):
+    """Lengths and starts that no caller should hand over stay in bounds: every
+    row of the sequences that are right is right, nothing else is written behind
+    the last start."""
+    b = Batch([(rows, 100), (rows, 200)], 2, 32, behind=4)
+    q8, qs = queries(b.rng, b.rows, 4)
+    want, mag, top = attend(b, q8, qs, 4, QK)
+    pool, _ = on_device(b)
+    kv_len = b.kv_len.copy()
+    for wrong in (1 << 30, 2147483647, -5, -2147483648):
+        kv_len[0] = wrong
+        seqs = ops.sequences(pool, dev(b.tables), dev(b.start), dev(kv_len), b.max_rows, b.max_kv)
+        out = torch.full((b.rows, 512), 7.5, device="cuda")
+        ops.attention_varlen_paged(dev(q8), dev(qs), pool, seqs, out, qk_scale=QK)
+        got = out.cpu().numpy()
+        assert (np.abs(got - want) <= attend_bound(mag, top, b.max_kv))[rows:2 * rows].all()
+        assert (got[2 * rows:] == 7.5).all()
+    for start in ([0, rows, 1 << 30], [-7, rows, 2 * rows], [-2147483648, 2147483647, 2 * rows], [2 * rows, rows, 0]):
+        seqs = ops.sequences(pool, dev(b.tables), dev(np.array(start, np.int32)), dev(b.kv_len), b.max_rows, b.max_kv)
+        out = torch.full((b.rows + 8, 512), 7.5, device="cuda")
+        ops.attention_varlen_paged(dev(q8), dev(qs), pool, seqs, out, qk_scale=QK)
+        assert (out.cpu().numpy()[b.rows:] == 7.5).all()
+
+
+def test_attention_scales(cuda):
+    """Query scales of zero and below zero; one key scale that outweighs the rest;
+    subnormal and large V scales."""
+    b = Batch([(1, 300), (37, 90)], 2, 32, seed=3)
+    s = b.rng.integers(0, b.n_pages, 5)
+    b.ks[s, 3] *= 40
+    for i in range(2):
+        t = np.arange(int(b.kv_len[i]))
+        at = b.tables[i, t // 32], t % 32
+        b.vs[at] *= np.where(t % 7 == 0, F(1e-38), np.where(t % 7 == 1, F(1e30), F(1)))[:, None].astype(F)
+    q8, qs = queries(b.rng, b.rows, 4)
+    qs[::3] = 0
+    qs[1::3] *= -1
+    want, mag, top = attend(b, q8, qs, 4, QK)
+    pool, seqs = on_device(b)
+    out = torch.empty((b.rows, 512), device="cuda")
+    ops.attention_varlen_paged(dev(q8), dev(qs), pool, seqs, out, qk_scale=QK)
+    got = out.cpu().numpy()
+    err, bound = np.abs(got - want), attend_bound(mag, top, b.max_kv)
+    assert (err <= bound).all(), float((err / bound).max())
+
+
+def test_attention_strided(cuda):
+    """Query and result rows inside wider ones."""
+    b = Batch([(5, 60), (1, 700), (50, 0)], 2, 32, seed=4)
+    q8, qs = queries(b.rng, b.rows, 4)
+    want, mag, top = attend(b, q8, qs, 4, QK)
+    pool, seqs = on_device(b)
+    wq = torch.zeros((b.rows, 4 * 128 + 48), dtype=torch.int8, device="cuda")
+    wq[:, 16:16 + 512] = dev(q8)
+    ws = torch.zeros((b.rows, 9), device="cuda")
+    ws[:, 2:6] = dev(qs)
+    wo = torch.full((b.rows, 512 + 7), 7.5, device="cuda")
+    ops.attention_varlen_paged(wq[:, 16:528], ws[:, 2:6], pool, seqs, wo[:, 3:515], qk_scale=QK)
+    got = wo.cpu().numpy()
+    assert (np.abs(got[:, 3:515] - want) <= attend_bound(mag, top, b.max_kv)).all()
+    assert (got[:, :3] == 7.5).all() and (got[:, 515:] == 7.5).all()
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_attention_far_pages(cuda, rows):
+    """Pages whose bytes lie behind 2^32 of a long cache."""
+    n_pages, page, kvh = 20000, 256, 8
+    b = Batch([(rows, 700)], kvh, page, seed=6)
+    k = torch.empty((n_pages, page, kvh * 128), dtype=torch.int8, device="cuda")
+    v = torch.empty_like(k)
+    ks = torch.empty((n_pages, page, kvh), device="cuda")
+    vs = torch.empty_like(ks)
+    far = n_pages - b.n_pages
+    k[far:], v[far:] = dev(b.k).view(b.n_pages, page, -1), dev(b.v).view(b.n_pages, page, -1)
+    ks[far:], vs[far:] = dev(b.ks), dev(b.vs)
+    pool = ops.kv_pool(k, v, ks, vs)
+    seqs = ops.sequences(pool, dev((b.tables.astype(np.int64) + far).astype(np.uint16)), dev(b.start), dev(b.kv_len),
+                         b.max_rows, b.max_kv)
+    q8, qs = queries(b.rng, b.rows, 16)
+    out = torch.empty((b.rows, 2048), device="cuda")
+    ops.attention_varlen_paged(dev(q8), dev(qs), pool, seqs, out, qk_scale=QK)
+    want, mag, top = attend(b, q8, qs, 16, QK)
+    assert (np.abs(out.cpu().numpy() - want) <= attend_bound(mag, top, b.max_kv)).all()
+    x = torch.randn((b.rows, 3 * 1024), device="cuda")
+    ops.rope_append_paged(None, x[:, :1024], x[:, 1024:2048], pool, seqs)
+    r8, rs = quantise(x[:, :1024].cpu().numpy())
+    pos = b.kv_len[0] - rows + np.arange(rows)
+    p = dev(b.tables[0, pos // page].astype(np.int64) + far)
+    assert bits_equal(k[p, dev(pos % page)].cpu().numpy(), r8) and bits_equal(ks[p, dev(pos % page)].cpu().numpy(), rs)
+
+
+@pytest.mark.parametrize("heads,kv_heads,page,n_sel", [(16, 8, 32, 4), (6, 2, 96, 1), (16, 1, 32, 7), (64, 2, 64, 40), (33, 1, 32, 5)])
+def test_attention_pages(cuda, heads, kv_heads, page, n_sel):
+    """Listed pages in any order; ids that name none of the row's pages are passed
+    over, a page listed twice counts twice; rows with no page at all."""
+    b = Batch([(1, 900), (7, 300), (1, 0), (20, 1500), (3, -2)], kv_heads, page, seed=heads, before=1, behind=2)
+    ids = b.rng.integers(-2, b.tables.shape[1] + 2, (b.rows, kv_heads * n_sel)).astype(np.int32)
+    ids[3] = -1
+    ids[5, :] = ids[5, 0]
+    ids[6, ::2] = 2147483647
+    ids[7, ::2] = -2147483648
+    check_attention(b, heads, ids=ids, n_sel=n_sel)
+
+
+# ---- appending ----------------------------------------------------------------
+
+
+def append_case(b, heads, rot, interleaved, norm, fused=True, seed=0):
+    """Runs the append and its plain form; returns what the device holds."""
+    rng, kvh = np.random.default_rng(seed), b.kv_heads
+    x = rng.standard_normal((b.rows, (heads + 2 * kvh) * 128 + 1)).astype(F)
+    x[0, :128] = 0
+    off = 0 if fused else 1  # 1: rows that no 16-byte word fits
+    tx = dev(x)[:, off:off + (heads + 2 * kvh) * 128]
+    xn = x[:, off:off + (heads + 2 * kvh) * 128]
+    if fused:
+        tx = tx.contiguous()
+    q, k, v = tx[:, :heads * 128], tx[:, heads * 128:(heads + kvh) * 128], tx[:, (heads + kvh) * 128:]
+    nw = [(1 + 0.1 * rng.standard_normal(128)).astype(F) for _ in range(2)]
+    cos, sin = rope_tables(max(b.max_kv, 1), rot) if rot else (None, None)
+    pool, seqs = on_device(b)
+    q8 = torch.full((b.rows, heads * 128), 99, dtype=torch.int8, device="cuda")
+    qs = torch.full((b.rows, heads), 7.5, device="cuda")
+    ops.rope_append_paged(q, k, v, pool, seqs, q8, qs, nwq=dev(nw[0]) if norm else None, nwk=dev(nw[1]) if norm else None,
+                          inv_hd=1 / 128, cos=dev(cos) if rot else None, sin=dev(sin) if rot else None, rot_dim=rot,
+                          interleaved=interleaved)
+    want = dict(q8=np.full((b.rows, heads * 128), 99, np.int8), qs=np.full((b.rows, heads), 7.5, F),
+                k=b.k.copy(), ks=b.ks.copy(), v=b.v.copy(), vs=b.vs.copy())
+    for row, s, pos in b.row_positions():
+        if pos < 0:
+            continue
+        r = xn[row].reshape(-1, 128)
+        for name, h0, h1, w in (("q", 0, heads, nw[0]), ("k", heads, heads + kvh, nw[1]), ("v", heads + kvh, heads + 2 * kvh, None)):
+            y = r[h0:h1]
+            if name != "v":
+                y = seqref.head_norm(y, w) if norm else y
+                y = seqref.rotate(y, cos[pos], sin[pos], rot, interleaved) if rot else y
+            y8, ys = quantise(y.reshape(1, -1))
+            if name == "q":
+                want["q8"][row], want["qs"][row] = y8[0], ys[0]
+            elif b.tables[s, pos // b.page] < b.n_pages:
+                at = b.tables[s, pos // b.page], pos % b.page
+                want[name][at], want[name + "s"][at] = y8.reshape(-1, 128), ys[0]
+    tk, tv, tks, tvs = pool._keep
+    got = dict(q8=q8, qs=qs, k=tk, ks=tks, v=tv, vs=tvs)
+    for n, t in got.items():
+        g, w = t.cpu().numpy(), want[n]
+        assert bits_equal(g.reshape(w.shape), w), (n, describe_diff(g.reshape(w.shape), w))
+    return pool, seqs, want
+
+
+@pytest.mark.parametrize("lens", ["one", "decode", "chunks", "empty_ones", "none_before", "page_edges"])
+@pytest.mark.parametrize("heads,kv_heads,page", [(16, 8, 32), (5, 3, 96)])
+def test_append(cuda, lens, heads, kv_heads, page):
+    append_case(Batch(LENS[lens], kv_heads, page, seed=2, before=2, behind=3), heads, 128, False, True)
+
+
+@pytest.mark.parametrize("rot", [0, 2, 6, 32, 64, 96, 100, 126, 128])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("fused", [False, True])
+def test_append_rotations(cuda, rot, interleaved, fused):
+    append_case(Batch([(7, 50), (1, 31), (1, 4000)], 2, 32, seed=rot), 4, rot, interleaved, rot % 4 == 0, fused, seed=rot)
+
+
+def test_append_bad_pages(cuda):
+    b = Batch([(40, 20), (1, 64)], 2, 32)
+    b.tables[0, 1] = b.n_pages
+    append_case(b, 4, 128, False, True)
+
+
+def test_append_keys_alone(cuda):
+    b = Batch([(4, 30), (1, 5)], 2, 32)
+    pool, seqs = on_device(b)
+    x = torch.randn((b.rows, 256), device="cuda")
+    ops.rope_append_paged(None, x, x, pool, seqs)
+    r8, rs = quantise(x.cpu().numpy())
+    for row, s, pos in b.row_positions():
+        at = int(b.tables[s, pos // 32]), pos % 32
+        for i in (0, 1):
+            assert bits_equal(pool._keep[i][at].cpu().numpy(), r8[row]) and bits_equal(pool._keep[2 + i][at].cpu().numpy(), rs[row])
+
+
+def test_append_equals_norm_rope_quant_heads(cuda):
+    """Bit for bit what the one-sequence operator gives for the same rows."""
+    b = Batch([(60, 77)], 8, 32)
+    rng = np.random.default_rng(0)
+    x = dev((5 * rng.standard_normal((60, 32 * 128))).astype(F))
+    w = dev((1 + 0.1 * rng.standard_normal(128)).astype(F))
+    cos, sin = (dev(t) for t in rope_tables(b.max_kv))
+    pool, seqs = on_device(b)
+    q8, qs = torch.empty((60, 2048), dtype=torch.int8, device="cuda"), torch.empty((60, 16), device="cuda")
+    ops.rope_append_paged(x[:, :2048], x[:, 2048:3072], x[:, 3072:], pool, seqs, q8, qs, nwq=w, nwk=w, inv_hd=1 / 128, cos=cos, sin=sin)
+    for heads, rows, got, gs in ((16, x[:, :2048], q8, qs), (8, x[:, 2048:3072], None, None)):
+        r8, rs = torch.empty((60, heads * 128), dtype=torch.int8, device="cuda"), torch.empty((60, heads), device="cuda")
+        ops.norm_rope_quant_heads(rows, w, cos[77:], sin[77:], r8, rs, heads, 1 / 128)
+        if got is None:
+            t = np.arange(77, 137)
+            p = dev(b.tables[0, t // 32].astype(np.int64))
+            got, gs = pool._keep[0][p, dev(t % 32)], pool._keep[2][p, dev(t % 32)]
+        assert torch.equal(got, r8) and torch.equal(gs, rs)
+
+
+# ---- page bounds and selection ---------------------------------------------------
+
+
+def bounds_on_host(b):
+    """Bounds of every page of the batch's sequences."""
+    bounds = np.full((b.n_pages * b.kv_heads, 256), 5, np.int8)
+    scale = np.full((b.n_pages, b.kv_heads), 7.5, F)
+    touched = np.zeros(b.n_pages, bool)
+    for s, (n, _) in enumerate(b.lens):
+        kv = int(b.kv_len[s])
+        for i in range(-(-max(kv, 0) // b.page)):
+            p, tokens = int(b.tables[s, i]), min(b.page, kv - i * b.page)
+            if p >= b.n_pages:
+                continue
+            touched[p] = n > 0 and (i + 1) * b.page > kv - n
+            for h in range(b.kv_heads):
+                bounds[p * b.kv_heads + h], scale[p, h] = seqref.bounds_of(b.k[p, :tokens, h], b.ks[p, :tokens, h])
+    return bounds, scale, touched
+
+
+@pytest.mark.parametrize("lens", ["one", "decode", "chunks", "empty_ones", "none_before", "page_edges"])
+@pytest.mark.parametrize("kv_heads,page", [(8, 32), (3, 96), (2, 256)])
+def test_page_bounds(cuda, lens, kv_heads, page):
+    b = Batch(LENS[lens], kv_heads, page, seed=9)
+    want, wscale, touched = bounds_on_host(b)
+    pool, seqs = on_device(b)
+    bounds = torch.full(want.shape, 5, dtype=torch.int8, device="cuda")
+    scale = torch.full(wscale.shape, 7.5, device="cuda")
+    ops.page_bounds(pool, seqs, bounds, scale, b.rows)
+    got, gs = bounds.cpu().numpy().reshape(b.n_pages, -1), scale.cpu().numpy()
+    w = want.reshape(b.n_pages, -1)
+    assert bits_equal(got[touched], w[touched]) and bits_equal(gs[touched], wscale[touched])
+    assert (got[~touched] == 5).all() and (gs[~touched] == 7.5).all()
+
+
+def test_page_bounds_bound_the_scores(cuda):
+    """q . k * qs * ks of every key is at most its page's score, within the f32
+    roundings of the scale (2^-23) and of the score (2^-23)."""
+    b = Batch([(64, 0)], 2, 32, seed=11)
+    pool, seqs = on_device(b)
+    bounds, scale = torch.zeros((b.n_pages * 2, 256), dtype=torch.int8, device="cuda"), torch.zeros((b.n_pages, 2), device="cuda")
+    ops.page_bounds(pool, seqs, bounds, scale, b.rows)
+    bh, sh = bounds.cpu().numpy().astype(np.float64), scale.cpu().numpy().astype(np.float64)
+    q = b.rng.integers(-127, 128, (50, 128)).astype(np.float64)
+    for i in range(2):
+        p = int(b.tables[0, i])
+        for h in range(2):
+            k = b.k[p, :, h].astype(np.float64) * b.ks[p, :, h][:, None].astype(np.float64)
+            lo, hi = bh[p * 2 + h, :128], bh[p * 2 + h, 128:]
+            top = (np.where(q > 0, hi, lo) * q).sum(1) * sh[p, h]
+            room = np.abs(q).sum(1) * 127 * sh[p, h] * 2.0 ** -22
+            assert ((q @ k.T).max(1) <= top + room).all()
+
+
+@pytest.mark.parametrize("heads,kv_heads,page,n_sel", [(16, 8, 32, 4), (6, 2, 96, 1), (16, 1, 32, 7), (32, 2, 64, 33), (20, 4, 32, 20), (2, 2, 32, 300)])
+def test_select_pages(cuda, heads, kv_heads, page, n_sel):
+    b = Batch([(1, 2900), (7, 300), (1, 0), (20, 1500), (3, -2), (0, 40), (1, 5000)], kv_heads, page, seed=heads, before=1, behind=2, smooth=True)
+    b.tables[0, 5] = 65535
+    bounds, scale, _ = bounds_on_host(b)
+    q8, qs = queries(b.rng, b.rows, heads)
+    pool, seqs = on_device(b)
+    ids = torch.full((b.rows, kv_heads * n_sel), -9, dtype=torch.int32, device="cuda")
+    ops.select_pages(dev(q8), dev(qs), pool, seqs, dev(bounds), dev(scale), ids, n_sel)
+    want = seqref.select(b, q8, qs, heads, bounds, scale, n_sel)
+    assert np.array_equal(ids.cpu().numpy(), want), np.argwhere(ids.cpu().numpy() != want)[:5]
+
+
+@pytest.mark.parametrize("n_sel", [1, 2, 17, 255, 256, 257, 300])
+def test_select_ties(cuda, n_sel):
+    """Few distinct scores: equal ones go to the lowest pages, over many waves."""
+    b = Batch([(1, 32 * 300 + 3), (2, 32 * 290)], 2, 32, seed=n_sel)
+    bounds = np.repeat(b.rng.integers(-2, 3, (b.n_pages * 2, 1)), 256, 1).astype(np.int8)
+    scale = np.full((b.n_pages, 2), 0.5, F)
+    q8 = np.ones((b.rows, 4 * 128), np.int8)
+    qs = np.full((b.rows, 4), 0.25, F)
+    qs[1] = 0  # all scores are zeros of either sign
+    pool, seqs = on_device(b)
+    ids = torch.empty((b.rows, 2 * n_sel), dtype=torch.int32, device="cuda")
+    ops.select_pages(dev(q8), dev(qs), pool, seqs, dev(bounds), dev(scale), ids, n_sel)
+    want = seqref.select(b, q8, qs, 4, bounds, scale, n_sel)
+    assert np.array_equal(ids.cpu().numpy(), want)
+
+
+def test_select_extremes(cuda):
+    """Scores of the int8 limits (-128 included), NaN scales first of all, -inf last."""
+    b = Batch([(1, 32 * 40)], 1, 32, seed=1)
+    bounds = b.rng.integers(-128, 128, (b.n_pages, 256)).astype(np.int8)
+    scale = b.rng.uniform(0.1, 1, (b.n_pages, 1)).astype(F)
+    t = b.tables[0]
+    scale[t[7]] = np.nan
+    scale[t[9]] = -np.inf
+    bounds[t[9], 128:] = 127
+    q8 = np.full((1, 256), -128, np.int8)
+    q8[0, 128:] = 127
+    qs = np.ones((1, 2), F)
+    pool, seqs = on_device(b)
+    ids = torch.empty((1, 40), dtype=torch.int32, device="cuda")
+    ops.select_pages(dev(q8), dev(qs), pool, seqs, dev(bounds), dev(scale), ids, 2)
+    assert ids[0, :2].tolist() == [7, 40]
+    scale[t[7]] = 0.5
+    scale[t[9]] = 0.0
+    ids.fill_(-9)
+    ops.select_pages(dev(q8), dev(qs), pool, seqs, dev(bounds), dev(scale), ids, 40)
+    assert np.array_equal(ids.cpu().numpy(), seqref.select(b, q8, qs, 2, bounds, scale, 40))
+
+
+# ---- together --------------------------------------------------------------------
+
+
+def test_steps_together(cuda):
+    """Prompt chunks, then decoding steps: each step's rows appended, their pages'
+    bounds refreshed, dense attention and attention over chosen pages, all against
+    the plain forms on the cache as it then is."""
+    heads, kvh, page, n_sel = 8, 2, 32, 3
+    b = Batch([(40, 0), (75, 0), (1, 200)], kvh, page, seed=20)
+    b.max_kv += 4
+    b.tables = np.concatenate((b.tables, np.full((3, 1), 65535, np.uint16)), 1)
+    cos, sin = rope_tables(b.max_kv, scaling="yarn", factor=4.0, original=64)
+    rng = np.random.default_rng(0)
+    pool, _ = on_device(b, max_kv=1)
+    tk, tv, tks, tvs = pool._keep
+    bounds = torch.zeros((b.n_pages * kvh, 256), dtype=torch.int8, device="cuda")
+    scale = torch.zeros((b.n_pages, kvh), device="cuda")
+    # the third sequence's old pages
+    old = ops.sequences(pool, dev(b.tables), dev(np.array([0, 0, 0, 200], np.int32)), dev(np.array([0, 0, 200], np.int32)), 200, 200)
+    ops.page_bounds(pool, old, bounds, scale, 200)
+    free = [p for p in range(b.n_pages) if p not in b.tables]
+    for step in range(3):
+        rows = int(b.start[-1])
+        x = rng.standard_normal((rows, (heads + 2 * kvh) * 128)).astype(F)
+        tx = dev(x)
+        seqs = ops.sequences(pool, dev(b.tables), dev(b.start), dev(b.kv_len), max(r for r, _ in b.lens), b.max_kv)
+        q8, qs = torch.empty((rows, heads * 128), dtype=torch.int8, device="cuda"), torch.empty((rows, heads), device="cuda")
+        ops.rope_append_paged(tx[:, :1024], tx[:, 1024:1280], tx[:, 1280:], pool, seqs, q8, qs, cos=dev(cos), sin=dev(sin))
+        ops.page_bounds(pool, seqs, bounds, scale, rows)
+        out, sparse = torch.empty((rows, heads * 128), device="cuda"), torch.empty((rows, heads * 128), device="cuda")
+        ids = torch.empty((rows, kvh * n_sel), dtype=torch.int32, device="cuda")
+        ws = torch.empty(max(16, ops.seqs_workspace_bytes(pool, seqs, rows, heads, n_sel)), dtype=torch.uint8, device="cuda")
+        ops.attention_varlen_paged(q8, qs, pool, seqs, out, qk_scale=QK, workspace=ws)
+        ops.select_pages(q8, qs, pool, seqs, bounds, scale, ids, n_sel, workspace=ws)
+        ops.attention_pages(q8, qs, pool, seqs, ids, n_sel, sparse, qk_scale=QK, workspace=ws)
+        b.k, b.v = (t.cpu().numpy().reshape(b.n_pages, page, kvh, 128) for t in (tk, tv))
+        b.ks, b.vs = tks.cpu().numpy(), tvs.cpu().numpy()
+        hb, hs, _ = bounds_on_host(b)
+        hq, hqs = q8.cpu().numpy(), qs.cpu().numpy()
+        for row, s, pos in b.row_positions():  # the rows that were appended are the ones in the cache
+            y = x[row, 1024:1280].reshape(kvh, 128)
+            r8, rs = quantise(seqref.rotate(y, cos[pos], sin[pos], 128, False).reshape(1, -1))
+            at = b.tables[s, pos // page], pos % page
+            assert bits_equal(b.k[at].reshape(-1), r8[0]) and bits_equal(b.ks[at], rs[0])
+        want, mag, top = attend(b, hq, hqs, heads, QK)
+        assert (np.abs(out.cpu().numpy() - want) <= attend_bound(mag, top, b.max_kv)).all()
+        wids = seqref.select(b, hq, hqs, heads, hb, hs, n_sel)
+        assert np.array_equal(ids.cpu().numpy(), wids)
+        want, mag, top = attend(b, hq, hqs, heads, QK, ids=wids, n_sel=n_sel)
+        assert (np.abs(sparse.cpu().numpy() - want) <= attend_bound(mag, top, b.max_kv)).all()
+        # one decoding token each
+        b.lens = [(1, int(n)) for n in b.kv_len]
+        b.start = np.arange(4, dtype=np.int32)
+        b.kv_len = b.kv_len + 1
+        b.rows = 3
+        for s in range(3):
+            if b.tables[s, (int(b.kv_len[s]) - 1) // page] == 65535:
+                b.tables[s, (int(b.kv_len[s]) - 1) // page] = free.pop()
+
+
+@pytest.mark.parametrize("rows", [1, 33])
+def test_captured_and_replayed(cuda, rows):
+    """A step captured once and replayed on other lengths, tables and rows, with
+    eager calls of the same operators between the replays; two graphs that share
+    a workspace, replayed in turn."""
+    heads, kvh, page, n_sel, n = 8, 4, 32, 4, 3
+    b = Batch([(rows, 500)] * n, kvh, page, seed=30, smooth=True)
+    pool, _ = on_device(b)
+    tk, tv, tks, tvs = pool._keep
+    total, max_kv = n * rows, b.max_kv
+    tables, start, kv_len = dev(b.tables), dev(b.start), dev(b.kv_len)
+    seqs = ops.sequences(pool, tables, start, kv_len, rows, max_kv)
+    hb, hs, _ = bounds_on_host(b)
+    bounds, scale = dev(hb), dev(hs)
+    q8, qs = (dev(t) for t in queries(b.rng, total, heads))
+    ws = torch.empty(max(16, ops.seqs_workspace_bytes(pool, seqs, total, heads, n_sel)), dtype=torch.uint8, device="cuda")
+
+    def step(o, ids, sp, w):
+        ops.attention_varlen_paged(q8, qs, pool, seqs, o, qk_scale=QK, workspace=w)
+        ops.select_pages(q8, qs, pool, seqs, bounds, scale, ids, n_sel, workspace=w)
+        ops.attention_pages(q8, qs, pool, seqs, ids, n_sel, sp, qk_scale=QK, workspace=w)
+
+    new = lambda: (torch.empty((total, heads * 128), device="cuda"),  # noqa: E731
+                   torch.empty((total, kvh * n_sel), dtype=torch.int32, device="cuda"), torch.empty((total, heads * 128), device="cuda"))
+    sets, graphs = [new(), new()], []
+    side = torch.cuda.Stream()
+    for s in sets:
+        g = torch.cuda.CUDAGraph()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.graph(g, stream=side):
+            step(*s, ws)
+        graphs.append(g)
+    for lens in ([(rows, 400)] * n, [(rows, 0), (rows, 90), (rows, 500)], [(0, 40), (rows, 33), (1, 31)], [(rows, 500)] * n):
+        kv_len.copy_(torch.tensor([r + c for r, c in lens], dtype=torch.int32))
+        start.copy_(torch.tensor(np.cumsum([0] + [r for r, _ in lens]).astype(np.int32)))
+        eager = new()
+        for t in (*sets[0], *sets[1], *eager):
+            t.zero_()
+        graphs[0].replay()
+        step(*eager, None)
+        graphs[1].replay()
+        graphs[0].replay()
+        torch.cuda.synchronize()
+        for s in sets:
+            for got, want in zip(s, eager):
+                assert torch.equal(got, want), lens
+
+
+def test_two_streams(cuda):
+    """Calls of one pool on two streams at once, each with its own workspace."""
+    b = Batch([(1, 3000), (40, 100)], 2, 32, seed=40)
+    pool, seqs = on_device(b)
+    q8, qs = (dev(t) for t in queries(b.rng, b.rows, 4))
+    want = torch.empty((b.rows, 512), device="cuda")
+    ops.attention_varlen_paged(q8, qs, pool, seqs, want, qk_scale=QK)
+    n = max(16, ops.seqs_workspace_bytes(pool, seqs, b.rows, 4))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    ws = [torch.empty(n, dtype=torch.uint8, device="cuda") for _ in streams]
+    outs = [[torch.zeros_like(want) for _ in range(5)] for _ in streams]
+    torch.cuda.synchronize()
+    for i in range(5):
+        for st, w, o in zip(streams, ws, outs):
+            ops.attention_varlen_paged(q8, qs, pool, seqs, o[i], qk_scale=QK, workspace=w, stream=st)
+    torch.cuda.synchronize()
+    assert all(torch.equal(t, want) for o in outs for t in o)
+
+
+def test_no_rows(cuda):
+    b = Batch([(0, 40), (0, 0)], 2, 32)
+    pool, seqs = on_device(b)
+    e = lambda *s, dt=torch.float32: torch.empty(s, dtype=dt, device="cuda")  # noqa: E731
+    ops.rope_append_paged(e(0, 512), e(0, 256), e(0, 256), pool, seqs, e(0, 512, dt=torch.int8), e(0, 4))
+    ops.page_bounds(pool, seqs, e(b.n_pages * 2, 256, dt=torch.int8), e(b.n_pages, 2), 0)
+    ops.attention_varlen_paged(e(0, 512, dt=torch.int8), e(0, 4), pool, seqs, e(0, 512))
+    ops.select_pages(e(0, 512, dt=torch.int8), e(0, 4), pool, seqs, e(b.n_pages * 2, 256, dt=torch.int8), e(b.n_pages, 2),
+                     e(0, 8, dt=torch.int32), 4)
+    none = ops.sequences(pool, e(0, 4, dt=torch.int16), torch.zeros(1, dtype=torch.int32, device="cuda"), e(0, dt=torch.int32), 0, 0)
+    out = torch.full((3, 512), 7.5, device="cuda")
+    ops.attention_varlen_paged(e(3, 512, dt=torch.int8), e(3, 4), pool, none, out)
+    assert (out == 7.5).all()
+
+
+def test_refused_on_the_device(cuda):
+    b = Batch([(1, 40)], 2, 32)
+    pool, seqs = on_device(b)
+    q8, qs = (dev(t) for t in queries(b.rng, 1, 4))
+    out = torch.empty((1, 512), device="cuda")
+    with pytest.raises(ValueError):
+        ops.attention_varlen_paged(q8.cpu(), qs, pool, seqs, out)
+    with pytest.raises(ValueError):
+        ops.attention_varlen_paged(q8, qs, pool, seqs, out.t())
+    with pytest.raises(ops.Q3Error):
+        ops.attention_varlen_paged(q8, qs, pool, seqs, out[:, :511])
+    with pytest.raises(ops.Q3Error):
+        ops.attention_varlen_paged(q8, qs, pool, seqs)
+    with pytest.raises(ValueError):
+        ops.kv_pool(*(t[:, :, ::2] for t in pool._keep))
+    with pytest.raises(TypeError):
+        ops.sequences(pool, seqs._keep[0].int(), *seqs._keep[1:], 1, 41)
