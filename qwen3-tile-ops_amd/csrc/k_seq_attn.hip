@@ -1,105 +1,513 @@
 // Attention of the rows of many sequences over the paged int8 cache.
 //
-//   x[key] = (q . k[key]) * (qs * qk_scale) * ks[key]    q . k exact in int32
+//   x[key] = (q . k[key]) * ks[key] * (qs * qk_scale)     q . k exact in int32
 //   out    = sum_key softmax(x)[key] * vs[key] * v[key]
 //
 // over the keys at or before the row's position (causal), all cached keys, or
-// the keys of listed pages.  Maximum, sum and products are f32.
+// the keys of listed pages.  One pass with the running maximum and sum of the
+// softmax, both in f32 and in base 2 (log2 e goes into the query's scale).
+//
+// The query heads of a KV head and the rows of a sequence are columns alike:
+// column c is row c / group, head c % group, and K and V are read once for all
+// columns of a tile.  Scores come transposed, S^T = K Q^T, so that a lane of the
+// int8 MFMA's result holds keys of one column: the maximum and the sum of a column
+// are register operations and two lane exchanges, and its P is already the B
+// operand of O^T = V^T P^T, the keys of a step in the order in which the
+// transposing LDS read delivers V.
+//
+// P is not rounded to 8 bits, nor to one bf16: p * vs goes to the matrix cores as
+// the sum of three bf16 numbers, all of its f32 bits (measured against float64,
+// 2-norm: two numbers leave 2.3e-6, three 2e-7 at 2000 keys, where f32 sums in torch leave 6e-7;
+// one would leave 1.6e-3), V as bf16, which holds every int8.  bf16 because the
+// range of the V scales is the user's, which f16 does not hold.
+#include "q3_attn_v.h"
 #include "q3_seq.h"
 
 namespace q3 {
 namespace {
 
-constexpr int HD = 128;
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
-// One workgroup per (row, head), 256 keys a step: a thread per key for the
-// scores, then a thread per (channel, half of the keys) for P V.
-__global__ void __launch_bounds__(256) seq_attn_kernel(SeqAttnArgs a) {
-  __shared__ float p[256], acc_s[2][HD], red[8];
-  const int tid = threadIdx.x;
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// ---- exchanges and conversions -------------------------------------------------
+
+// max / sum over the four 16-lane rows that share a column
+__device__ __forceinline__ float col_max(float x) {
+  LanePair p = lane_pair16(__float_as_uint(x));
+  x = fmaxf(__uint_as_float(p.a), __uint_as_float(p.b));
+  p = lane_pair32(__float_as_uint(x));
+  return fmaxf(__uint_as_float(p.a), __uint_as_float(p.b));
+}
+__device__ __forceinline__ float col_sum(float x) {
+  LanePair p = lane_pair16(__float_as_uint(x));
+  x = __uint_as_float(p.a) + __uint_as_float(p.b);
+  p = lane_pair32(__float_as_uint(x));
+  return __uint_as_float(p.a) + __uint_as_float(p.b);
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  const v2f t = {a, b};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(t, v2bf));
+}
+
+// x[0..7] as the sum of three bf16 numbers, the B operands of as many products
+struct Bf16x3 {
+  v8bf part[3];
+};
+__device__ __forceinline__ Bf16x3 split_bf16(const float (&x)[8]) {
+  v4u w[3];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float a = x[2 * i], b = x[2 * i + 1];
+#pragma unroll
+    for (int t = 0; t < 3; ++t) {
+      w[t][i] = pack_bf16(a, b);
+      a -= __uint_as_float(w[t][i] << 16);
+      b -= __uint_as_float(w[t][i] & 0xffff0000u);
+    }
+  }
+  Bf16x3 r;
+#pragma unroll
+  for (int t = 0; t < 3; ++t) r.part[t] = __builtin_bit_cast(v8bf, w[t]);
+  return r;
+}
+
+// 8 int8 as bf16, exactly
+__device__ __forceinline__ v8bf int8_bf16(v2i_d w) {
+  v4u r;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float f[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = static_cast<float>(static_cast<int8_t>(w[i] >> (8 * j)));
+    r[2 * i] = pack_bf16(f[0], f[1]);
+    r[2 * i + 1] = pack_bf16(f[2], f[3]);
+  }
+  return __builtin_bit_cast(v8bf, r);
+}
+
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// 4 bytes per lane global -> LDS (lane l writes lds + 4 l), see lds_copy16
+__device__ __forceinline__ void lds_copy4(const void *src, const void *lds) {
+  const uint32_t m0v =
+      __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(to_lds(lds))));
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(m0v) : "memory", "m0");
+}
+
+// ---- the result ---------------------------------------------------------------
+
+// 8 channels of a finished row: f32, or int8 with the head's scale, whose
+// maximum is taken over the 16 lanes that hold the head's other channels.
+__device__ __forceinline__ void store_row8(const SeqAttnArgs &a, int row, int head, int d0, const float (&o)[8]) {
+  if (a.out) {
+    float *dst = a.out + row * a.ldo + head * HD + d0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dst[i] = o[i];
+    return;
+  }
+  float m = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(o[i]));
+  m = fmaxf(m, lane_xor<1>(m));
+  m = fmaxf(m, lane_xor<2>(m));
+  m = fmaxf(m, lane_xor<4>(m));
+  m = fmaxf(m, lane_xor<8>(m));
+  const float scale = __fmul_rn(m, inv127());
+  const double y = rcp64(scale);
+  int8_t *dst = a.o8 + row * a.ldo8 + head * HD + d0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) dst[i] = static_cast<int8_t>(quant_rcp(o[i], y));
+  if (d0 == 0) a.os[row * a.ldos + head * a.os_col] = scale;
+}
+
+// Partial results of a (row, head): per split the unnormalised O [128], then for
+// all splits (maximum, sum).
+struct Partials {
+  float *o;   // [row * heads + head][split][128]
+  float2 *ml; // [row * heads + head][split]
+  int splits, span;  // keys of a split (listed pages: of the list's keys)
+};
+
+__device__ __forceinline__ float exp2_from(float x, float base) { return __builtin_amdgcn_exp2f(x - base); }
+
+// ---- few columns: 16 to a tile -------------------------------------------------
+//
+// A workgroup takes one tile of 16 columns, one KV head and one split of the keys;
+// its four waves take 32-key blocks in turn, each with its own running maximum and
+// sum, and join at the end.  A block is K [32][128] and V [32][128] int8 and their
+// 64 scales, 8.25 KiB: copied straight into the wave's own LDS stage while the block
+// before is worked on, so no wave waits for another and what is in flight costs no
+// registers.  16-byte chunk c of key r lies at chunk c ^ (r & 7) (V: c ^ vswz(r)),
+// so that neither the K operand's reads (16 keys, one chunk) nor the transposing
+// reads of V (8 keys, one chunk) meet in a bank.
+constexpr int KB = 32;
+constexpr int FEW_COLS = 16;
+constexpr int FEW_WAVES = 4;
+constexpr int FEW_STAGES = 2;
+constexpr int FEW_COPIES = 9;  // of a block: 4 K, 4 V, 1 scales
+constexpr int FEW_K = 0, FEW_V = KB * HD, FEW_S = 2 * KB * HD, FEW_STAGE = 2 * KB * HD + 2 * KB * 4;
+constexpr int FEW_ROW = HD + 4;  // floats of a column's row where the waves join
+constexpr int FEW_SPAN = 64 * KB * FEW_WAVES;  // keys of a split: a lane of each wave names one block
+static_assert(FEW_WAVES * FEW_COLS * FEW_ROW * 4 <= FEW_WAVES * FEW_STAGES * FEW_STAGE, "the join fits the stages");
+
+struct FewPlan {
+  Partials part;
+  int64_t units;     // (sequence or row) x tiles of 16 columns
+  int tiles;
+  int most;          // columns of a sequence that are taken here
+};
+
+template <bool LIST>
+__global__ void __launch_bounds__(64 * FEW_WAVES, 2) seq_attn_few_kernel(SeqAttnArgs a, FewPlan p) {
+  __shared__ __align__(16) uint8_t stage_s[FEW_WAVES * FEW_STAGES * FEW_STAGE];
+  __shared__ float m_s[FEW_WAVES][FEW_COLS], l_s[FEW_WAVES][FEW_COLS];
+  const int lane = threadIdx.x & 63, wave = wave_id();
+  const int col = lane & 15, quarter = lane >> 4;
+
+  // Workgroups go round the 8 XCDs: the KV heads of one (unit, split) share an
+  // XCD, whose L2 then holds the lines of scales that they share.
+  const int group_heads = a.heads / a.kv_heads;
+  const int rest = blockIdx.x >> 3;
+  const int kvh = rest % a.kv_heads;
+  const int us = (rest / a.kv_heads) * 8 + (blockIdx.x & 7);
+  const int unit = us / p.part.splits, split = us % p.part.splits;
+  if (unit >= p.units) return;
+  const int tile = unit % p.tiles;
+
+  int seq, row0 = 0;
+  if constexpr (LIST) {
+    row0 = unit / p.tiles;
+    seq = seq_of_row(a.seqs, row0);
+    if (seq >= a.seqs.n_seq) return;
+  } else {
+    seq = unit / p.tiles;
+  }
+  const SeqSpan sp = seq_span(a.seqs, seq);
+  const int pt = a.pool.page_tokens;
+
+  // this lane's column, and how many keys it sees
+  const int c = tile * FEW_COLS + col;
+  int row, g, cols;
+  if constexpr (LIST) {
+    if (row0 < sp.r0 || row0 >= sp.r0 + sp.n) return;
+    row = row0, g = c, cols = group_heads;
+  } else {
+    cols = sp.n * group_heads;
+    if (cols > p.most || tile * FEW_COLS >= cols) return;
+    row = sp.r0 + c / group_heads, g = c % group_heads;
+  }
+  const bool live = c < cols;
+  const int sees = !live ? 0 : a.causal ? max(sp.pos(row) + 1, 0) : sp.kv;
+  // the tile's first column sees the fewest keys, its last the most
+  const int vmin = __builtin_amdgcn_readlane(sees, 0);
+  const int vmax = __builtin_amdgcn_readlane(sees, min(cols - tile * FEW_COLS, FEW_COLS) - 1);
+
+  // Lane i names the wave's block i: its page, its place there, its first key.
+  const int span_blocks = p.part.span / KB;
+  const int first = split * span_blocks;  // blocks from 0, or of the list
+  int bpage = -1, bkey = 0, bt = 0;
+  {
+    const int b = first + lane * FEW_WAVES + wave;
+    if (lane * FEW_WAVES + wave < span_blocks) {
+      const int per_page = pt / KB;
+      const int nth = b / per_page;
+      bt = (b % per_page) * KB;
+      if constexpr (LIST) {
+        if (nth < a.n_sel) {
+          const int id = a.ids[row0 * a.ld_ids + static_cast<int64_t>(kvh) * a.n_sel + nth];
+          // a page of the row's: its first key is seen, so it lies in the table
+          if (vmax > 0 && id >= 0 && id <= (vmax - 1) / pt) {
+            bkey = id * pt + bt;
+            if (bkey < vmax) bpage = seq_page(a.seqs, a.pool, seq, id);
+          }
+        }
+      } else {
+        bkey = b * KB;
+        if (bkey < vmax) bpage = seq_page(a.seqs, a.pool, seq, nth);
+      }
+    }
+  }
+  uint64_t todo = __ballot(bpage >= 0);
+  if constexpr (!LIST) {
+    if (split > 0 && first * KB >= vmax) return;  // behind the tile's last key: nobody joins this split
+  }
+
+  // Q as the B operand: column l % 16, 16 bytes of each 64-byte half
+  v4i_d qf[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+  float cs = 0.0f;
+  if (live) {
+    const int8_t *q = a.q8 + row * a.ldq + (kvh * group_heads + g) * HD + 16 * quarter;
+    qf[0] = *reinterpret_cast<const v4i_d *>(q);
+    qf[1] = *reinterpret_cast<const v4i_d *>(q + 64);
+    cs = a.qs[row * a.ldqs + (kvh * group_heads + g) * a.qs_col] * a.qk_scale * kLog2e;
+  }
+
+  uint8_t *const stages = stage_s + wave * FEW_STAGES * FEW_STAGE;
+  const int r8 = lane >> 3, ch = lane & 7;
+  const int64_t lane_k = r8 * a.pool.row_bytes + 16 * (ch ^ r8);
+  const int64_t lane_v = r8 * a.pool.row_bytes + 16 * (ch ^ (r8 & 3));
+  const int64_t lane_v4 = r8 * a.pool.row_bytes + 16 * (ch ^ ((r8 & 3) | 4));
+
+  auto issue = [&](int i, uint8_t *st) {
+    const int page = __builtin_amdgcn_readlane(bpage, i), t0 = __builtin_amdgcn_readlane(bt, i);
+    const int64_t at = page * a.pool.page_bytes + t0 * a.pool.row_bytes + kvh * HD;
+    const int8_t *k = a.pool.k + at, *v = a.pool.v + at;
+    const int64_t eight = 8 * a.pool.row_bytes;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) lds_copy16(k + q * eight + lane_k, st + FEW_K + q * 1024);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) lds_copy16(v + q * eight + (q < 2 ? lane_v : lane_v4), st + FEW_V + q * 1024);
+    const int64_t sat = page * a.pool.spage + (t0 + (lane & 31)) * a.pool.srow + kvh;
+    lds_copy4((lane < 32 ? a.pool.ks : a.pool.vs) + sat, st + FEW_S);
+  };
+
+  float m = -INFINITY, l = 0.0f;
+  v4f o[8];
+#pragma unroll
+  for (int t = 0; t < 8; ++t) o[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+
+  int ahead = -1;  // the block in flight
+  if (todo) {
+    ahead = __builtin_ctzll(todo);
+    todo &= todo - 1;
+    issue(ahead, stages);
+  }
+  int buf = 0;
+  while (ahead >= 0) {
+    const int now = ahead;
+    uint8_t *const st = stages + buf * FEW_STAGE;
+    buf ^= 1;
+    ahead = -1;
+    if (todo) {
+      ahead = __builtin_ctzll(todo);
+      todo &= todo - 1;
+      // the reads of the block that lay there have been used
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      issue(ahead, stages + buf * FEW_STAGE);
+      wait_copies<FEW_COPIES>();
+    } else {
+      wait_copies<0>();
+    }
+
+    // S^T of two 16-key tiles: lane holds keys 4 quarter + i of each
+    float x[8], vsc[8];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint8_t *kr = st + FEW_K + (t * 16 + col) * HD;
+      const v4i_d k0 = *reinterpret_cast<const v4i_d *>(kr + 16 * (quarter ^ (col & 7)));
+      const v4i_d k1 = *reinterpret_cast<const v4i_d *>(kr + 16 * ((4 + quarter) ^ (col & 7)));
+      v4i_d s = {0, 0, 0, 0};
+      s = __builtin_amdgcn_mfma_i32_16x16x64_i8(k0, qf[0], s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_i32_16x16x64_i8(k1, qf[1], s, 0, 0, 0);
+      const v4f ks = *reinterpret_cast<const v4f *>(st + FEW_S + 4 * (t * 16 + 4 * quarter));
+      const v4f vs = *reinterpret_cast<const v4f *>(st + FEW_S + 4 * (KB + t * 16 + 4 * quarter));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[4 * t + i] = static_cast<float>(s[i]) * ks[i] * cs;
+        vsc[4 * t + i] = vs[i];
+      }
+    }
+    const int key0 = __builtin_amdgcn_readlane(bkey, now);
+    const bool edge = key0 + KB > vmin;  // some column does not see the whole block
+    if (edge) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (key0 + (j >> 2) * 16 + 4 * quarter + (j & 3) >= sees) x[j] = -INFINITY;
+    }
+    float mb = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+    mb = fmaxf(col_max(mb), m);
+    const float base = mb == -INFINITY ? 0.0f : mb;
+    if (__ballot(mb != m)) {
+      const float alpha = exp2_from(m, base);
+      l *= alpha;
+#pragma unroll
+      for (int t = 0; t < 8; ++t) o[t] *= alpha;
+      m = mb;
+    }
+    float pv[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float e = exp2_from(x[j], base);
+      l += e;
+      pv[j] = e * vsc[j];
+    }
+    if (edge) {  // a scale behind the sequence's end may be anything
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (key0 + (j >> 2) * 16 + 4 * quarter + (j & 3) >= sees) pv[j] = 0.0f;
+    }
+    const Bf16x3 pb = split_bf16(pv);
+
+    // the key that this lane's address names for the transposing read: the 16
+    // lanes of a row take 8 keys, two halves of a 16-byte chunk each
+    const int rj = (lane & 15) >> 1;
+    const int key = 4 * quarter + (rj & 3) + 16 * (rj >> 2);
+    const uint8_t *vq = st + FEW_V + key * HD + 8 * (lane & 1);
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      const v2i_d w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(reinterpret_cast<lds_v2i_ptr_d>(to_lds(vq + 16 * (t ^ vswz(key)))));
+      const v8bf vt = int8_bf16(w);
+#pragma unroll
+      for (int u = 0; u < 3; ++u) o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt, pb.part[u], o[t], 0, 0, 0);
+    }
+  }
+
+  // join the waves: each column's rows of O by wave, and (m, l)
+  l = col_sum(l);
+  __syncthreads();  // every wave is done with its stages
+  float *join = reinterpret_cast<float *>(stage_s);
+#pragma unroll
+  for (int t = 0; t < 8; ++t)
+    *reinterpret_cast<v4f *>(join + (wave * FEW_COLS + col) * FEW_ROW + 16 * t + 4 * quarter) = o[t];
+  if (quarter == 0) m_s[wave][col] = m, l_s[wave][col] = l;
+  __syncthreads();
+  const int jc = threadIdx.x >> 4, d0 = 8 * (threadIdx.x & 15);
+  const int cc = tile * FEW_COLS + jc;
+  if (cc >= cols) return;
+  float top = m_s[0][jc];
+#pragma unroll
+  for (int w = 1; w < FEW_WAVES; ++w) top = fmaxf(top, m_s[w][jc]);
+  const float base = top == -INFINITY ? 0.0f : top;
+  float sum = 0.0f, r[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+  for (int w = 0; w < FEW_WAVES; ++w) {
+    const float f = exp2_from(m_s[w][jc], base);
+    sum += f * l_s[w][jc];
+    const float *src = join + (w * FEW_COLS + jc) * FEW_ROW + d0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] += f * src[i];
+  }
+  const int jrow = LIST ? row0 : sp.r0 + cc / group_heads;
+  const int jhead = kvh * group_heads + (LIST ? cc : cc % group_heads);
+  if (p.part.splits == 1) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = top == -INFINITY ? 0.0f : r[i] / sum;
+    store_row8(a, jrow, jhead, d0, r);
+    return;
+  }
+  const int64_t at = (static_cast<int64_t>(jrow) * a.heads + jhead) * p.part.splits + split;
+  v4f *dst = reinterpret_cast<v4f *>(p.part.o + at * HD + d0);
+  dst[0] = v4f{r[0], r[1], r[2], r[3]};
+  dst[1] = v4f{r[4], r[5], r[6], r[7]};
+  if (d0 == 0) p.part.ml[at] = make_float2(top, sum);
+}
+
+// Joins the splits of a (row, head): 16 lanes of 8 channels, 16 such groups over
+// the splits in turn.
+__global__ void __launch_bounds__(256) seq_attn_join_kernel(SeqAttnArgs a, Partials p, int list, int most) {
+  __shared__ float o_s[4][HD];
+  __shared__ float sum_s[4];
   const int row = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
-  const int kvh = head / (a.heads / a.kv_heads);
   const int seq = seq_of_row(a.seqs, row);
   if (seq >= a.seqs.n_seq) return;
   const SeqSpan sp = seq_span(a.seqs, seq);
   if (row < sp.r0 || row >= sp.r0 + sp.n) return;
-  const int pt = a.pool.page_tokens;
-  const int visible = a.causal ? sp.pos(row) + 1 : sp.kv;  // <= 0: nothing
-  const int64_t keys = a.ids ? static_cast<int64_t>(a.n_sel) * pt : max(visible, 0);
-  const int *q = reinterpret_cast<const int *>(a.q8 + row * a.ldq + head * HD);
-  const float c = a.qs[row * a.ldqs + head * a.qs_col] * a.qk_scale;
-  float m = -INFINITY, l = 0.0f, acc = 0.0f;
-  for (int64_t k0 = 0; k0 < keys; k0 += 256) {
-    __shared__ int64_t vat[256];
-    const int64_t i = k0 + tid;
-    float x = -INFINITY;
-    float sv = 0.0f;
-    vat[tid] = -1;
-    if (i < keys) {
-      int key = static_cast<int>(i);
-      if (a.ids) {
-        const int id = a.ids[row * a.ld_ids + kvh * a.n_sel + i / pt];
-        key = id >= 0 && id <= (a.seqs.max_kv - 1) / pt ? id * pt + static_cast<int>(i % pt) : -1;
-      }
-      if (key >= 0 && key < visible) {
-        const int page = seq_page(a.seqs, a.pool, seq, key / pt);
-        if (page >= 0) {
-          const int t = key % pt;
-          const int *k = reinterpret_cast<const int *>(a.pool.k + page * a.pool.page_bytes + t * a.pool.row_bytes + kvh * HD);
-          int dot = 0;
-          for (int j = 0; j < HD / 4; ++j) dot = __builtin_amdgcn_sdot4(q[j], k[j], dot, false);
-          const int64_t at = page * a.pool.spage + t * a.pool.srow + kvh;
-          x = static_cast<float>(dot) * a.pool.ks[at] * c;
-          sv = a.pool.vs[at];
-          vat[tid] = page * a.pool.page_bytes + t * a.pool.row_bytes + kvh * HD;
-        }
-      }
-    }
-    const float w = max64(x);
-    if ((tid & 63) == 0) red[tid >> 6] = w;
-    __syncthreads();
-    const float m1 = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-    const float base = m1 == -INFINITY ? 0.0f : m1;
-    const float e = vat[tid] >= 0 ? expf(x - base) : 0.0f;
-    const float scale = expf(m - base);
-    m = m1;
-    p[tid] = vat[tid] >= 0 ? e * sv : 0.0f;
-    float t = e;
-    for (int d = 1; d < 64; d *= 2) t += __shfl_xor(t, d);
-    if ((tid & 63) == 0) red[4 + (tid >> 6)] = t;
-    __syncthreads();
-    l = l * scale + (red[4] + red[5] + red[6] + red[7]);
-    acc *= scale;
-    const int ch = tid & 127, half = tid >> 7;
-    for (int j = half * 128; j < half * 128 + 128; ++j)
-      if (vat[j] >= 0) acc += p[j] * static_cast<float>(a.pool.v[vat[j] + ch]);
-    __syncthreads();
+  if (!list && sp.n * (a.heads / a.kv_heads) > most) return;
+  const int sees = a.causal ? max(sp.pos(row) + 1, 0) : sp.kv;
+  const int n = list ? p.splits : (sees + p.span - 1) / p.span;
+  const int64_t at = (static_cast<int64_t>(row) * a.heads + head) * p.splits;
+  float top = -INFINITY;
+  for (int s = threadIdx.x & 63; s < n; s += 64) top = fmaxf(top, p.ml[at + s].x);
+  top = max64(top);
+  const float base = top == -INFINITY ? 0.0f : top;
+  const int d0 = 8 * (threadIdx.x & 15);
+  float r[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sum = 0.0f;
+#pragma unroll 4
+  for (int s = threadIdx.x >> 4; s < n; s += 16) {
+    const float2 ml = p.ml[at + s];
+    const float f = exp2_from(ml.x, base);
+    sum += f * ml.y;
+    const v4f *src = reinterpret_cast<const v4f *>(p.o + (at + s) * HD + d0);
+    const v4f u = src[0], v = src[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] += f * u[i], r[4 + i] += f * v[i];
   }
-  acc_s[tid >> 7][tid & 127] = acc;
-  __syncthreads();
-  float o = 0.0f;
-  if (tid < HD) {
-    o = acc_s[0][tid] + acc_s[1][tid];
-    o = l == 0.0f && m == -INFINITY ? 0.0f : o / l;
-    if (a.out) a.out[row * a.ldo + head * HD + tid] = o;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = col_sum(r[i]);
+  sum = col_sum(sum);
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) < 16) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o_s[wave][d0 + i] = r[i];
+    if (d0 == 0) sum_s[wave] = sum;
   }
-  if (!a.o8) return;
-  const float pk = max64(fabsf(o));
-  if ((tid & 63) == 0) red[tid >> 6] = pk;
   __syncthreads();
-  if (tid >= HD) return;
-  const float sc = __fmul_rn(fmaxf(red[0], red[1]), inv127());
-  a.o8[row * a.ldo8 + head * HD + tid] = static_cast<int8_t>(quant1(o, sc));
-  if (tid == 0) a.os[row * a.ldos + head * a.os_col] = sc;
+  if (threadIdx.x >= 16) return;
+  sum = (sum_s[0] + sum_s[1]) + (sum_s[2] + sum_s[3]);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    r[i] = (o_s[0][d0 + i] + o_s[1][d0 + i]) + (o_s[2][d0 + i] + o_s[3][d0 + i]);
+    r[i] = top == -INFINITY ? 0.0f : r[i] / sum;
+  }
+  store_row8(a, row, head, d0, r);
+}
+
+// ---- plans --------------------------------------------------------------------
+
+constexpr int64_t kMaxGrid = (int64_t(1) << 32) / 256 - 1;  // workgroups of 256 lanes in a launch
+
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// How the keys are split.  `units` workgroups a KV head would run without a split;
+// keys: the most that a row can see.
+void plan_splits(int64_t units, int64_t keys, Partials &p) {
+  const int64_t want = units >= 2048 ? 1 : 2048 / (units < 1 ? 1 : units);
+  int64_t splits = want < 64 ? want : 64;
+  int64_t span = cdiv(cdiv(keys < 1 ? 1 : keys, splits), FEW_WAVES * KB) * FEW_WAVES * KB;
+  if (span < 256) span = 256;
+  if (span > FEW_SPAN) span = FEW_SPAN;
+  p.span = static_cast<int>(span);
+  p.splits = static_cast<int>(cdiv(keys < 1 ? 1 : keys, span));
+}
+
+FewPlan plan_few(const SeqAttnArgs &a) {
+  FewPlan p{};
+  const int64_t g = a.heads / a.kv_heads;
+  const bool list = a.ids != nullptr;
+  p.most = INT32_MAX;
+  p.tiles = static_cast<int>(cdiv(list ? g : a.seqs.max_rows * g, FEW_COLS));
+  if (p.tiles < 1) p.tiles = 1;
+  p.units = (list ? a.seqs.rows : a.seqs.n_seq) * int64_t(p.tiles);
+  const int64_t keys = list ? int64_t(a.n_sel) * a.pool.page_tokens : a.seqs.max_kv;
+  plan_splits(p.units * a.kv_heads, keys, p.part);
+  return p;
+}
+
+uint64_t partial_floats(const SeqAttnArgs &a, const Partials &p) {
+  return p.splits == 1 ? 0 : uint64_t(a.seqs.rows) * a.heads * p.splits;
 }
 
 }  // namespace
 
-uint64_t seq_attn_ws_bytes(const SeqAttnArgs &a) { return 0; }
+uint64_t seq_attn_ws_bytes(const SeqAttnArgs &a) {
+  return partial_floats(a, plan_few(a).part) * (HD * 4 + 8);
+}
 
 hipError_t launch_seq_attn(const SeqAttnArgs &a, hipStream_t s) {
   if (a.seqs.rows == 0 || a.seqs.n_seq == 0) return hipSuccess;
-  hipLaunchKernelGGL(seq_attn_kernel, dim3(static_cast<unsigned>(static_cast<int64_t>(a.seqs.rows) * a.heads)), dim3(256), 0, s, a);
+  FewPlan p = plan_few(a);
+  const uint64_t slots = partial_floats(a, p.part);
+  p.part.o = static_cast<float *>(a.ws);
+  p.part.ml = reinterpret_cast<float2 *>(p.part.o + slots * HD);
+  const int64_t wgs = cdiv(p.units * p.part.splits, 8) * 8 * a.kv_heads;
+  if (wgs > kMaxGrid) return hipErrorInvalidValue;
+  const dim3 grid(static_cast<unsigned>(wgs));
+  if (a.ids)
+    hipLaunchKernelGGL(seq_attn_few_kernel<true>, grid, dim3(64 * FEW_WAVES), 0, s, a, p);
+  else
+    hipLaunchKernelGGL(seq_attn_few_kernel<false>, grid, dim3(64 * FEW_WAVES), 0, s, a, p);
+  if (const hipError_t e = hipGetLastError(); e != hipSuccess || p.part.splits == 1) return e;
+  hipLaunchKernelGGL(seq_attn_join_kernel, dim3(static_cast<unsigned>(int64_t(a.seqs.rows) * a.heads)), dim3(256), 0, s, a,
+                     p.part, a.ids != nullptr, p.most);
   return hipGetLastError();
 }
 
