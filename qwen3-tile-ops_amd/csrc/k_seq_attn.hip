@@ -129,12 +129,13 @@ __device__ __forceinline__ void store_row8(const SeqAttnArgs &a, int row, int he
   if (d0 == 0) a.os[row * a.ldos + head * a.os_col] = scale;
 }
 
-// Partial results of a (row, head): per split the unnormalised O [128], then for
-// all splits (maximum, sum).
+// Partial results of a (row, head) by split: the unnormalised O, its maximum and
+// its sum.  A row's splits are those of the kernel that takes its sequence.
 struct Partials {
-  float *o;   // [row * heads + head][split][128]
-  float2 *ml; // [row * heads + head][split]
+  float *o;    // [row * heads + head][split of stride][128]
+  float2 *ml;  // [row * heads + head][split of stride]
   int splits, span;  // keys of a split (listed pages: of the list's keys)
+  int stride;
 };
 
 __device__ __forceinline__ float exp2_from(float x, float base) { return __builtin_amdgcn_exp2f(x - base); }
@@ -394,16 +395,334 @@ __global__ void __launch_bounds__(64 * FEW_WAVES, 2) seq_attn_few_kernel(SeqAttn
     store_row8(a, jrow, jhead, d0, r);
     return;
   }
-  const int64_t at = (static_cast<int64_t>(jrow) * a.heads + jhead) * p.part.splits + split;
+  const int64_t at = (static_cast<int64_t>(jrow) * a.heads + jhead) * p.part.stride + split;
   v4f *dst = reinterpret_cast<v4f *>(p.part.o + at * HD + d0);
   dst[0] = v4f{r[0], r[1], r[2], r[3]};
   dst[1] = v4f{r[4], r[5], r[6], r[7]};
   if (d0 == 0) p.part.ml[at] = make_float2(top, sum);
 }
 
+// ---- many columns: 128 to a tile -----------------------------------------------
+//
+// A workgroup takes one tile of 128 columns and one KV head; each of its four waves
+// has 32 columns, and all share the keys, 64 a step.  K [64][128] goes to the K
+// operand's LDS image as it is; V int8 is turned once for all four waves into the
+// bf16 image of the A operand of V^T P^T (a quarter of it by each wave: a
+// transposing read hands a lane 8 keys of one channel, in the order in which P's
+// keys lie in the registers).  While a step's scores and products are computed, the
+// next step's V is turned and its K and the V after next are copied, so a step has
+// one barrier.  What a step costs a SIMD: 8 int8 MFMAs for S (256 cycles), 48 bf16
+// ones for P V (1536), and about 15 VALU instructions per (key, column) lane.
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef int v16i __attribute__((ext_vector_type(16)));
+
+constexpr int WIDE_COLS = 128;
+constexpr int WIDE_KEYS = 64;
+constexpr int WIDE_SPAN = 32768;  // keys of a split: its page ids lie in LDS
+constexpr int WIDE_OROW = 32 + 4;  // floats of a column's row where the results turn
+
+struct WidePlan {
+  Partials part;
+  int64_t tiles;  // at most
+  int least;      // columns of a sequence that are taken here
+};
+
+// Key r's 16-byte chunk c of V lies at chunk c ^ vswz_wide(r): the 8 keys of a
+// transposing read (two runs of four, 8 apart) meet 8 chunks.
+__device__ __forceinline__ int vswz_wide(int key) { return (key & 3) | ((key >> 1) & 4); }
+
+__global__ void __launch_bounds__(256, 2) seq_attn_wide_kernel(SeqAttnArgs a, WidePlan p) {
+  __shared__ __align__(16) uint8_t k_s[2][WIDE_KEYS * HD];
+  __shared__ __align__(16) uint8_t v8_s[2][WIDE_KEYS * HD];
+  __shared__ __align__(16) uint8_t vb_s[2][WIDE_KEYS * HD * 2];
+  __shared__ __align__(16) float sc_s[3][2 * WIDE_KEYS];  // ks, then vs
+  __shared__ int page_s[WIDE_SPAN / KB];
+  static_assert(sizeof(vb_s) >= 4 * 32 * WIDE_OROW * 4, "the results fit where V was");
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
+  const int half = lane >> 5, n32 = lane & 31;
+  const int group_heads = a.heads / a.kv_heads;
+
+  // which sequence's tile this is: tiles of the sequences before, 64 at a time
+  const int kvh = blockIdx.x % a.kv_heads;
+  const int64_t us = blockIdx.x / a.kv_heads;
+  const int split = us % p.part.splits;
+  int64_t nth = us / p.part.splits;
+  int seq = -1;
+  for (int b = 0; b < a.seqs.n_seq && seq < 0; b += 64) {
+    int tiles = 0;
+    if (b + lane < a.seqs.n_seq) {
+      const int64_t cols = static_cast<int64_t>(seq_span(a.seqs, b + lane).n) * group_heads;
+      tiles = cols < p.least ? 0 : static_cast<int>((cols + WIDE_COLS - 1) / WIDE_COLS);
+    }
+    int upto = tiles;  // inclusive sum over the lanes
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int t = __shfl_up(upto, d);
+      upto += lane >= d ? t : 0;
+    }
+    const uint64_t holds = __ballot(upto > nth);
+    if (holds) {
+      const int at = __builtin_ctzll(holds);
+      seq = b + at;
+      // a sequence's last rows see the most keys: its tiles start with them
+      nth = __builtin_amdgcn_readlane(upto, at) - 1 - nth;
+    } else {
+      nth -= __builtin_amdgcn_readlane(upto, 63);
+    }
+  }
+  if (seq < 0) return;
+  const SeqSpan sp = seq_span(a.seqs, seq);
+  const int cols = sp.n * group_heads;
+  const int pt = a.pool.page_tokens;
+  const int col0 = static_cast<int>(nth) * WIDE_COLS;
+  const int c = col0 + wave * 32 + n32;
+  const bool live = c < cols;
+  const int row = sp.r0 + c / group_heads, head = kvh * group_heads + c % group_heads;
+  const int sees = !live ? 0 : a.causal ? max(sp.pos(row) + 1, 0) : sp.kv;
+  // the wave's first column sees the fewest keys of its columns; the tile's last
+  // the most of all
+  const int vmin = __builtin_amdgcn_readfirstlane(sees);
+  const int rest = min(cols - (col0 + wave * 32), 32);
+  const int vmax = rest <= 0 ? 0 : __builtin_amdgcn_readlane(sees, max(rest, 1) - 1);
+  const int last_row = sp.r0 + (min(cols, col0 + WIDE_COLS) - 1) / group_heads;
+  const int tile_max = a.causal ? max(sp.pos(last_row) + 1, 0) : sp.kv;
+  const int first = split * p.part.span;
+  const int end = min(tile_max, first + p.part.span);
+  if (split > 0 && first >= tile_max) return;
+  const int steps = (end - first + WIDE_KEYS - 1) / WIDE_KEYS;  // <= 0: none
+
+  for (int i = tid; i < steps * (WIDE_KEYS / KB); i += 256) {
+    const int key = first + i * KB;
+    page_s[i] = key < end ? seq_page(a.seqs, a.pool, seq, key / pt) : -1;
+  }
+
+  v4i_d qf[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) qf[i] = v4i_d{0, 0, 0, 0};
+  float cs = 0.0f;
+  if (live) {
+    const int8_t *q = a.q8 + row * a.ldq + head * HD + 16 * half;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) qf[i] = *reinterpret_cast<const v4i_d *>(q + 32 * i);
+    cs = a.qs[row * a.ldqs + head * a.qs_col] * a.qk_scale * kLog2e;
+  }
+  __syncthreads();
+
+  // Copies: wave w takes keys 16 w .. 16 w + 15 of a step, all in one 32-key block.
+  const int r8 = lane >> 3, ch = lane & 7;
+  const int64_t lane_k = (16 * wave + r8) * a.pool.row_bytes + 16 * (ch ^ r8);
+  const int64_t lane_v[2] = {(16 * wave + r8) * a.pool.row_bytes + 16 * (ch ^ (r8 & 3)),
+                             (16 * wave + r8) * a.pool.row_bytes + 16 * (ch ^ ((r8 & 3) | 4))};
+  // (page and first token of a step's 32-key block)
+  auto block_at = [&](int step, int b, int *t0) {
+    *t0 = (first + step * WIDE_KEYS + b * KB) % pt;
+    return __builtin_amdgcn_readfirstlane(page_s[step * 2 + b]);
+  };
+  auto copy_k = [&](int step) {
+    int t0;
+    const int b = wave >> 1, page = block_at(step, b, &t0);
+    if (page >= 0) {
+      const int8_t *k = a.pool.k + page * a.pool.page_bytes + (t0 - b * KB) * a.pool.row_bytes + kvh * HD + lane_k;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) lds_copy16(k + q * 8 * a.pool.row_bytes, k_s[step & 1] + (2 * wave + q) * 1024);
+    }
+  };
+  auto copy_v = [&](int step) {
+    int t0;
+    const int b = wave >> 1, page = block_at(step, b, &t0);
+    if (page >= 0) {
+      const int8_t *v = a.pool.v + page * a.pool.page_bytes + (t0 - b * KB) * a.pool.row_bytes + kvh * HD;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) lds_copy16(v + q * 8 * a.pool.row_bytes + lane_v[q], v8_s[step & 1] + (2 * wave + q) * 1024);
+    }
+    if (wave < 2) {  // wave 0: the K scales of the step's 64 keys, wave 1: V's
+      int ta, tb;
+      const int pa = block_at(step, 0, &ta), pb = block_at(step, 1, &tb);
+      if (pa >= 0 || pb >= 0) {
+        // (a block without a page is masked: the other's scales will do)
+        const int page2 = (lane < KB || pb < 0) && pa >= 0 ? pa : pb, t = (lane < KB ? ta : tb) + n32;
+        const float *src = wave == 0 ? a.pool.ks : a.pool.vs;
+        lds_copy4(src + page2 * a.pool.spage + t * a.pool.srow + kvh, sc_s[step % 3] + wave * WIDE_KEYS);
+      }
+    }
+  };
+  // A quarter of a step's V: channels 32 wave .. + 31 of its four 16-key runs.
+  const int vj = (lane & 15) >> 1;
+  const int vkey = 8 * (vj >> 2) + 4 * half + (vj & 3);
+  auto turn_v = [&](int step) {
+#pragma unroll
+    for (int kc = 0; kc < 4; ++kc) {
+      const int key = 16 * kc + vkey, chunk = 2 * wave + ((lane >> 4) & 1);
+      const uint8_t *src = v8_s[step & 1] + key * HD + 16 * (chunk ^ vswz_wide(key)) + 8 * (lane & 1);
+      const v8bf w = int8_bf16(__builtin_amdgcn_ds_read_tr8_b64_v2i32(reinterpret_cast<lds_v2i_ptr_d>(to_lds(src))));
+      *reinterpret_cast<v8bf *>(vb_s[step & 1] + ((kc * 4 + wave) * 64 + lane) * 16) = w;
+    }
+  };
+
+  float m = -INFINITY, l = 0.0f;
+  v16f o[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
+
+  if (steps > 0) {
+    copy_v(0);
+    copy_k(0);
+    wait_copies<0>();
+    lds_barrier();
+    turn_v(0);
+    if (steps > 1) copy_v(1);
+    wait_copies<0>();
+    lds_barrier();
+  }
+  for (int step = 0; step < steps; ++step) {
+    if (step + 2 < steps) copy_v(step + 2);
+    if (step + 1 < steps) {
+      copy_k(step + 1);
+      turn_v(step + 1);
+    }
+    const int key0 = first + step * WIDE_KEYS;
+    if (key0 < vmax) {
+      const int pages[2] = {page_s[2 * step], page_s[2 * step + 1]};
+      float x[32];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const uint8_t *kr = k_s[step & 1] + (32 * t + n32) * HD;
+        v16i s;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const v4i_d kf = *reinterpret_cast<const v4i_d *>(kr + 16 * ((2 * i + half) ^ (n32 & 7)));
+          s = __builtin_amdgcn_mfma_i32_32x32x32_i8(kf, qf[i], s, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const v4f ks = *reinterpret_cast<const v4f *>(sc_s[step % 3] + 32 * t + 8 * i + 4 * half);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[16 * t + 4 * i + j] = static_cast<float>(s[4 * i + j]) * ks[j] * cs;
+        }
+      }
+      // register i of a tile is key 8 (i / 4) + 4 half + i % 4
+      const bool edge = key0 + WIDE_KEYS > vmin || pages[0] < 0 || pages[1] < 0;
+      uint32_t seen = ~0u;
+      if (edge) {
+        seen = 0;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const int key = 32 * (i >> 4) + 8 * ((i & 15) >> 2) + 4 * half + (i & 3);
+          const bool s = key0 + key < sees && pages[i >> 4] >= 0;
+          seen |= static_cast<uint32_t>(s) << i;
+          if (!s) x[i] = -INFINITY;
+        }
+      }
+      float mb = x[0];
+#pragma unroll
+      for (int i = 1; i < 32; ++i) mb = fmaxf(mb, x[i]);
+      {
+        const LanePair pr = lane_pair32(__float_as_uint(mb));
+        mb = fmaxf(fmaxf(__uint_as_float(pr.a), __uint_as_float(pr.b)), m);
+      }
+      const float base = mb == -INFINITY ? 0.0f : mb;
+      if (__ballot(mb != m)) {
+        const float alpha = exp2_from(m, base);
+        l *= alpha;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) o[t] *= alpha;
+        m = mb;
+      }
+#pragma unroll
+      for (int kc = 0; kc < 4; ++kc) {  // 16 keys: registers 8 kc .. 8 kc + 7
+        const v4f va = *reinterpret_cast<const v4f *>(sc_s[step % 3] + WIDE_KEYS + 16 * kc + 4 * half);
+        const v4f vc = *reinterpret_cast<const v4f *>(sc_s[step % 3] + WIDE_KEYS + 16 * kc + 8 + 4 * half);
+        float pv[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float e = exp2_from(x[8 * kc + j], base);
+          l += e;
+          pv[j] = e * (j < 4 ? va[j] : vc[j - 4]);
+        }
+        if (edge) {  // a scale behind the sequence's end may be anything
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (!(seen >> (8 * kc + j) & 1)) pv[j] = 0.0f;
+        }
+        const Bf16x3 pb = split_bf16(pv);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const v8bf vt = *reinterpret_cast<const v8bf *>(vb_s[step & 1] + ((kc * 4 + t) * 64 + lane) * 16);
+#pragma unroll
+          for (int u = 0; u < 3; ++u) o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt, pb.part[u], o[t], 0, 0, 0);
+        }
+      }
+    }
+    wait_copies<0>();
+    lds_barrier();
+  }
+
+  {
+    const LanePair pr = lane_pair32(__float_as_uint(l));
+    l = __uint_as_float(pr.a) + __uint_as_float(pr.b);
+  }
+  const bool whole = p.part.splits == 1;
+  const int64_t at = whole || !live ? 0 : (static_cast<int64_t>(row) * a.heads + head) * p.part.stride + split;
+  if (whole) {
+    const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) o[t] *= inv;
+  } else if (live && half == 0) {
+    p.part.ml[at] = make_float2(m, l);
+  }
+  if (whole && a.o8) {
+    float pk = 0.0f;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) pk = fmaxf(pk, fabsf(o[t][i]));
+    const LanePair pr = lane_pair32(__float_as_uint(pk));
+    const float scale = __fmul_rn(fmaxf(__uint_as_float(pr.a), __uint_as_float(pr.b)), inv127());
+    if (!live) return;
+    const double y = rcp64(scale);
+    int8_t *dst = a.o8 + row * a.ldo8 + head * HD;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        dst[32 * t + 8 * (i >> 2) + 4 * half + (i & 3)] = static_cast<int8_t>(quant_rcp(o[t][i], y));
+    if (half == 0) a.os[row * a.ldos + head * a.os_col] = scale;
+    return;
+  }
+  // f32 rows through LDS (the steps' last barrier is behind every wave, and a
+  // wave keeps to its own part), 32 channels at a time: written in 128-byte pieces
+  float *const turn = reinterpret_cast<float *>(vb_s) + wave * 32 * WIDE_OROW;
+  const int64_t mine = !live ? -1 : whole ? row * a.ldo + head * HD : at * HD;
+  float *const to = whole ? a.out : p.part.o;
+  const bool words = !whole || a.out_words;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<v4f *>(turn + n32 * WIDE_OROW + 8 * i + 4 * half) = v4f{o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t off = __shfl(mine, 8 * k + r8);
+      const v4f r = *reinterpret_cast<const v4f *>(turn + (8 * k + r8) * WIDE_OROW + 4 * ch);
+      if (off < 0) continue;
+      float *dst = to + off + 32 * t + 4 * ch;
+      if (words) {
+        *reinterpret_cast<v4f *>(dst) = r;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dst[i] = r[i];
+      }
+    }
+  }
+}
+
 // Joins the splits of a (row, head): 16 lanes of 8 channels, 16 such groups over
 // the splits in turn.
-__global__ void __launch_bounds__(256) seq_attn_join_kernel(SeqAttnArgs a, Partials p, int list, int most) {
+__global__ void __launch_bounds__(256) seq_attn_join_kernel(SeqAttnArgs a, Partials few, Partials wide, int most) {
   __shared__ float o_s[4][HD];
   __shared__ float sum_s[4];
   const int row = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
@@ -411,10 +730,11 @@ __global__ void __launch_bounds__(256) seq_attn_join_kernel(SeqAttnArgs a, Parti
   if (seq >= a.seqs.n_seq) return;
   const SeqSpan sp = seq_span(a.seqs, seq);
   if (row < sp.r0 || row >= sp.r0 + sp.n) return;
-  if (!list && sp.n * (a.heads / a.kv_heads) > most) return;
+  const Partials &p = !a.ids && sp.n * (a.heads / a.kv_heads) > most ? wide : few;
+  if (p.splits == 1) return;  // written as it is
   const int sees = a.causal ? max(sp.pos(row) + 1, 0) : sp.kv;
-  const int n = list ? p.splits : (sees + p.span - 1) / p.span;
-  const int64_t at = (static_cast<int64_t>(row) * a.heads + head) * p.splits;
+  const int n = a.ids ? p.splits : (sees + p.span - 1) / p.span;
+  const int64_t at = (static_cast<int64_t>(row) * a.heads + head) * p.stride;
   float top = -INFINITY;
   for (int s = threadIdx.x & 63; s < n; s += 64) top = fmaxf(top, p.ml[at + s].x);
   top = max64(top);
@@ -457,57 +777,80 @@ constexpr int64_t kMaxGrid = (int64_t(1) << 32) / 256 - 1;  // workgroups of 256
 
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// How the keys are split.  `units` workgroups a KV head would run without a split;
-// keys: the most that a row can see.
-void plan_splits(int64_t units, int64_t keys, Partials &p) {
-  const int64_t want = units >= 2048 ? 1 : 2048 / (units < 1 ? 1 : units);
-  int64_t splits = want < 64 ? want : 64;
-  int64_t span = cdiv(cdiv(keys < 1 ? 1 : keys, splits), FEW_WAVES * KB) * FEW_WAVES * KB;
-  if (span < 256) span = 256;
-  if (span > FEW_SPAN) span = FEW_SPAN;
+// Splits `keys` over workgroups, `units` of which would run without a split, until
+// there are about `want` of them: spans of a multiple of `step` keys, from `least`
+// to `most`, and at most 64 splits within that.
+void plan_splits(int64_t units, int64_t keys, int64_t want, int step, int least, int most, Partials &p) {
+  if (keys < 1) keys = 1;
+  if (units < 1) units = 1;
+  int64_t splits = units >= want ? 1 : want / units;
+  if (splits > 64) splits = 64;
+  int64_t span = cdiv(cdiv(keys, splits), step) * step;
+  if (span < least) span = least;
+  if (span > most) span = most;
   p.span = static_cast<int>(span);
-  p.splits = static_cast<int>(cdiv(keys < 1 ? 1 : keys, span));
+  p.splits = static_cast<int>(cdiv(keys, span));
 }
 
-FewPlan plan_few(const SeqAttnArgs &a) {
-  FewPlan p{};
-  const int64_t g = a.heads / a.kv_heads;
-  const bool list = a.ids != nullptr;
-  p.most = INT32_MAX;
-  p.tiles = static_cast<int>(cdiv(list ? g : a.seqs.max_rows * g, FEW_COLS));
-  if (p.tiles < 1) p.tiles = 1;
-  p.units = (list ? a.seqs.rows : a.seqs.n_seq) * int64_t(p.tiles);
-  const int64_t keys = list ? int64_t(a.n_sel) * a.pool.page_tokens : a.seqs.max_kv;
-  plan_splits(p.units * a.kv_heads, keys, p.part);
+// Sequences of up to FEW_MOST columns go to the kernel of 16-column tiles.
+constexpr int FEW_MOST = 16;
+
+struct Plan {
+  FewPlan few;
+  WidePlan wide;
+  bool any_wide;
+  uint64_t slots;  // of partial results
+};
+
+Plan plan_attn(const SeqAttnArgs &a) {
+  Plan p{};
+  const int64_t g = a.heads / a.kv_heads, rows = a.seqs.rows, n_seq = a.seqs.n_seq;
+  const int64_t cols = a.ids ? g : a.seqs.max_rows * g;  // of a sequence (listed pages: of a row), at most
+  p.any_wide = !a.ids && cols > FEW_MOST;
+  const int64_t few_cols = p.any_wide ? FEW_MOST : cols;
+  p.few.most = FEW_MOST;
+  p.few.tiles = static_cast<int>(few_cols < 1 ? 1 : cdiv(few_cols, FEW_COLS));
+  p.few.units = (a.ids ? rows : n_seq) * p.few.tiles;
+  plan_splits(p.few.units * a.kv_heads, a.ids ? int64_t(a.n_sel) * a.pool.page_tokens : a.seqs.max_kv, 2048, FEW_WAVES * KB, 256,
+              FEW_SPAN, p.few.part);
+  p.few.part.stride = p.few.part.splits;
+  if (p.any_wide) {
+    p.wide.least = FEW_MOST + 1;
+    const int64_t wide_seqs = rows * g / p.wide.least;
+    p.wide.tiles = rows * g / WIDE_COLS + (n_seq < wide_seqs ? n_seq : wide_seqs);
+    plan_splits(p.wide.tiles * a.kv_heads, a.seqs.max_kv, 512, WIDE_KEYS, 512, WIDE_SPAN, p.wide.part);
+    if (p.wide.part.splits > p.few.part.stride) p.few.part.stride = p.wide.part.splits;
+    p.wide.part.stride = p.few.part.stride;
+  }
+  p.slots = p.few.part.stride == 1 ? 0 : static_cast<uint64_t>(rows) * a.heads * p.few.part.stride;
   return p;
-}
-
-uint64_t partial_floats(const SeqAttnArgs &a, const Partials &p) {
-  return p.splits == 1 ? 0 : uint64_t(a.seqs.rows) * a.heads * p.splits;
 }
 
 }  // namespace
 
-uint64_t seq_attn_ws_bytes(const SeqAttnArgs &a) {
-  return partial_floats(a, plan_few(a).part) * (HD * 4 + 8);
-}
+uint64_t seq_attn_ws_bytes(const SeqAttnArgs &a) { return plan_attn(a).slots * (HD * 4 + 8); }
 
-hipError_t launch_seq_attn(const SeqAttnArgs &a, hipStream_t s) {
-  if (a.seqs.rows == 0 || a.seqs.n_seq == 0) return hipSuccess;
-  FewPlan p = plan_few(a);
-  const uint64_t slots = partial_floats(a, p.part);
-  p.part.o = static_cast<float *>(a.ws);
-  p.part.ml = reinterpret_cast<float2 *>(p.part.o + slots * HD);
-  const int64_t wgs = cdiv(p.units * p.part.splits, 8) * 8 * a.kv_heads;
-  if (wgs > kMaxGrid) return hipErrorInvalidValue;
-  const dim3 grid(static_cast<unsigned>(wgs));
+hipError_t launch_seq_attn(const SeqAttnArgs &args, hipStream_t s) {
+  if (args.seqs.rows == 0 || args.seqs.n_seq == 0) return hipSuccess;
+  SeqAttnArgs a = args;
+  a.out_words = a.out && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && (a.ldo & 3) == 0;
+  Plan p = plan_attn(a);
+  p.few.part.o = p.wide.part.o = static_cast<float *>(a.ws);
+  p.few.part.ml = p.wide.part.ml = reinterpret_cast<float2 *>(p.few.part.o + p.slots * HD);
+  const int64_t few = cdiv(p.few.units * p.few.part.splits, 8) * 8 * a.kv_heads;
+  const int64_t wide = p.any_wide ? p.wide.tiles * p.wide.part.splits * a.kv_heads : 0;
+  if (few > kMaxGrid || wide > kMaxGrid) return hipErrorInvalidValue;
+  if (wide) {
+    hipLaunchKernelGGL(seq_attn_wide_kernel, dim3(static_cast<unsigned>(wide)), dim3(256), 0, s, a, p.wide);
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  }
   if (a.ids)
-    hipLaunchKernelGGL(seq_attn_few_kernel<true>, grid, dim3(64 * FEW_WAVES), 0, s, a, p);
+    hipLaunchKernelGGL(seq_attn_few_kernel<true>, dim3(static_cast<unsigned>(few)), dim3(64 * FEW_WAVES), 0, s, a, p.few);
   else
-    hipLaunchKernelGGL(seq_attn_few_kernel<false>, grid, dim3(64 * FEW_WAVES), 0, s, a, p);
-  if (const hipError_t e = hipGetLastError(); e != hipSuccess || p.part.splits == 1) return e;
+    hipLaunchKernelGGL(seq_attn_few_kernel<false>, dim3(static_cast<unsigned>(few)), dim3(64 * FEW_WAVES), 0, s, a, p.few);
+  if (const hipError_t e = hipGetLastError(); e != hipSuccess || p.slots == 0) return e;
   hipLaunchKernelGGL(seq_attn_join_kernel, dim3(static_cast<unsigned>(int64_t(a.seqs.rows) * a.heads)), dim3(256), 0, s, a,
-                     p.part, a.ids != nullptr, p.most);
+                     p.few.part, p.wide.part, FEW_MOST);
   return hipGetLastError();
 }
 

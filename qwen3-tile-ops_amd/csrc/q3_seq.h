@@ -114,6 +114,7 @@ struct SeqAttnArgs {
   int n_sel;
   float *out;          // f32 rows, or
   int64_t ldo;
+  bool out_words;      // (the launcher's: rows that 16-byte stores fit)
   int8_t *o8;          // int8 rows with one scale per head
   int64_t ldo8;
   float *os;

@@ -16,7 +16,8 @@ using q3::no_data;
 using q3::unsupported;
 
 constexpr uint32_t kMaxTokens = 1u << 30;  // positions are 32-bit on the device
-constexpr uint32_t kMaxRows = 1u << 22;    // rows x heads workgroups fit a launch
+constexpr uint32_t kMaxRows = 1u << 21;    // rows x heads, and twice that, are 32-bit too
+constexpr int kMaxHeads = 512;
 
 bool aligned(const void *p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
@@ -47,7 +48,7 @@ int seq_common(const q3_paged_kv *kv, const q3_seqs *q, uint32_t rows, int kv_he
 // Queries [rows][heads * 128] int8 with a scale per head.
 int check_queries(const q3_view *q8, const q3_view *q_scale, int heads, int kv_heads) {
   Q3_TRY(check_view(q8, Q3_DT_I8));
-  if (heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads > 1024) return Q3_ERR_ARG;
+  if (heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads > kMaxHeads) return Q3_ERR_ARG;
   if (q8->cols < static_cast<uint32_t>(heads) * 128) return Q3_ERR_VIEW;
   if (q8->row_bytes % 16 || !aligned(q8->data, 16)) return Q3_ERR_VIEW;
   return check_scales(q_scale, q8->rows, static_cast<uint32_t>(heads));
@@ -118,7 +119,7 @@ int append(const q3_view *q, const q3_view *k, const q3_view *v, const q3_view *
   Q3_TRY(check_view(k, Q3_DT_F32));
   Q3_TRY(check_view(v, Q3_DT_F32));
   const uint32_t rows = k->rows;
-  if (kv_heads <= 0 || kv_heads > 1024 || heads < 0 || heads > 1024) return Q3_ERR_ARG;
+  if (kv_heads <= 0 || kv_heads > kMaxHeads || heads < 0 || heads > kMaxHeads) return Q3_ERR_ARG;
   if (!q != (heads == 0) || !q != !q8 || !q8 != !qs || (!q && nwq)) return Q3_ERR_ARG;
   if (v->rows != rows || k->cols < kv_heads * 128u || v->cols < kv_heads * 128u) return Q3_ERR_VIEW;
   if (!aligned(k->data, 4) || !aligned(v->data, 4)) return Q3_ERR_VIEW;
@@ -280,7 +281,7 @@ int q3_attention_pages(const q3_view *q8, const q3_view *q_scale, const q3_paged
 
 int q3_seqs_workspace(const q3_seqs *seqs, uint32_t rows, uint32_t page_tokens, int heads, int kv_heads, uint32_t n_sel,
                       uint64_t *bytes) {
-  if (!seqs || !bytes || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads > 1024 || page_tokens == 0) return Q3_ERR_ARG;
+  if (!seqs || !bytes || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads > kMaxHeads || page_tokens == 0) return Q3_ERR_ARG;
   if (seqs->n_seq > 65535 || rows > kMaxRows || seqs->max_kv > kMaxTokens || seqs->max_rows > kMaxRows ||
       page_tokens > kMaxTokens || n_sel > 65536)
     return Q3_ERR_RANGE;

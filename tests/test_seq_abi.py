@@ -90,7 +90,7 @@ def test_append_refused(lib):
                    (dict(nwq=V(64, 1, DT_F32)), VIEW), (dict(nwk=V(128, 1, DT_I8)), DTYPE), (dict(cos=None), ARG),
                    (dict(cos=None, sin=None), ARG), (dict(rot=0), ARG), (dict(rot=130), UNSUPPORTED), (dict(rot=63), UNSUPPORTED),
                    (dict(cos=V(99, 64, DT_F32), sin=V(99, 64, DT_F32)), RANGE), (dict(sin=V(100, 65, DT_F32)), VIEW),
-                   (dict(cos=V(100, 63, DT_F32), sin=V(100, 63, DT_F32)), VIEW), (dict(kvh=1025), ARG)]:
+                   (dict(cos=V(100, 63, DT_F32), sin=V(100, 63, DT_F32)), VIEW), (dict(kvh=513), ARG)]:
         assert append(lib, **kw) == rc, kw
 
 
