@@ -129,13 +129,13 @@ __device__ __forceinline__ void store_row8(const SeqAttnArgs &a, int row, int he
   if (d0 == 0) a.os[row * a.ldos + head * a.os_col] = scale;
 }
 
-// Partial results of a (row, head) by split: the unnormalised O, its maximum and
-// its sum.  A row's splits are those of the kernel that takes its sequence.
+// Partial results of a kernel's (row, head) slots by split: the unnormalised O,
+// its maximum and its sum.
 struct Partials {
-  float *o;    // [row * heads + head][split of stride][128]
-  float2 *ml;  // [row * heads + head][split of stride]
+  float *o;    // [slot][split][128]
+  float2 *ml;  // [slot][split]
+  int64_t slots;
   int splits, span;  // keys of a split (listed pages: of the list's keys)
-  int stride;
 };
 
 __device__ __forceinline__ float exp2_from(float x, float base) { return __builtin_amdgcn_exp2f(x - base); }
@@ -161,10 +161,10 @@ constexpr int FEW_SPAN = 64 * KB * FEW_WAVES;  // keys of a split: a lane of eac
 static_assert(FEW_WAVES * FEW_COLS * FEW_ROW * 4 <= FEW_WAVES * FEW_STAGES * FEW_STAGE, "the join fits the stages");
 
 struct FewPlan {
-  Partials part;
-  int64_t units;     // (sequence or row) x tiles of 16 columns
+  Partials part;  // slots: (sequence, KV head, column), of listed pages (row, head)
+  int64_t units;  // (sequence or row) x tiles of 16 columns
   int tiles;
-  int most;          // columns of a sequence that are taken here
+  int most;       // columns of a sequence that are taken here
 };
 
 template <bool LIST>
@@ -395,7 +395,9 @@ __global__ void __launch_bounds__(64 * FEW_WAVES, 2) seq_attn_few_kernel(SeqAttn
     store_row8(a, jrow, jhead, d0, r);
     return;
   }
-  const int64_t at = (static_cast<int64_t>(jrow) * a.heads + jhead) * p.part.stride + split;
+  const int64_t slot = LIST ? static_cast<int64_t>(jrow) * a.heads + jhead
+                            : (static_cast<int64_t>(seq) * a.kv_heads + kvh) * p.most + cc;
+  const int64_t at = slot * p.part.splits + split;
   v4f *dst = reinterpret_cast<v4f *>(p.part.o + at * HD + d0);
   dst[0] = v4f{r[0], r[1], r[2], r[3]};
   dst[1] = v4f{r[4], r[5], r[6], r[7]};
@@ -422,7 +424,7 @@ constexpr int WIDE_SPAN = 32768;  // keys of a split: its page ids lie in LDS
 constexpr int WIDE_OROW = 32 + 4;  // floats of a column's row where the results turn
 
 struct WidePlan {
-  Partials part;
+  Partials part;  // slots: (row, head)
   int64_t tiles;  // at most
   int least;      // columns of a sequence that are taken here
 };
@@ -666,7 +668,7 @@ __global__ void __launch_bounds__(256, 2) seq_attn_wide_kernel(SeqAttnArgs a, Wi
     l = __uint_as_float(pr.a) + __uint_as_float(pr.b);
   }
   const bool whole = p.part.splits == 1;
-  const int64_t at = whole || !live ? 0 : (static_cast<int64_t>(row) * a.heads + head) * p.part.stride + split;
+  const int64_t at = whole || !live ? 0 : (static_cast<int64_t>(row) * a.heads + head) * p.part.splits + split;
   if (whole) {
     const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
 #pragma unroll
@@ -721,20 +723,38 @@ __global__ void __launch_bounds__(256, 2) seq_attn_wide_kernel(SeqAttnArgs a, Wi
 }
 
 // Joins the splits of a (row, head): 16 lanes of 8 channels, 16 such groups over
-// the splits in turn.
-__global__ void __launch_bounds__(256) seq_attn_join_kernel(SeqAttnArgs a, Partials few, Partials wide, int most) {
+// the splits in turn.  The first workgroups take the slots of the 16-column kernel,
+// the rest those of the 128-column one.
+__global__ void __launch_bounds__(256) seq_attn_join_kernel(SeqAttnArgs a, FewPlan fp, WidePlan wp) {
   __shared__ float o_s[4][HD];
   __shared__ float sum_s[4];
-  const int row = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
-  const int seq = seq_of_row(a.seqs, row);
-  if (seq >= a.seqs.n_seq) return;
-  const SeqSpan sp = seq_span(a.seqs, seq);
-  if (row < sp.r0 || row >= sp.r0 + sp.n) return;
-  const Partials &p = !a.ids && sp.n * (a.heads / a.kv_heads) > most ? wide : few;
-  if (p.splits == 1) return;  // written as it is
+  const bool few = blockIdx.x < fp.part.slots;
+  const Partials &p = few ? fp.part : wp.part;
+  const int64_t slot = blockIdx.x - (few ? 0 : fp.part.slots);
+  const int group_heads = a.heads / a.kv_heads;
+  int seq, row, head;
+  SeqSpan sp;
+  if (few && !a.ids) {
+    const int c = static_cast<int>(slot % fp.most);
+    const int sh = static_cast<int>(slot / fp.most);
+    seq = sh / a.kv_heads;
+    sp = seq_span(a.seqs, seq);
+    const int cols = sp.n * group_heads;
+    if (c >= cols || cols > fp.most) return;
+    row = sp.r0 + c / group_heads;
+    head = sh % a.kv_heads * group_heads + c % group_heads;
+  } else {
+    row = static_cast<int>(slot / a.heads);
+    head = static_cast<int>(slot % a.heads);
+    seq = seq_of_row(a.seqs, row);
+    if (seq >= a.seqs.n_seq) return;
+    sp = seq_span(a.seqs, seq);
+    if (row < sp.r0 || row >= sp.r0 + sp.n) return;
+    if (!few && sp.n * group_heads < wp.least) return;
+  }
   const int sees = a.causal ? max(sp.pos(row) + 1, 0) : sp.kv;
   const int n = a.ids ? p.splits : (sees + p.span - 1) / p.span;
-  const int64_t at = (static_cast<int64_t>(row) * a.heads + head) * p.stride;
+  const int64_t at = slot * p.splits;
   float top = -INFINITY;
   for (int s = threadIdx.x & 63; s < n; s += 64) top = fmaxf(top, p.ml[at + s].x);
   top = max64(top);
@@ -799,7 +819,6 @@ struct Plan {
   FewPlan few;
   WidePlan wide;
   bool any_wide;
-  uint64_t slots;  // of partial results
 };
 
 Plan plan_attn(const SeqAttnArgs &a) {
@@ -807,39 +826,46 @@ Plan plan_attn(const SeqAttnArgs &a) {
   const int64_t g = a.heads / a.kv_heads, rows = a.seqs.rows, n_seq = a.seqs.n_seq;
   const int64_t cols = a.ids ? g : a.seqs.max_rows * g;  // of a sequence (listed pages: of a row), at most
   p.any_wide = !a.ids && cols > FEW_MOST;
-  const int64_t few_cols = p.any_wide ? FEW_MOST : cols;
-  p.few.most = FEW_MOST;
-  p.few.tiles = static_cast<int>(few_cols < 1 ? 1 : cdiv(few_cols, FEW_COLS));
+  const int64_t few_cols = p.any_wide ? FEW_MOST : cols < 1 ? 1 : cols;
+  p.few.most = static_cast<int>(few_cols);
+  p.few.tiles = static_cast<int>(cdiv(few_cols, FEW_COLS));
   p.few.units = (a.ids ? rows : n_seq) * p.few.tiles;
   plan_splits(p.few.units * a.kv_heads, a.ids ? int64_t(a.n_sel) * a.pool.page_tokens : a.seqs.max_kv, 2048, FEW_WAVES * KB, 256,
               FEW_SPAN, p.few.part);
-  p.few.part.stride = p.few.part.splits;
+  if (p.few.part.splits > 1) p.few.part.slots = a.ids ? rows * a.heads : n_seq * a.kv_heads * few_cols;
   if (p.any_wide) {
     p.wide.least = FEW_MOST + 1;
     const int64_t wide_seqs = rows * g / p.wide.least;
     p.wide.tiles = rows * g / WIDE_COLS + (n_seq < wide_seqs ? n_seq : wide_seqs);
     plan_splits(p.wide.tiles * a.kv_heads, a.seqs.max_kv, 512, WIDE_KEYS, 512, WIDE_SPAN, p.wide.part);
-    if (p.wide.part.splits > p.few.part.stride) p.few.part.stride = p.wide.part.splits;
-    p.wide.part.stride = p.few.part.stride;
+    if (p.wide.part.splits > 1) p.wide.part.slots = rows * a.heads;
   }
-  p.slots = p.few.part.stride == 1 ? 0 : static_cast<uint64_t>(rows) * a.heads * p.few.part.stride;
   return p;
 }
 
+int64_t partials(const Partials &p) { return p.slots * p.splits; }
+
 }  // namespace
 
-uint64_t seq_attn_ws_bytes(const SeqAttnArgs &a) { return plan_attn(a).slots * (HD * 4 + 8); }
+uint64_t seq_attn_ws_bytes(const SeqAttnArgs &a) {
+  const Plan p = plan_attn(a);
+  return static_cast<uint64_t>(partials(p.few.part) + partials(p.wide.part)) * (HD * 4 + 8);
+}
 
 hipError_t launch_seq_attn(const SeqAttnArgs &args, hipStream_t s) {
   if (args.seqs.rows == 0 || args.seqs.n_seq == 0) return hipSuccess;
   SeqAttnArgs a = args;
   a.out_words = a.out && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && (a.ldo & 3) == 0;
   Plan p = plan_attn(a);
-  p.few.part.o = p.wide.part.o = static_cast<float *>(a.ws);
-  p.few.part.ml = p.wide.part.ml = reinterpret_cast<float2 *>(p.few.part.o + p.slots * HD);
+  const int64_t nf = partials(p.few.part), nw = partials(p.wide.part);
+  p.few.part.o = static_cast<float *>(a.ws);
+  p.wide.part.o = p.few.part.o + nf * HD;
+  p.few.part.ml = reinterpret_cast<float2 *>(p.wide.part.o + nw * HD);
+  p.wide.part.ml = p.few.part.ml + nf;
   const int64_t few = cdiv(p.few.units * p.few.part.splits, 8) * 8 * a.kv_heads;
   const int64_t wide = p.any_wide ? p.wide.tiles * p.wide.part.splits * a.kv_heads : 0;
-  if (few > kMaxGrid || wide > kMaxGrid) return hipErrorInvalidValue;
+  const int64_t join = p.few.part.slots + p.wide.part.slots;
+  if (few > kMaxGrid || wide > kMaxGrid || join > kMaxGrid) return hipErrorInvalidValue;
   if (wide) {
     hipLaunchKernelGGL(seq_attn_wide_kernel, dim3(static_cast<unsigned>(wide)), dim3(256), 0, s, a, p.wide);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
@@ -848,9 +874,8 @@ hipError_t launch_seq_attn(const SeqAttnArgs &args, hipStream_t s) {
     hipLaunchKernelGGL(seq_attn_few_kernel<true>, dim3(static_cast<unsigned>(few)), dim3(64 * FEW_WAVES), 0, s, a, p.few);
   else
     hipLaunchKernelGGL(seq_attn_few_kernel<false>, dim3(static_cast<unsigned>(few)), dim3(64 * FEW_WAVES), 0, s, a, p.few);
-  if (const hipError_t e = hipGetLastError(); e != hipSuccess || p.slots == 0) return e;
-  hipLaunchKernelGGL(seq_attn_join_kernel, dim3(static_cast<unsigned>(int64_t(a.seqs.rows) * a.heads)), dim3(256), 0, s, a,
-                     p.few.part, p.wide.part, FEW_MOST);
+  if (const hipError_t e = hipGetLastError(); e != hipSuccess || join == 0) return e;
+  hipLaunchKernelGGL(seq_attn_join_kernel, dim3(static_cast<unsigned>(join)), dim3(256), 0, s, a, p.few, p.wide);
   return hipGetLastError();
 }
 
