@@ -20,6 +20,8 @@
 // 2-norm: two numbers leave 2.3e-6, three 2e-7 at 2000 keys, where f32 sums in torch leave 6e-7;
 // one would leave 1.6e-3), V as bf16, which holds every int8.  bf16 because the
 // range of the V scales is the user's, which f16 does not hold.
+#include <type_traits>
+
 #include "q3_attn_v.h"
 #include "q3_seq.h"
 
@@ -31,6 +33,8 @@ typedef float v2f __attribute__((ext_vector_type(2)));
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -89,6 +93,39 @@ __device__ __forceinline__ v8bf int8_bf16(v2i_d w) {
     r[2 * i + 1] = pack_bf16(f[2], f[3]);
   }
   return __builtin_bit_cast(v8bf, r);
+}
+
+// The same in f16: x as two numbers (2^-22 of it while it is above 2^-3; below,
+// 2^-25), int8 exactly: 0x64 over the byte with its sign bit turned is 1024 + 128 + b.
+struct F16x2 {
+  v8h part[2];
+};
+__device__ __forceinline__ F16x2 split_f16(const float (&x)[8]) {
+  v4u w[2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const v2f t = {x[2 * i], x[2 * i + 1]};
+    w[0][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(t, v2h));
+    // what is left, x - h with h read as f16 (exact)
+    v2f r;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r.x) : "v"(w[0][i]), "v"(t.x));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r.y) : "v"(w[0][i]), "v"(t.y));
+    w[1][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, v2h));
+  }
+  F16x2 p;
+  p.part[0] = __builtin_bit_cast(v8h, w[0]);
+  p.part[1] = __builtin_bit_cast(v8h, w[1]);
+  return p;
+}
+__device__ __forceinline__ v8h int8_f16(v2i_d w) {
+  v4u r;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t u = static_cast<uint32_t>(w[i]) ^ 0x80808080u;
+    r[2 * i] = __builtin_amdgcn_perm(0x64646464u, u, 0x07010700u);
+    r[2 * i + 1] = __builtin_amdgcn_perm(0x64646464u, u, 0x07030702u);
+  }
+  return __builtin_bit_cast(v8h, r) - static_cast<_Float16>(1152.0f);
 }
 
 template <int N>
@@ -167,19 +204,23 @@ struct FewPlan {
   int most;       // columns of a sequence that are taken here
 };
 
+struct FewLds {
+  __align__(16) uint8_t stage[FEW_WAVES * FEW_STAGES * FEW_STAGE];
+  float m[FEW_WAVES][FEW_COLS], l[FEW_WAVES][FEW_COLS];
+};
+
+// (block: of the workgroups that the plan asks for)
 template <bool LIST>
-__global__ void __launch_bounds__(64 * FEW_WAVES, 2) seq_attn_few_kernel(SeqAttnArgs a, FewPlan p) {
-  __shared__ __align__(16) uint8_t stage_s[FEW_WAVES * FEW_STAGES * FEW_STAGE];
-  __shared__ float m_s[FEW_WAVES][FEW_COLS], l_s[FEW_WAVES][FEW_COLS];
+__device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, FewLds &lds) {
   const int lane = threadIdx.x & 63, wave = wave_id();
   const int col = lane & 15, quarter = lane >> 4;
 
   // Workgroups go round the 8 XCDs: the KV heads of one (unit, split) share an
   // XCD, whose L2 then holds the lines of scales that they share.
   const int group_heads = a.heads / a.kv_heads;
-  const int rest = blockIdx.x >> 3;
+  const int rest = block >> 3;
   const int kvh = rest % a.kv_heads;
-  const int us = (rest / a.kv_heads) * 8 + (blockIdx.x & 7);
+  const int us = (rest / a.kv_heads) * 8 + (block & 7);
   const int unit = us / p.part.splits, split = us % p.part.splits;
   if (unit >= p.units) return;
   const int tile = unit % p.tiles;
@@ -252,7 +293,7 @@ __global__ void __launch_bounds__(64 * FEW_WAVES, 2) seq_attn_few_kernel(SeqAttn
     cs = a.qs[row * a.ldqs + (kvh * group_heads + g) * a.qs_col] * a.qk_scale * kLog2e;
   }
 
-  uint8_t *const stages = stage_s + wave * FEW_STAGES * FEW_STAGE;
+  uint8_t *const stages = lds.stage + wave * FEW_STAGES * FEW_STAGE;
   const int r8 = lane >> 3, ch = lane & 7;
   const int64_t lane_k = r8 * a.pool.row_bytes + 16 * (ch ^ r8);
   const int64_t lane_v = r8 * a.pool.row_bytes + 16 * (ch ^ (r8 & 3));
@@ -365,24 +406,24 @@ __global__ void __launch_bounds__(64 * FEW_WAVES, 2) seq_attn_few_kernel(SeqAttn
   // join the waves: each column's rows of O by wave, and (m, l)
   l = col_sum(l);
   __syncthreads();  // every wave is done with its stages
-  float *join = reinterpret_cast<float *>(stage_s);
+  float *join = reinterpret_cast<float *>(lds.stage);
 #pragma unroll
   for (int t = 0; t < 8; ++t)
     *reinterpret_cast<v4f *>(join + (wave * FEW_COLS + col) * FEW_ROW + 16 * t + 4 * quarter) = o[t];
-  if (quarter == 0) m_s[wave][col] = m, l_s[wave][col] = l;
+  if (quarter == 0) lds.m[wave][col] = m, lds.l[wave][col] = l;
   __syncthreads();
   const int jc = threadIdx.x >> 4, d0 = 8 * (threadIdx.x & 15);
   const int cc = tile * FEW_COLS + jc;
   if (cc >= cols) return;
-  float top = m_s[0][jc];
+  float top = lds.m[0][jc];
 #pragma unroll
-  for (int w = 1; w < FEW_WAVES; ++w) top = fmaxf(top, m_s[w][jc]);
+  for (int w = 1; w < FEW_WAVES; ++w) top = fmaxf(top, lds.m[w][jc]);
   const float base = top == -INFINITY ? 0.0f : top;
   float sum = 0.0f, r[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
   for (int w = 0; w < FEW_WAVES; ++w) {
-    const float f = exp2_from(m_s[w][jc], base);
-    sum += f * l_s[w][jc];
+    const float f = exp2_from(lds.m[w][jc], base);
+    sum += f * lds.l[w][jc];
     const float *src = join + (w * FEW_COLS + jc) * FEW_ROW + d0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) r[i] += f * src[i];
@@ -407,21 +448,38 @@ __global__ void __launch_bounds__(64 * FEW_WAVES, 2) seq_attn_few_kernel(SeqAttn
 // ---- many columns: 128 to a tile -----------------------------------------------
 //
 // A workgroup takes one tile of 128 columns and one KV head; each of its four waves
-// has 32 columns, and all share the keys, 64 a step.  K [64][128] goes to the K
-// operand's LDS image as it is; V int8 is turned once for all four waves into the
-// bf16 image of the A operand of V^T P^T (a quarter of it by each wave: a
-// transposing read hands a lane 8 keys of one channel, in the order in which P's
-// keys lie in the registers).  While a step's scores and products are computed, the
-// next step's V is turned and its K and the V after next are copied, so a step has
-// one barrier.  What a step costs a SIMD: 8 int8 MFMAs for S (256 cycles), 48 bf16
-// ones for P V (1536), and about 15 VALU instructions per (key, column) lane.
+// has 32 columns, and all share the keys, 32 a step.  K [32][128] goes to the K
+// operand's LDS image as it is; V int8 is turned once for all waves into the 16-bit
+// image of the A operand of V^T P^T (a quarter of it by each wave: a transposing read
+// hands a lane 8 keys of one channel, in the order in which P's keys lie in the
+// registers).  A wave works on a step's values beside the next step's products,
+// whose operands have nothing in common, and the copies of four steps are in LDS or
+// in flight: one barrier a step.
+//
+// A matrix instruction takes 33 cycles of its SIMD, under which four to five vector
+// instructions go for nothing; each further one costs 2.5, a conversion from int32 4
+// and an exponential 8 (measured).  So the number of vector instructions counts as
+// much as that of the 20 matrix ones a step: two terms of P instead of three, keys'
+// scales in the scores but the column's in the exponent's FMA, a reference that moves
+// by steps of 2^8, whole steps without a mask in a loop of their own.
+//
+// P: where the split's V scales lie within a factor of 16 of each other (as they do
+// but for crafted caches) p * vs fits two f16 numbers, with a reference that puts
+// the largest at 2^7 .. 2^15: 22 bits down to 2^-10 of it, and nothing is off by more
+// than 2^-25 / 2^7.  Otherwise the three bf16 numbers of the 16-column kernel.
+//
+// Two workgroups a CU: a third would fit LDS, but not the registers (spills cost more
+// than it gives), and eight waves that halve the keys were slower for whole prompts.
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef int v16i __attribute__((ext_vector_type(16)));
 
 constexpr int WIDE_COLS = 128;
-constexpr int WIDE_KEYS = 64;
-constexpr int WIDE_SPAN = 32768;  // keys of a split: its page ids lie in LDS
+constexpr int WIDE_KEYS = KB;      // of a step
+constexpr int WIDE_WAVES = 4;
+constexpr int WIDE_DEPTH = 4;      // steps whose K and V lie in LDS or on their way
+constexpr int WIDE_SPAN = 8192;   // keys of a split: its blocks' places lie in LDS
 constexpr int WIDE_OROW = 32 + 4;  // floats of a column's row where the results turn
+constexpr float WIDE_ROOM = 8.0f;  // P may reach 2^8 of its reference before O is scaled down
 
 struct WidePlan {
   Partials part;  // slots: (row, head)
@@ -433,20 +491,28 @@ struct WidePlan {
 // transposing read (two runs of four, 8 apart) meet 8 chunks.
 __device__ __forceinline__ int vswz_wide(int key) { return (key & 3) | ((key >> 1) & 4); }
 
-__global__ void __launch_bounds__(256, 2) seq_attn_wide_kernel(SeqAttnArgs a, WidePlan p) {
-  __shared__ __align__(16) uint8_t k_s[2][WIDE_KEYS * HD];
-  __shared__ __align__(16) uint8_t v8_s[2][WIDE_KEYS * HD];
-  __shared__ __align__(16) uint8_t vb_s[2][WIDE_KEYS * HD * 2];
-  __shared__ __align__(16) float sc_s[3][2 * WIDE_KEYS];  // ks, then vs
-  __shared__ int page_s[WIDE_SPAN / KB];
-  static_assert(sizeof(vb_s) >= 4 * 32 * WIDE_OROW * 4, "the results fit where V was");
+struct WideLds {
+  struct Stages {
+    uint8_t vt[2][WIDE_KEYS * HD * 2];
+    uint8_t k[WIDE_DEPTH][WIDE_KEYS * HD];
+    uint8_t v8[WIDE_DEPTH][WIDE_KEYS * HD];
+  };
+  static_assert(sizeof(Stages) >= 4 * 32 * WIDE_OROW * 4, "the results fit where the steps were");
+  __align__(16) Stages st;
+  __align__(16) float sc[2 * WIDE_DEPTH][2 * WIDE_KEYS];  // of a step's block ks, then vs
+  int2 block[WIDE_SPAN / KB];                             // page, first token
+  uint32_t range[2];
+};
+
+__device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block, WideLds &lds) {
+  WideLds::Stages &st = lds.st;
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
   const int half = lane >> 5, n32 = lane & 31;
   const int group_heads = a.heads / a.kv_heads;
 
   // which sequence's tile this is: tiles of the sequences before, 64 at a time
-  const int kvh = blockIdx.x % a.kv_heads;
-  const int64_t us = blockIdx.x / a.kv_heads;
+  const int kvh = block % a.kv_heads;
+  const int64_t us = block / a.kv_heads;
   const int split = us % p.part.splits;
   int64_t nth = us / p.part.splits;
   int seq = -1;
@@ -481,22 +547,15 @@ __global__ void __launch_bounds__(256, 2) seq_attn_wide_kernel(SeqAttnArgs a, Wi
   const bool live = c < cols;
   const int row = sp.r0 + c / group_heads, head = kvh * group_heads + c % group_heads;
   const int sees = !live ? 0 : a.causal ? max(sp.pos(row) + 1, 0) : sp.kv;
-  // the wave's first column sees the fewest keys of its columns; the tile's last
-  // the most of all
-  const int vmin = __builtin_amdgcn_readfirstlane(sees);
-  const int rest = min(cols - (col0 + wave * 32), 32);
-  const int vmax = rest <= 0 ? 0 : __builtin_amdgcn_readlane(sees, max(rest, 1) - 1);
+  // the fewest and the most keys that a column sees: the first row's, the last's
+  const int first_row = sp.r0 + col0 / group_heads;
   const int last_row = sp.r0 + (min(cols, col0 + WIDE_COLS) - 1) / group_heads;
+  const int tile_min = a.causal ? max(sp.pos(first_row) + 1, 0) : sp.kv;
   const int tile_max = a.causal ? max(sp.pos(last_row) + 1, 0) : sp.kv;
   const int first = split * p.part.span;
   const int end = min(tile_max, first + p.part.span);
   if (split > 0 && first >= tile_max) return;
   const int steps = (end - first + WIDE_KEYS - 1) / WIDE_KEYS;  // <= 0: none
-
-  for (int i = tid; i < steps * (WIDE_KEYS / KB); i += 256) {
-    const int key = first + i * KB;
-    page_s[i] = key < end ? seq_page(a.seqs, a.pool, seq, key / pt) : -1;
-  }
 
   v4i_d qf[4];
 #pragma unroll
@@ -508,159 +567,227 @@ __global__ void __launch_bounds__(256, 2) seq_attn_wide_kernel(SeqAttnArgs a, Wi
     for (int i = 0; i < 4; ++i) qf[i] = *reinterpret_cast<const v4i_d *>(q + 32 * i);
     cs = a.qs[row * a.ldqs + head * a.qs_col] * a.qk_scale * kLog2e;
   }
-  __syncthreads();
 
-  // Copies: wave w takes keys 16 w .. 16 w + 15 of a step, all in one 32-key block.
-  const int r8 = lane >> 3, ch = lane & 7;
-  const int64_t lane_k = (16 * wave + r8) * a.pool.row_bytes + 16 * (ch ^ r8);
-  const int64_t lane_v[2] = {(16 * wave + r8) * a.pool.row_bytes + 16 * (ch ^ (r8 & 3)),
-                             (16 * wave + r8) * a.pool.row_bytes + 16 * (ch ^ ((r8 & 3) | 4))};
-  // (page and first token of a step's 32-key block)
-  auto block_at = [&](int step, int b, int *t0) {
-    *t0 = (first + step * WIDE_KEYS + b * KB) % pt;
-    return __builtin_amdgcn_readfirstlane(page_s[step * 2 + b]);
-  };
-  auto copy_k = [&](int step) {
-    int t0;
-    const int b = wave >> 1, page = block_at(step, b, &t0);
-    if (page >= 0) {
-      const int8_t *k = a.pool.k + page * a.pool.page_bytes + (t0 - b * KB) * a.pool.row_bytes + kvh * HD + lane_k;
-#pragma unroll
-      for (int q = 0; q < 2; ++q) lds_copy16(k + q * 8 * a.pool.row_bytes, k_s[step & 1] + (2 * wave + q) * 1024);
-    }
-  };
-  auto copy_v = [&](int step) {
-    int t0;
-    const int b = wave >> 1, page = block_at(step, b, &t0);
-    if (page >= 0) {
-      const int8_t *v = a.pool.v + page * a.pool.page_bytes + (t0 - b * KB) * a.pool.row_bytes + kvh * HD;
-#pragma unroll
-      for (int q = 0; q < 2; ++q) lds_copy16(v + q * 8 * a.pool.row_bytes + lane_v[q], v8_s[step & 1] + (2 * wave + q) * 1024);
-    }
-    if (wave < 2) {  // wave 0: the K scales of the step's 64 keys, wave 1: V's
-      int ta, tb;
-      const int pa = block_at(step, 0, &ta), pb = block_at(step, 1, &tb);
-      if (pa >= 0 || pb >= 0) {
-        // (a block without a page is masked: the other's scales will do)
-        const int page2 = (lane < KB || pb < 0) && pa >= 0 ? pa : pb, t = (lane < KB ? ta : tb) + n32;
-        const float *src = wave == 0 ? a.pool.ks : a.pool.vs;
-        lds_copy4(src + page2 * a.pool.spage + t * a.pool.srow + kvh, sc_s[step % 3] + wave * WIDE_KEYS);
+  // the split's blocks, and the range of its V scales' magnitudes (as integers;
+  // zeros aside), 32 lanes a block
+  if (tid < 2) lds.range[tid] = tid == 0 ? 0u : 0x7f800000u;
+  __syncthreads();
+  bool hole = false;
+  {
+    uint32_t most = 0, least = 0x7f800000u;
+#pragma unroll 4
+    for (int i = tid >> 5; i < steps; i += 2 * WIDE_WAVES) {
+      const int key = first + i * KB;
+      const int2 at = key < end ? make_int2(seq_page(a.seqs, a.pool, seq, key / pt), key % pt) : make_int2(-1, 0);
+      hole |= key < end && at.x < 0;
+      if (n32 == 0) lds.block[i] = at;
+      if (at.x >= 0 && key + n32 < end) {
+        const uint32_t v = __float_as_uint(a.pool.vs[at.x * a.pool.spage + (at.y + n32) * a.pool.srow + kvh]) & 0x7fffffffu;
+        most = max(most, v);
+        if (v) least = min(least, v);
       }
     }
-  };
-  // A quarter of a step's V: channels 32 wave .. + 31 of its four 16-key runs.
-  const int vj = (lane & 15) >> 1;
-  const int vkey = 8 * (vj >> 2) + 4 * half + (vj & 3);
-  auto turn_v = [&](int step) {
 #pragma unroll
-    for (int kc = 0; kc < 4; ++kc) {
-      const int key = 16 * kc + vkey, chunk = 2 * wave + ((lane >> 4) & 1);
-      const uint8_t *src = v8_s[step & 1] + key * HD + 16 * (chunk ^ vswz_wide(key)) + 8 * (lane & 1);
-      const v8bf w = int8_bf16(__builtin_amdgcn_ds_read_tr8_b64_v2i32(reinterpret_cast<lds_v2i_ptr_d>(to_lds(src))));
-      *reinterpret_cast<v8bf *>(vb_s[step & 1] + ((kc * 4 + wave) * 64 + lane) * 16) = w;
+    for (int d = 1; d < 64; d *= 2) {
+      most = max(most, lane_xor_m(most, d));
+      least = min(least, lane_xor_m(least, d));
     }
+    if (lane == 0) {
+      atomicMax(&lds.range[0], most);
+      atomicMin(&lds.range[1], least);
+    }
+  }
+  const bool missing = __syncthreads_or(hole);
+  const uint32_t most = __builtin_amdgcn_readfirstlane(lds.range[0]), least = __builtin_amdgcn_readfirstlane(lds.range[1]);
+  // Narrow: exponents 4 apart at most, and no closer to the ends than 2^64.
+  const int expo = static_cast<int>(most >> 23) - 127;
+  const bool narrow = most == 0 || (expo >= -64 && expo <= 64 && least >= most - (4u << 23));
+  // with p = 2^(x - base), base = the largest x less `lift`: p vs <= 2^7 there
+  const float lift = narrow && most ? static_cast<float>(6 - expo) : 0.0f;
+
+  // Copies: wave w takes keys 8 w .. 8 w + 7 of a step (of block w / 4).
+  const int r8 = lane >> 3, ch = lane & 7;
+  const int64_t my_row = (8 * wave + r8) * a.pool.row_bytes + kvh * HD;
+  const int64_t lane_k = my_row + 16 * (ch ^ r8), lane_v = my_row + 16 * (ch ^ vswz_wide(8 * wave + r8));
+  auto copy = [&](int step) {
+    int2 at = lds.block[step];
+    at = make_int2(__builtin_amdgcn_readfirstlane(at.x), __builtin_amdgcn_readfirstlane(at.y));
+    if (at.x < 0) return;
+    const int64_t bytes = at.x * a.pool.page_bytes + at.y * a.pool.row_bytes;
+    lds_copy16(a.pool.v + bytes + lane_v, st.v8[step % WIDE_DEPTH] + wave * 8 * HD);
+    lds_copy16(a.pool.k + bytes + lane_k, st.k[step % WIDE_DEPTH] + wave * 8 * HD);
+    if (wave == 0)
+      lds_copy4((half ? a.pool.vs : a.pool.ks) + at.x * a.pool.spage + (at.y + n32) * a.pool.srow + kvh, lds.sc[step % (2 * WIDE_DEPTH)]);
   };
 
-  float m = -INFINITY, l = 0.0f;
+  // The softmax's reference (base 2), at most WIDE_ROOM short of the largest score
+  // less lift, so that O is scaled down a few times in all, not at every new maximum.
+  float base = -INFINITY, l = 0.0f;
   v16f o[4];
 #pragma unroll
   for (int t = 0; t < 4; ++t)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
+  const float size = fabsf(cs);
+  const bool turned = __ballot(cs < 0.0f) != 0;  // some column's scale is negative
 
-  if (steps > 0) {
-    copy_v(0);
-    copy_k(0);
-    wait_copies<0>();
-    lds_barrier();
-    turn_v(0);
-    if (steps > 1) copy_v(1);
-    wait_copies<0>();
-    lds_barrier();
-  }
-  for (int step = 0; step < steps; ++step) {
-    if (step + 2 < steps) copy_v(step + 2);
-    if (step + 1 < steps) {
-      copy_k(step + 1);
-      turn_v(step + 1);
+  // S of a step, as int32.
+  auto products = [&](int step, v16i &s) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const v4i_d kf = *reinterpret_cast<const v4i_d *>(st.k[step % WIDE_DEPTH] + n32 * HD + 16 * ((2 * i + half) ^ (n32 & 7)));
+      s = __builtin_amdgcn_mfma_i32_32x32x32_i8(kf, qf[i], s, 0, 0, 0);
     }
-    const int key0 = first + step * WIDE_KEYS;
-    if (key0 < vmax) {
-      const int pages[2] = {page_s[2 * step], page_s[2 * step + 1]};
-      float x[32];
+  };
+
+  // Their scores but for the column's scale: register i is key 8 (i / 4) + 4 half +
+  // i % 4.  EDGE: some column does not see some key; `seen` keeps which, since
+  // nothing of that key may enter the sums, not even a scale's NaN.
+  float x[16];
+  uint32_t seen = ~0u;
+  auto scores = [&](int step, const v16i &s, auto edge_tag) {
+    constexpr bool EDGE = decltype(edge_tag)::value;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const uint8_t *kr = k_s[step & 1] + (32 * t + n32) * HD;
-        v16i s;
+    for (int i = 0; i < 4; ++i) {
+      const v4f ks = *reinterpret_cast<const v4f *>(lds.sc[step % (2 * WIDE_DEPTH)] + 8 * i + 4 * half);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = 0;
+      for (int j = 0; j < 4; ++j) x[4 * i + j] = static_cast<float>(s[4 * i + j]) * ks[j];
+    }
+    if (turned) {
+      const float sign = __builtin_copysignf(1.0f, cs);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const v4i_d kf = *reinterpret_cast<const v4i_d *>(kr + 16 * ((2 * i + half) ^ (n32 & 7)));
-          s = __builtin_amdgcn_mfma_i32_32x32x32_i8(kf, qf[i], s, 0, 0, 0);
-        }
+      for (int i = 0; i < 16; ++i) x[i] *= sign;
+      asm volatile("");  // a branch, not sixteen selects in every step
+    }
+    seen = ~0u;
+    if constexpr (EDGE) {
+      seen = 0;
+      const int limit = lds.block[step].x < 0 ? 0 : sees - (first + step * WIDE_KEYS + 4 * half);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const v4f ks = *reinterpret_cast<const v4f *>(sc_s[step % 3] + 32 * t + 8 * i + 4 * half);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) x[16 * t + 4 * i + j] = static_cast<float>(s[4 * i + j]) * ks[j] * cs;
-        }
+      for (int i = 0; i < 16; ++i) {
+        const bool in = 8 * (i >> 2) + (i & 3) < limit;
+        seen |= static_cast<uint32_t>(in) << i;
+        if (!in) x[i] = -INFINITY;
       }
-      // register i of a tile is key 8 (i / 4) + 4 half + i % 4
-      const bool edge = key0 + WIDE_KEYS > vmin || pages[0] < 0 || pages[1] < 0;
-      uint32_t seen = ~0u;
-      if (edge) {
-        seen = 0;
+    }
+    float mb = x[0];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const int key = 32 * (i >> 4) + 8 * ((i & 15) >> 2) + 4 * half + (i & 3);
-          const bool s = key0 + key < sees && pages[i >> 4] >= 0;
-          seen |= static_cast<uint32_t>(s) << i;
-          if (!s) x[i] = -INFINITY;
-        }
+    for (int i = 1; i < 16; ++i) mb = fmaxf(mb, x[i]);
+    {
+      const LanePair pr = lane_pair32(__float_as_uint(mb));
+      mb = fmaxf(__uint_as_float(pr.a), __uint_as_float(pr.b));
+    }
+    const float top = mb == -INFINITY ? -INFINITY : mb * size - lift;
+    if (__ballot(top > base + WIDE_ROOM)) {
+      const float to = fmaxf(top, base);
+      const float alpha = base == -INFINITY ? 0.0f : exp2_from(base, to);
+      l *= alpha;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) o[t] *= alpha;
+      base = to;
+    }
+  };
+
+  // P and O += P V of the step whose scores are at hand.
+  auto values = [&](int step, auto edge_tag, auto narrow_tag) {
+    constexpr bool EDGE = decltype(edge_tag)::value;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {  // 16 keys: registers 8 r .. 8 r + 7
+      const float *vs = lds.sc[step % (2 * WIDE_DEPTH)] + KB + 16 * r + 4 * half;
+      const v4f va = *reinterpret_cast<const v4f *>(vs), vc = *reinterpret_cast<const v4f *>(vs + 8);
+      float e[8], pv[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * r + j], size, -base));
+        const bool in = !EDGE || (seen >> (8 * r + j) & 1);
+        if (!in) e[j] = 0.0f;
+        pv[j] = e[j] * (j < 4 ? va[j] : vc[j - 4]);
+        if (!in) pv[j] = 0.0f;
       }
-      float mb = x[0];
+      l += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+      const uint8_t *vt = st.vt[step & 1] + (r * 4 * 64 + lane) * 16;
+      if constexpr (decltype(narrow_tag)::value) {
+        const F16x2 pb = split_f16(pv);
 #pragma unroll
-      for (int i = 1; i < 32; ++i) mb = fmaxf(mb, x[i]);
-      {
-        const LanePair pr = lane_pair32(__float_as_uint(mb));
-        mb = fmaxf(fmaxf(__uint_as_float(pr.a), __uint_as_float(pr.b)), m);
-      }
-      const float base = mb == -INFINITY ? 0.0f : mb;
-      if (__ballot(mb != m)) {
-        const float alpha = exp2_from(m, base);
-        l *= alpha;
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int t = 0; t < 4; ++t) o[t] *= alpha;
-        m = mb;
-      }
-#pragma unroll
-      for (int kc = 0; kc < 4; ++kc) {  // 16 keys: registers 8 kc .. 8 kc + 7
-        const v4f va = *reinterpret_cast<const v4f *>(sc_s[step % 3] + WIDE_KEYS + 16 * kc + 4 * half);
-        const v4f vc = *reinterpret_cast<const v4f *>(sc_s[step % 3] + WIDE_KEYS + 16 * kc + 8 + 4 * half);
-        float pv[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float e = exp2_from(x[8 * kc + j], base);
-          l += e;
-          pv[j] = e * (j < 4 ? va[j] : vc[j - 4]);
-        }
-        if (edge) {  // a scale behind the sequence's end may be anything
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (!(seen >> (8 * kc + j) & 1)) pv[j] = 0.0f;
-        }
+          for (int t = 0; t < 4; ++t)
+            o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const v8h *>(vt + t * 1024), pb.part[u], o[t], 0, 0, 0);
+      } else {
         const Bf16x3 pb = split_bf16(pv);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const v8bf vt = *reinterpret_cast<const v8bf *>(vb_s[step & 1] + ((kc * 4 + t) * 64 + lane) * 16);
+        for (int u = 0; u < 3; ++u)
 #pragma unroll
-          for (int u = 0; u < 3; ++u) o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt, pb.part[u], o[t], 0, 0, 0);
-        }
+          for (int t = 0; t < 4; ++t)
+            o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const v8bf *>(vt + t * 1024), pb.part[u], o[t], 0, 0, 0);
       }
     }
+  };
+
+  // This wave's quarter of a step's V: channels 32 wave .. + 31.
+  const int vj = (lane & 15) >> 1;
+  const int vkey = 8 * (vj >> 2) + 4 * half + (vj & 3);
+  auto turn = [&](int step, auto narrow_tag) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int key = 16 * r + vkey, chunk = 2 * wave + ((lane >> 4) & 1);
+      const uint8_t *src = st.v8[step % WIDE_DEPTH] + key * HD + 16 * (chunk ^ vswz_wide(key)) + 8 * (lane & 1);
+      const v2i_d w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(reinterpret_cast<lds_v2i_ptr_d>(to_lds(src)));
+      uint8_t *dst = st.vt[step & 1] + ((r * 4 + wave) * 64 + lane) * 16;
+      if constexpr (decltype(narrow_tag)::value)
+        *reinterpret_cast<v8h *>(dst) = int8_f16(w);
+      else
+        *reinterpret_cast<v8bf *>(dst) = int8_bf16(w);
+    }
+  };
+
+  int step = 0;
+  auto run = [&](int to, auto edge_tag, auto narrow_tag) {
+    for (; step < to; ++step) {
+      const bool more = !decltype(edge_tag)::value || step + 1 < steps;
+      if (step + WIDE_DEPTH < steps) copy(step + WIDE_DEPTH);
+      v16i s;
+      if (more) {
+        products(step + 1, s);
+        turn(step + 1, narrow_tag);
+      }
+      values(step, edge_tag, narrow_tag);
+      if (more) scores(step + 1, s, edge_tag);
+      // the step after next is needed now; those behind it may be on their way, as
+      // many copies as a wave issues for them (fewer where a page is missing)
+      if (missing || step + WIDE_DEPTH >= steps)
+        wait_copies<0>();
+      else if (wave == 0)
+        wait_copies<3 * (WIDE_DEPTH - 2)>();
+      else
+        wait_copies<2 * (WIDE_DEPTH - 2)>();
+      lds_barrier();
+    }
+  };
+  auto all = [&](auto narrow_tag) {
+#pragma unroll
+    for (int i = 0; i < WIDE_DEPTH; ++i)
+      if (i < steps) copy(i);
     wait_copies<0>();
     lds_barrier();
+    turn(0, narrow_tag);
+    v16i s;
+    products(0, s);
+    scores(0, s, std::true_type{});
+    lds_barrier();
+    // Steps that every column sees whole, then the others (all, where a page is
+    // missing): two loops, since one with both forms of a step keeps O twice.
+    if constexpr (decltype(narrow_tag)::value)
+      run(missing ? 0 : clampi((tile_min - first) / WIDE_KEYS, 0, steps) - 1, std::false_type{}, narrow_tag);
+    run(steps, std::true_type{}, narrow_tag);
+  };
+  if (steps > 0) {
+    if (narrow)
+      all(std::true_type{});
+    else
+      all(std::false_type{});
   }
 
   {
@@ -670,11 +797,11 @@ __global__ void __launch_bounds__(256, 2) seq_attn_wide_kernel(SeqAttnArgs a, Wi
   const bool whole = p.part.splits == 1;
   const int64_t at = whole || !live ? 0 : (static_cast<int64_t>(row) * a.heads + head) * p.part.splits + split;
   if (whole) {
-    const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
+    const float inv = base == -INFINITY ? 0.0f : 1.0f / l;
 #pragma unroll
     for (int t = 0; t < 4; ++t) o[t] *= inv;
   } else if (live && half == 0) {
-    p.part.ml[at] = make_float2(m, l);
+    p.part.ml[at] = make_float2(base, l);
   }
   if (whole && a.o8) {
     float pk = 0.0f;
@@ -695,9 +822,10 @@ __global__ void __launch_bounds__(256, 2) seq_attn_wide_kernel(SeqAttnArgs a, Wi
     if (half == 0) a.os[row * a.ldos + head * a.os_col] = scale;
     return;
   }
-  // f32 rows through LDS (the steps' last barrier is behind every wave, and a
-  // wave keeps to its own part), 32 channels at a time: written in 128-byte pieces
-  float *const turn = reinterpret_cast<float *>(vb_s) + wave * 32 * WIDE_OROW;
+  // f32 rows through LDS (the steps' last barrier is behind every wave, and a wave
+  // keeps to its own part), 32 channels at a time:
+  // written in 128-byte pieces
+  float *const turn_row = reinterpret_cast<float *>(&st) + wave * 32 * WIDE_OROW;
   const int64_t mine = !live ? -1 : whole ? row * a.ldo + head * HD : at * HD;
   float *const to = whole ? a.out : p.part.o;
   const bool words = !whole || a.out_words;
@@ -705,11 +833,11 @@ __global__ void __launch_bounds__(256, 2) seq_attn_wide_kernel(SeqAttnArgs a, Wi
   for (int t = 0; t < 4; ++t) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      *reinterpret_cast<v4f *>(turn + n32 * WIDE_OROW + 8 * i + 4 * half) = v4f{o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]};
+      *reinterpret_cast<v4f *>(turn_row + n32 * WIDE_OROW + 8 * i + 4 * half) = v4f{o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]};
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int64_t off = __shfl(mine, 8 * k + r8);
-      const v4f r = *reinterpret_cast<const v4f *>(turn + (8 * k + r8) * WIDE_OROW + 4 * ch);
+      const v4f r = *reinterpret_cast<const v4f *>(turn_row + (8 * k + r8) * WIDE_OROW + 4 * ch);
       if (off < 0) continue;
       float *dst = to + off + 32 * t + 4 * ch;
       if (words) {
@@ -720,6 +848,27 @@ __global__ void __launch_bounds__(256, 2) seq_attn_wide_kernel(SeqAttnArgs a, Wi
       }
     }
   }
+}
+
+// ---- launches -------------------------------------------------------------------
+
+template <bool LIST>
+__global__ void __launch_bounds__(256, 2) seq_attn_few_kernel(SeqAttnArgs a, FewPlan p) {
+  __shared__ FewLds lds;
+  few_columns<LIST>(a, p, blockIdx.x, lds);
+}
+
+// Both kinds of sequences in one launch, so that short ones fill the CUs beside the
+// long ones: the first `wide` workgroups take the 128-column tiles.
+__global__ void __launch_bounds__(256, 2) seq_attn_mixed_kernel(SeqAttnArgs a, FewPlan fp, WidePlan wp, int wide) {
+  __shared__ union Lds {
+    FewLds few;
+    WideLds wide;
+  } lds;
+  if (static_cast<int>(blockIdx.x) < wide)
+    wide_columns(a, wp, blockIdx.x, lds.wide);
+  else
+    few_columns<false>(a, fp, blockIdx.x - wide, lds.few);
 }
 
 // Joins the splits of a (row, head): 16 lanes of 8 channels, 16 such groups over
@@ -814,6 +963,7 @@ void plan_splits(int64_t units, int64_t keys, int64_t want, int step, int least,
 
 // Sequences of up to FEW_MOST columns go to the kernel of 16-column tiles.
 constexpr int FEW_MOST = 16;
+constexpr int FEW_WANT = 2048, WIDE_WANT = 1536;  // workgroups
 
 struct Plan {
   FewPlan few;
@@ -830,14 +980,14 @@ Plan plan_attn(const SeqAttnArgs &a) {
   p.few.most = static_cast<int>(few_cols);
   p.few.tiles = static_cast<int>(cdiv(few_cols, FEW_COLS));
   p.few.units = (a.ids ? rows : n_seq) * p.few.tiles;
-  plan_splits(p.few.units * a.kv_heads, a.ids ? int64_t(a.n_sel) * a.pool.page_tokens : a.seqs.max_kv, 2048, FEW_WAVES * KB, 256,
+  plan_splits(p.few.units * a.kv_heads, a.ids ? int64_t(a.n_sel) * a.pool.page_tokens : a.seqs.max_kv, FEW_WANT, FEW_WAVES * KB, 256,
               FEW_SPAN, p.few.part);
   if (p.few.part.splits > 1) p.few.part.slots = a.ids ? rows * a.heads : n_seq * a.kv_heads * few_cols;
   if (p.any_wide) {
     p.wide.least = FEW_MOST + 1;
     const int64_t wide_seqs = rows * g / p.wide.least;
     p.wide.tiles = rows * g / WIDE_COLS + (n_seq < wide_seqs ? n_seq : wide_seqs);
-    plan_splits(p.wide.tiles * a.kv_heads, a.seqs.max_kv, 512, WIDE_KEYS, 512, WIDE_SPAN, p.wide.part);
+    plan_splits(p.wide.tiles * a.kv_heads, a.seqs.max_kv, WIDE_WANT, WIDE_KEYS, 512, WIDE_SPAN, p.wide.part);
     if (p.wide.part.splits > 1) p.wide.part.slots = rows * a.heads;
   }
   return p;
@@ -865,15 +1015,15 @@ hipError_t launch_seq_attn(const SeqAttnArgs &args, hipStream_t s) {
   const int64_t few = cdiv(p.few.units * p.few.part.splits, 8) * 8 * a.kv_heads;
   const int64_t wide = p.any_wide ? p.wide.tiles * p.wide.part.splits * a.kv_heads : 0;
   const int64_t join = p.few.part.slots + p.wide.part.slots;
-  if (few > kMaxGrid || wide > kMaxGrid || join > kMaxGrid) return hipErrorInvalidValue;
-  if (wide) {
-    hipLaunchKernelGGL(seq_attn_wide_kernel, dim3(static_cast<unsigned>(wide)), dim3(256), 0, s, a, p.wide);
-    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  }
-  if (a.ids)
-    hipLaunchKernelGGL(seq_attn_few_kernel<true>, dim3(static_cast<unsigned>(few)), dim3(64 * FEW_WAVES), 0, s, a, p.few);
+  if (few + wide > kMaxGrid || join > kMaxGrid) return hipErrorInvalidValue;
+  static_assert(64 * FEW_WAVES == 256 && 64 * WIDE_WAVES == 256, "one launch shape");
+  if (wide)
+    hipLaunchKernelGGL(seq_attn_mixed_kernel, dim3(static_cast<unsigned>(wide + few)), dim3(256), 0, s, a, p.few, p.wide,
+                       static_cast<int>(wide));
+  else if (a.ids)
+    hipLaunchKernelGGL(seq_attn_few_kernel<true>, dim3(static_cast<unsigned>(few)), dim3(256), 0, s, a, p.few);
   else
-    hipLaunchKernelGGL(seq_attn_few_kernel<false>, dim3(static_cast<unsigned>(few)), dim3(64 * FEW_WAVES), 0, s, a, p.few);
+    hipLaunchKernelGGL(seq_attn_few_kernel<false>, dim3(static_cast<unsigned>(few)), dim3(256), 0, s, a, p.few);
   if (const hipError_t e = hipGetLastError(); e != hipSuccess || join == 0) return e;
   hipLaunchKernelGGL(seq_attn_join_kernel, dim3(static_cast<unsigned>(join)), dim3(256), 0, s, a, p.few, p.wide);
   return hipGetLastError();
