@@ -221,8 +221,10 @@ __device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, F
   const int rest = block >> 3;
   const int kvh = rest % a.kv_heads;
   const int us = (rest / a.kv_heads) * 8 + (block & 7);
-  const int unit = us / p.part.splits, split = us % p.part.splits;
-  if (unit >= p.units) return;
+  // Split by split: the dispatcher goes round the CUs' groups strictly, so a pattern
+  // of splits with work and without would leave some of them idle.
+  const int unit = us % static_cast<int>(p.units), split = us / static_cast<int>(p.units);
+  if (split >= p.part.splits) return;
   const int tile = unit % p.tiles;
 
   int seq, row0 = 0;
@@ -474,6 +476,7 @@ typedef float v16f __attribute__((ext_vector_type(16)));
 typedef int v16i __attribute__((ext_vector_type(16)));
 
 constexpr int WIDE_COLS = 128;
+constexpr int WIDE_SLOTS = 512;    // workgroups at a time, two a CU
 constexpr int WIDE_KEYS = KB;      // of a step
 constexpr int WIDE_WAVES = 4;
 constexpr int WIDE_DEPTH = 4;      // steps whose K and V lie in LDS or on their way
@@ -482,7 +485,7 @@ constexpr int WIDE_OROW = 32 + 4;  // floats of a column's row where the results
 constexpr float WIDE_ROOM = 8.0f;  // P may reach 2^8 of its reference before O is scaled down
 
 struct WidePlan {
-  Partials part;  // slots: (row, head)
+  Partials part;  // slots: (tile, KV head, column)
   int64_t tiles;  // at most
   int least;      // columns of a sequence that are taken here
 };
@@ -490,6 +493,56 @@ struct WidePlan {
 // Key r's 16-byte chunk c of V lies at chunk c ^ vswz_wide(r): the 8 keys of a
 // transposing read (two runs of four, 8 apart) meet 8 chunks.
 __device__ __forceinline__ int vswz_wide(int key) { return (key & 3) | ((key >> 1) & 4); }
+
+// The sequence of the unit-th tile of 128 columns, -1 behind the last, and which of
+// its tiles it is: tiles are counted 64 sequences at a time, one per lane.  *span:
+// the keys of a split, the plan's or more: with splits as long as the work for each
+// of WIDE_SLOTS workgroups (the plan knows no sequence's length, only limits).
+__device__ __forceinline__ int wide_tile(const SeqAttnArgs &a, const WidePlan &p, int unit, int *nth, int *span, SeqSpan *seq) {
+  const int lane = threadIdx.x & 63;
+  const int group_heads = a.heads / a.kv_heads;
+  int found = -1;
+  float steps = 0.0f;
+  for (int b = 0; b < a.seqs.n_seq; b += 64) {
+    int tiles = 0;
+    SeqSpan sp{0, 0, 0};
+    if (b + lane < a.seqs.n_seq) {
+      sp = seq_span(a.seqs, b + lane);
+      const int cols = sp.n * group_heads;
+      tiles = cols < p.least ? 0 : (cols + WIDE_COLS - 1) / WIDE_COLS;
+      const int keys = a.causal ? max(sp.kv - sp.n / 2, 0) : sp.kv;
+      steps += static_cast<float>(tiles) * static_cast<float>(keys / WIDE_KEYS + 1);
+    }
+    if (found >= 0) continue;
+    int upto = tiles;  // inclusive sum over the lanes
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int t = __shfl_up(upto, d);
+      upto += lane >= d ? t : 0;
+    }
+    const uint64_t holds = __ballot(upto > unit);
+    if (holds) {
+      const int at = __builtin_ctzll(holds);
+      // a sequence's last rows see the most keys: its tiles start with them
+      *nth = __builtin_amdgcn_readlane(upto, at) - 1 - unit;
+      *seq = {__builtin_amdgcn_readlane(sp.r0, at), __builtin_amdgcn_readlane(sp.n, at), __builtin_amdgcn_readlane(sp.kv, at)};
+      found = b + at;
+    }
+    unit -= __builtin_amdgcn_readlane(upto, 63);
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) steps += __shfl_xor(steps, d);
+  const float each = steps * static_cast<float>(a.kv_heads) / WIDE_SLOTS;
+  const int even = static_cast<int>(fminf(each, static_cast<float>(WIDE_SPAN / WIDE_KEYS))) * WIDE_KEYS;
+  *span = __builtin_amdgcn_readfirstlane(max(p.part.span, even));
+  return found;
+}
+
+// The most keys that a column of a tile sees.
+__device__ __forceinline__ int tile_keys(const SeqAttnArgs &a, const SeqSpan &sp, int col0, int cols) {
+  const int group_heads = a.heads / a.kv_heads;
+  return a.causal ? max(sp.pos(sp.r0 + (min(cols, col0 + WIDE_COLS) - 1) / group_heads) + 1, 0) : sp.kv;
+}
 
 struct WideLds {
   struct Stages {
@@ -510,51 +563,28 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
   const int half = lane >> 5, n32 = lane & 31;
   const int group_heads = a.heads / a.kv_heads;
 
-  // which sequence's tile this is: tiles of the sequences before, 64 at a time
   const int kvh = block % a.kv_heads;
-  const int64_t us = block / a.kv_heads;
-  const int split = us % p.part.splits;
-  int64_t nth = us / p.part.splits;
-  int seq = -1;
-  for (int b = 0; b < a.seqs.n_seq && seq < 0; b += 64) {
-    int tiles = 0;
-    if (b + lane < a.seqs.n_seq) {
-      const int64_t cols = static_cast<int64_t>(seq_span(a.seqs, b + lane).n) * group_heads;
-      tiles = cols < p.least ? 0 : static_cast<int>((cols + WIDE_COLS - 1) / WIDE_COLS);
-    }
-    int upto = tiles;  // inclusive sum over the lanes
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int t = __shfl_up(upto, d);
-      upto += lane >= d ? t : 0;
-    }
-    const uint64_t holds = __ballot(upto > nth);
-    if (holds) {
-      const int at = __builtin_ctzll(holds);
-      seq = b + at;
-      // a sequence's last rows see the most keys: its tiles start with them
-      nth = __builtin_amdgcn_readlane(upto, at) - 1 - nth;
-    } else {
-      nth -= __builtin_amdgcn_readlane(upto, 63);
-    }
-  }
+  const int us = block / a.kv_heads;
+  // (split by split: a CU is fed in turn, whether the one before had work or not)
+  const int unit = us % static_cast<int>(p.tiles), split = us / static_cast<int>(p.tiles);
+  int nth, span;
+  SeqSpan sp;
+  const int seq = wide_tile(a, p, unit, &nth, &span, &sp);
   if (seq < 0) return;
-  const SeqSpan sp = seq_span(a.seqs, seq);
   const int cols = sp.n * group_heads;
   const int pt = a.pool.page_tokens;
-  const int col0 = static_cast<int>(nth) * WIDE_COLS;
+  const int col0 = nth * WIDE_COLS;
   const int c = col0 + wave * 32 + n32;
   const bool live = c < cols;
   const int row = sp.r0 + c / group_heads, head = kvh * group_heads + c % group_heads;
   const int sees = !live ? 0 : a.causal ? max(sp.pos(row) + 1, 0) : sp.kv;
   // the fewest and the most keys that a column sees: the first row's, the last's
   const int first_row = sp.r0 + col0 / group_heads;
-  const int last_row = sp.r0 + (min(cols, col0 + WIDE_COLS) - 1) / group_heads;
   const int tile_min = a.causal ? max(sp.pos(first_row) + 1, 0) : sp.kv;
-  const int tile_max = a.causal ? max(sp.pos(last_row) + 1, 0) : sp.kv;
-  const int first = split * p.part.span;
-  const int end = min(tile_max, first + p.part.span);
-  if (split > 0 && first >= tile_max) return;
+  const int tile_max = tile_keys(a, sp, col0, cols);
+  if (split > 0 && split * static_cast<int64_t>(span) >= tile_max) return;
+  const int first = split * span;
+  const int end = min(tile_max, first + span);
   const int steps = (end - first + WIDE_KEYS - 1) / WIDE_KEYS;  // <= 0: none
 
   v4i_d qf[4];
@@ -568,42 +598,16 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
     cs = a.qs[row * a.ldqs + head * a.qs_col] * a.qk_scale * kLog2e;
   }
 
-  // the split's blocks, and the range of its V scales' magnitudes (as integers;
-  // zeros aside), 32 lanes a block
+  // the split's blocks
   if (tid < 2) lds.range[tid] = tid == 0 ? 0u : 0x7f800000u;
-  __syncthreads();
   bool hole = false;
-  {
-    uint32_t most = 0, least = 0x7f800000u;
-#pragma unroll 4
-    for (int i = tid >> 5; i < steps; i += 2 * WIDE_WAVES) {
-      const int key = first + i * KB;
-      const int2 at = key < end ? make_int2(seq_page(a.seqs, a.pool, seq, key / pt), key % pt) : make_int2(-1, 0);
-      hole |= key < end && at.x < 0;
-      if (n32 == 0) lds.block[i] = at;
-      if (at.x >= 0 && key + n32 < end) {
-        const uint32_t v = __float_as_uint(a.pool.vs[at.x * a.pool.spage + (at.y + n32) * a.pool.srow + kvh]) & 0x7fffffffu;
-        most = max(most, v);
-        if (v) least = min(least, v);
-      }
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      most = max(most, lane_xor_m(most, d));
-      least = min(least, lane_xor_m(least, d));
-    }
-    if (lane == 0) {
-      atomicMax(&lds.range[0], most);
-      atomicMin(&lds.range[1], least);
-    }
+  for (int i = tid; i < steps; i += 256) {
+    const int key = first + i * KB;
+    const int2 at = make_int2(seq_page(a.seqs, a.pool, seq, key / pt), key % pt);
+    hole |= at.x < 0;
+    lds.block[i] = at;
   }
   const bool missing = __syncthreads_or(hole);
-  const uint32_t most = __builtin_amdgcn_readfirstlane(lds.range[0]), least = __builtin_amdgcn_readfirstlane(lds.range[1]);
-  // Narrow: exponents 4 apart at most, and no closer to the ends than 2^64.
-  const int expo = static_cast<int>(most >> 23) - 127;
-  const bool narrow = most == 0 || (expo >= -64 && expo <= 64 && least >= most - (4u << 23));
-  // with p = 2^(x - base), base = the largest x less `lift`: p vs <= 2^7 there
-  const float lift = narrow && most ? static_cast<float>(6 - expo) : 0.0f;
 
   // Copies: wave w takes keys 8 w .. 8 w + 7 of a step (of block w / 4).
   const int r8 = lane >> 3, ch = lane & 7;
@@ -619,6 +623,41 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
     if (wave == 0)
       lds_copy4((half ? a.pool.vs : a.pool.ks) + at.x * a.pool.spage + (at.y + n32) * a.pool.srow + kvh, lds.sc[step % (2 * WIDE_DEPTH)]);
   };
+
+  // the first steps' copies, and beside them the range of the V scales' magnitudes
+  // (as integers; zeros aside), 32 lanes a block
+#pragma unroll
+  for (int i = 0; i < WIDE_DEPTH; ++i)
+    if (i < steps) copy(i);
+  {
+    uint32_t most = 0, least = 0x7f800000u;
+#pragma unroll 4
+    for (int i = tid >> 5; i < steps; i += 2 * WIDE_WAVES) {
+      const int2 at = lds.block[i];
+      if (at.x >= 0 && first + i * KB + n32 < end) {
+        const uint32_t v = __float_as_uint(a.pool.vs[at.x * a.pool.spage + (at.y + n32) * a.pool.srow + kvh]) & 0x7fffffffu;
+        most = max(most, v);
+        if (v) least = min(least, v);
+      }
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      most = max(most, lane_xor_m(most, d));
+      least = min(least, lane_xor_m(least, d));
+    }
+    if (lane == 0) {
+      atomicMax(&lds.range[0], most);
+      atomicMin(&lds.range[1], least);
+    }
+  }
+  wait_copies<0>();
+  lds_barrier();
+  const uint32_t most = __builtin_amdgcn_readfirstlane(lds.range[0]), least = __builtin_amdgcn_readfirstlane(lds.range[1]);
+  // Narrow: exponents 4 apart at most, and no closer to the ends than 2^64.
+  const int expo = static_cast<int>(most >> 23) - 127;
+  const bool narrow = most == 0 || (expo >= -64 && expo <= 64 && least >= most - (4u << 23));
+  // with p = 2^(x - base), base = the largest x less `lift`: p vs <= 2^7 there
+  const float lift = narrow && most ? static_cast<float>(6 - expo) : 0.0f;
 
   // The softmax's reference (base 2), at most WIDE_ROOM short of the largest score
   // less lift, so that O is scaled down a few times in all, not at every new maximum.
@@ -767,11 +806,6 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
     }
   };
   auto all = [&](auto narrow_tag) {
-#pragma unroll
-    for (int i = 0; i < WIDE_DEPTH; ++i)
-      if (i < steps) copy(i);
-    wait_copies<0>();
-    lds_barrier();
     turn(0, narrow_tag);
     v16i s;
     products(0, s);
@@ -794,8 +828,8 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
     const LanePair pr = lane_pair32(__float_as_uint(l));
     l = __uint_as_float(pr.a) + __uint_as_float(pr.b);
   }
-  const bool whole = p.part.splits == 1;
-  const int64_t at = whole || !live ? 0 : (static_cast<int64_t>(row) * a.heads + head) * p.part.splits + split;
+  const bool whole = tile_max <= span;
+  const int64_t at = whole || !live ? 0 : ((static_cast<int64_t>(unit) * a.kv_heads + kvh) * WIDE_COLS + c - col0) * p.part.splits + split;
   if (whole) {
     const float inv = base == -INFINITY ? 0.0f : 1.0f / l;
 #pragma unroll
@@ -871,47 +905,61 @@ __global__ void __launch_bounds__(256, 2) seq_attn_mixed_kernel(SeqAttnArgs a, F
     few_columns<false>(a, fp, blockIdx.x - wide, lds.few);
 }
 
-// Joins the splits of a (row, head): 16 lanes of 8 channels, 16 such groups over
-// the splits in turn.  The first workgroups take the slots of the 16-column kernel,
-// the rest those of the 128-column one.
-__global__ void __launch_bounds__(256) seq_attn_join_kernel(SeqAttnArgs a, FewPlan fp, WidePlan wp) {
+// Joins the splits of slots: 16 lanes of 8 channels a slot, of many splits 16 such
+// groups over the splits in turn (GROUPS; 16 slots a workgroup otherwise).  A cell is
+// what slots are counted in: (sequence, KV head) or row of the 16-column kernel,
+// (tile, KV head) of the 128-column one.
+template <int GROUPS, bool WIDE>
+__global__ void __launch_bounds__(256) seq_attn_join_kernel(SeqAttnArgs a, std::conditional_t<WIDE, WidePlan, FewPlan> plan, int cell_cols) {
+  const Partials &p = plan.part;
   __shared__ float o_s[4][HD];
   __shared__ float sum_s[4];
-  const bool few = blockIdx.x < fp.part.slots;
-  const Partials &p = few ? fp.part : wp.part;
-  const int64_t slot = blockIdx.x - (few ? 0 : fp.part.slots);
+  constexpr int PER = 16 / GROUPS;
+  const int group = threadIdx.x >> 4, d0 = 8 * (threadIdx.x & 15);
+  const int blocks = (cell_cols + PER - 1) / PER;
+  const int cell = blockIdx.x / blocks;
+  const int c = blockIdx.x % blocks * PER + (GROUPS == 1 ? group : 0);  // column of the cell
   const int group_heads = a.heads / a.kv_heads;
-  int seq, row, head;
+  int seq, row, head, span = p.span;
   SeqSpan sp;
-  if (few && !a.ids) {
-    const int c = static_cast<int>(slot % fp.most);
-    const int sh = static_cast<int>(slot / fp.most);
-    seq = sh / a.kv_heads;
-    sp = seq_span(a.seqs, seq);
-    const int cols = sp.n * group_heads;
-    if (c >= cols || cols > fp.most) return;
-    row = sp.r0 + c / group_heads;
-    head = sh % a.kv_heads * group_heads + c % group_heads;
-  } else {
-    row = static_cast<int>(slot / a.heads);
-    head = static_cast<int>(slot % a.heads);
+  if (!WIDE && a.ids) {
+    row = cell, head = c;
     seq = seq_of_row(a.seqs, row);
     if (seq >= a.seqs.n_seq) return;
     sp = seq_span(a.seqs, seq);
-    if (row < sp.r0 || row >= sp.r0 + sp.n) return;
-    if (!few && sp.n * group_heads < wp.least) return;
+    if (row < sp.r0 || row >= sp.r0 + sp.n || c >= a.heads) return;
+  } else {
+    int col = c, cols;
+    if constexpr (WIDE) {
+      int nth;
+      seq = wide_tile(a, plan, cell / a.kv_heads, &nth, &span, &sp);
+      if (seq < 0) return;
+      cols = sp.n * group_heads;
+      if (tile_keys(a, sp, nth * WIDE_COLS, cols) <= span) return;  // written as it is
+      col += nth * WIDE_COLS;
+    } else {
+      seq = cell / a.kv_heads;
+      sp = seq_span(a.seqs, seq);
+      cols = sp.n * group_heads;
+      if (cols > plan.most) return;
+    }
+    if (c >= cell_cols || col >= cols) return;
+    row = sp.r0 + col / group_heads;
+    head = cell % a.kv_heads * group_heads + col % group_heads;
   }
   const int sees = a.causal ? max(sp.pos(row) + 1, 0) : sp.kv;
-  const int n = a.ids ? p.splits : (sees + p.span - 1) / p.span;
-  const int64_t at = slot * p.splits;
+  const int n = !WIDE && a.ids ? p.splits : (sees + span - 1) / span;
+  const int64_t at = (static_cast<int64_t>(cell) * cell_cols + c) * p.splits;
   float top = -INFINITY;
-  for (int s = threadIdx.x & 63; s < n; s += 64) top = fmaxf(top, p.ml[at + s].x);
-  top = max64(top);
+  for (int s = threadIdx.x & 15; s < n; s += 16) top = fmaxf(top, p.ml[at + s].x);
+  top = fmaxf(top, lane_xor<1>(top));
+  top = fmaxf(top, lane_xor<2>(top));
+  top = fmaxf(top, lane_xor<4>(top));
+  top = fmaxf(top, lane_xor<8>(top));
   const float base = top == -INFINITY ? 0.0f : top;
-  const int d0 = 8 * (threadIdx.x & 15);
   float r[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sum = 0.0f;
 #pragma unroll 4
-  for (int s = threadIdx.x >> 4; s < n; s += 16) {
+  for (int s = GROUPS == 1 ? 0 : group; s < n; s += GROUPS) {
     const float2 ml = p.ml[at + s];
     const float f = exp2_from(ml.x, base);
     sum += f * ml.y;
@@ -920,24 +968,40 @@ __global__ void __launch_bounds__(256) seq_attn_join_kernel(SeqAttnArgs a, FewPl
 #pragma unroll
     for (int i = 0; i < 4; ++i) r[i] += f * u[i], r[4 + i] += f * v[i];
   }
+  if constexpr (GROUPS > 1) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = col_sum(r[i]);
-  sum = col_sum(sum);
-  const int wave = threadIdx.x >> 6;
-  if ((threadIdx.x & 63) < 16) {
+    for (int i = 0; i < 8; ++i) r[i] = col_sum(r[i]);
+    sum = col_sum(sum);
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) < 16) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o_s[wave][d0 + i] = r[i];
-    if (d0 == 0) sum_s[wave] = sum;
+      for (int i = 0; i < 8; ++i) o_s[wave][d0 + i] = r[i];
+      if (d0 == 0) sum_s[wave] = sum;
+    }
+    __syncthreads();
+    if (threadIdx.x >= 16) return;
+    sum = (sum_s[0] + sum_s[1]) + (sum_s[2] + sum_s[3]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = (o_s[0][d0 + i] + o_s[1][d0 + i]) + (o_s[2][d0 + i] + o_s[3][d0 + i]);
   }
-  __syncthreads();
-  if (threadIdx.x >= 16) return;
-  sum = (sum_s[0] + sum_s[1]) + (sum_s[2] + sum_s[3]);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    r[i] = (o_s[0][d0 + i] + o_s[1][d0 + i]) + (o_s[2][d0 + i] + o_s[3][d0 + i]);
-    r[i] = top == -INFINITY ? 0.0f : r[i] / sum;
-  }
+  for (int i = 0; i < 8; ++i) r[i] = top == -INFINITY ? 0.0f : r[i] / sum;
   store_row8(a, row, head, d0, r);
+}
+
+template <bool WIDE, class P>
+hipError_t launch_join(const SeqAttnArgs &a, const P &plan, int cell_cols, hipStream_t s) {
+  const Partials &p = plan.part;
+  if (p.slots == 0) return hipSuccess;
+  const int64_t cells = p.slots / cell_cols;
+  const bool many = p.splits > 12;
+  const int64_t wgs = cells * (many ? cell_cols : (cell_cols + 15) / 16);
+  if (wgs > INT32_MAX / 256) return hipErrorInvalidValue;
+  if (many)
+    hipLaunchKernelGGL((seq_attn_join_kernel<16, WIDE>), dim3(static_cast<unsigned>(wgs)), dim3(256), 0, s, a, plan, cell_cols);
+  else
+    hipLaunchKernelGGL((seq_attn_join_kernel<1, WIDE>), dim3(static_cast<unsigned>(wgs)), dim3(256), 0, s, a, plan, cell_cols);
+  return hipGetLastError();
 }
 
 // ---- plans --------------------------------------------------------------------
@@ -961,8 +1025,14 @@ void plan_splits(int64_t units, int64_t keys, int64_t want, int step, int least,
   p.splits = static_cast<int>(cdiv(keys, span));
 }
 
-// Sequences of up to FEW_MOST columns go to the kernel of 16-column tiles.
+// Sequences of up to FEW_MOST columns go to the kernel of 16-column tiles, and all
+// of a call do while rows x heads x max_kv stays small: its tiles fill the CUs
+// sooner.  us, 16-column / 128-column tiles, 16 heads on 8: 32 rows behind 500 keys
+// 11 / 29, 512 rows 20 / 26, 64 rows behind 4000 keys (4.2e6) 24 / 31, 1024 rows (17e6)
+// 44 / 37, 256 rows behind 4000 keys 60 / 47, 8 x 64 rows behind 1000 keys (8.7e6)
+// 40 / 35.
 constexpr int FEW_MOST = 16;
+constexpr int64_t FEW_PAIRS = 6 << 20;
 constexpr int FEW_WANT = 2048, WIDE_WANT = 1536;  // workgroups
 
 struct Plan {
@@ -975,7 +1045,8 @@ Plan plan_attn(const SeqAttnArgs &a) {
   Plan p{};
   const int64_t g = a.heads / a.kv_heads, rows = a.seqs.rows, n_seq = a.seqs.n_seq;
   const int64_t cols = a.ids ? g : a.seqs.max_rows * g;  // of a sequence (listed pages: of a row), at most
-  p.any_wide = !a.ids && cols > FEW_MOST;
+  const bool small = rows * a.heads * a.seqs.max_kv <= FEW_PAIRS && n_seq * cdiv(cols, FEW_COLS) * a.kv_heads <= 4 * FEW_WANT;
+  p.any_wide = !a.ids && cols > FEW_MOST && !small;
   const int64_t few_cols = p.any_wide ? FEW_MOST : cols < 1 ? 1 : cols;
   p.few.most = static_cast<int>(few_cols);
   p.few.tiles = static_cast<int>(cdiv(few_cols, FEW_COLS));
@@ -988,7 +1059,7 @@ Plan plan_attn(const SeqAttnArgs &a) {
     const int64_t wide_seqs = rows * g / p.wide.least;
     p.wide.tiles = rows * g / WIDE_COLS + (n_seq < wide_seqs ? n_seq : wide_seqs);
     plan_splits(p.wide.tiles * a.kv_heads, a.seqs.max_kv, WIDE_WANT, WIDE_KEYS, 512, WIDE_SPAN, p.wide.part);
-    if (p.wide.part.splits > 1) p.wide.part.slots = rows * a.heads;
+    if (p.wide.part.splits > 1) p.wide.part.slots = p.wide.tiles * a.kv_heads * WIDE_COLS;
   }
   return p;
 }
@@ -1014,8 +1085,7 @@ hipError_t launch_seq_attn(const SeqAttnArgs &args, hipStream_t s) {
   p.wide.part.ml = p.few.part.ml + nf;
   const int64_t few = cdiv(p.few.units * p.few.part.splits, 8) * 8 * a.kv_heads;
   const int64_t wide = p.any_wide ? p.wide.tiles * p.wide.part.splits * a.kv_heads : 0;
-  const int64_t join = p.few.part.slots + p.wide.part.slots;
-  if (few + wide > kMaxGrid || join > kMaxGrid) return hipErrorInvalidValue;
+  if (few + wide > kMaxGrid) return hipErrorInvalidValue;
   static_assert(64 * FEW_WAVES == 256 && 64 * WIDE_WAVES == 256, "one launch shape");
   if (wide)
     hipLaunchKernelGGL(seq_attn_mixed_kernel, dim3(static_cast<unsigned>(wide + few)), dim3(256), 0, s, a, p.few, p.wide,
@@ -1024,9 +1094,9 @@ hipError_t launch_seq_attn(const SeqAttnArgs &args, hipStream_t s) {
     hipLaunchKernelGGL(seq_attn_few_kernel<true>, dim3(static_cast<unsigned>(few)), dim3(256), 0, s, a, p.few);
   else
     hipLaunchKernelGGL(seq_attn_few_kernel<false>, dim3(static_cast<unsigned>(few)), dim3(256), 0, s, a, p.few);
-  if (const hipError_t e = hipGetLastError(); e != hipSuccess || join == 0) return e;
-  hipLaunchKernelGGL(seq_attn_join_kernel, dim3(static_cast<unsigned>(join)), dim3(256), 0, s, a, p.few, p.wide);
-  return hipGetLastError();
+  if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  if (const hipError_t e = launch_join<true>(a, p.wide, WIDE_COLS, s); e != hipSuccess) return e;
+  return launch_join<false>(a, p.few, a.ids ? a.heads : p.few.most, s);
 }
 
 }  // namespace q3
