@@ -398,6 +398,25 @@ def test_select_ties(cuda, n_sel):
     assert np.array_equal(ids.cpu().numpy(), want)
 
 
+@pytest.mark.parametrize("pages", [4095, 4096, 4097, 6000])
+def test_select_many_pages(cuda, pages):
+    """Both sides of what the keys' registers hold; a table that names its few pages
+    over and over, so most scores tie."""
+    b = Batch([(1, 32 * 40), (2, 32 * 20)], 2, 32, seed=pages)
+    b.tables = b.rng.integers(0, b.n_pages, (2, pages)).astype(np.uint16)
+    b.kv_len = np.array([32 * pages - 5, 32 * (pages - 1) + 1], np.int32)
+    b.lens = [(1, int(b.kv_len[0]) - 1), (2, int(b.kv_len[1]) - 2)]
+    b.max_kv = int(b.kv_len.max())
+    bounds = b.rng.integers(-127, 128, (b.n_pages * 2, 256)).astype(np.int8)
+    scale = b.rng.uniform(0.1, 1, (b.n_pages, 2)).astype(F)
+    q8, qs = queries(b.rng, b.rows, 6)
+    pool, seqs = on_device(b)
+    for n_sel in (5, 700):
+        ids = torch.empty((b.rows, 2 * n_sel), dtype=torch.int32, device="cuda")
+        ops.select_pages(dev(q8), dev(qs), pool, seqs, dev(bounds), dev(scale), ids, n_sel)
+        assert np.array_equal(ids.cpu().numpy(), seqref.select(b, q8, qs, 6, bounds, scale, n_sel))
+
+
 def test_select_extremes(cuda):
     """Scores of the int8 limits (-128 included), NaN scales first of all, -inf last."""
     b = Batch([(1, 32 * 40)], 1, 32, seed=1)
