@@ -12,108 +12,203 @@ namespace q3 {
 namespace {
 
 constexpr int HD = 128;
+constexpr int64_t APPEND_WGS = 1024;
 
-// A workgroup takes 8 heads (of Q, K and V in this order) of one row, 32 lanes a
+// Four values as int8 with their head's scale: quant_rcp's results, with its f64
+// arithmetic (half of this kernel's time) only where a quotient lies near a half.
+// x * rcp(scale) is within 127 * 3 * 2^-24 < 3e-5 of x / scale where the scale is a
+// normal number whose reciprocal is one too, so elsewhere both round alike.
+__device__ __forceinline__ char4 quant4(const float (&x)[4], float scale) {
+  const float inv = __builtin_amdgcn_rcpf(scale);
+  float r[4];
+  bool sure = scale > 0x1p-100f && scale < 0x1p+100f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float t = __fmul_rn(x[i], inv);
+    r[i] = rintf(t);
+    sure &= fabsf(__fsub_rn(t, r[i])) < 0.4999f;
+    r[i] = fminf(127.0f, fmaxf(-127.0f, r[i]));
+  }
+  char4 q;
+  q.x = static_cast<signed char>(r[0]);
+  q.y = static_cast<signed char>(r[1]);
+  q.z = static_cast<signed char>(r[2]);
+  q.w = static_cast<signed char>(r[3]);
+  if (__ballot(!sure)) {
+    const double y = rcp64(scale);
+    q.x = static_cast<signed char>(quant_rcp(x[0], y));
+    q.y = static_cast<signed char>(quant_rcp(x[1], y));
+    q.z = static_cast<signed char>(quant_rcp(x[2], y));
+    q.w = static_cast<signed char>(quant_rcp(x[3], y));
+  }
+  return q;
+}
+
+// ((b0 + b1) + b2) + b3 of the four 8-lane groups' sums in each 32-lane half.
+__device__ __forceinline__ float ordered_sum4(float s, int lane) {
+  const float b = lane_xor<8>(s), c = lane_xor<16>(s);
+  const float d = lane_xor<8>(c);
+  const bool odd = lane & 8, second = lane & 16;
+  const float lo = __fadd_rn(second ? c : s, second ? d : b);
+  const float b2 = second ? (odd ? b : s) : (odd ? d : c), b3 = second ? (odd ? s : b) : (odd ? c : d);
+  return __fadd_rn(__fadd_rn(lo, b2), b3);
+}
+
+// A workgroup takes 8 heads (of Q, K and V in this order) of ROWS rows, 32 lanes a
 // head, 4 columns a lane: a head's reads and writes are then whole 16- and 4-byte
 // words, its 32-column norm blocks 8 lanes each, and a decoding row of 16 + 2 x 8
-// heads is 4 workgroups.  Bound by the reads (1 KiB a wave) at many rows, by the
-// chain start -> length -> page and angles -> store at one.
-// VEC: x rows, gains' and angles' accesses may be 16-byte words.
-template <bool VEC>
-__global__ void __launch_bounds__(256) seq_append_kernel(SeqAppendArgs a, int groups) {
+// heads is 4 workgroups.  At one row bound by the chain start -> length -> page and
+// angles -> store (4.1 us), at many by how many rows' reads are under way: with one row
+// a workgroup 2048 rows took 35 us, with four, whose loads go out together, APPEND_US.
+// VEC: x rows may be read as 16-byte words; angles: so may a lane's angles (and its
+// four columns are rotated alike).
+template <bool VEC, int ROWS>
+__global__ void __launch_bounds__(256) seq_append_kernel(SeqAppendArgs a, int groups, bool angles) {
   __shared__ __align__(16) float ex[8][HD];
   const int lane = threadIdx.x & 63, wave = wave_id();
-  const int row = blockIdx.x / groups, group = blockIdx.x % groups;
+  const int row0 = blockIdx.x / groups * ROWS, group = blockIdx.x % groups;
   const int slot = wave * 2 + (lane >> 5), item = group * 8 + slot;
   const int c0 = 4 * (lane & 31);
   const bool is_q = item < a.heads, is_v = item >= a.heads + a.kv_heads;
   const bool live = item < a.heads + 2 * a.kv_heads;
   const int head = is_q ? item : is_v ? item - a.heads - a.kv_heads : item - a.heads;
 
-  float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (live) {
-    const float *src = (is_q   ? a.q + static_cast<int64_t>(row) * a.ldq
-                        : is_v ? a.v + static_cast<int64_t>(row) * a.ldv
-                               : a.k + static_cast<int64_t>(row) * a.ldk) +
-                       static_cast<int64_t>(head) * HD + c0;
-    if constexpr (VEC) {
-      const float4 t = *reinterpret_cast<const float4 *>(src);
-      x[0] = t.x, x[1] = t.y, x[2] = t.z, x[3] = t.w;
-    } else {
+  float x[ROWS][4];
+  const float *src = (is_q ? a.q : is_v ? a.v : a.k) + static_cast<int64_t>(head) * HD + c0;
+  const int64_t ldx = is_q ? a.ldq : is_v ? a.ldv : a.ldk;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = src[i];
-    }
-  }
-
-  const int seq = seq_of_row(a.seqs, row);
-  if (seq >= a.seqs.n_seq) return;  // behind the last sequence
-  const SeqSpan sp = seq_span(a.seqs, seq);
-  const int pos = sp.pos(row);
-  if (row < sp.r0 || row >= sp.r0 + sp.n || pos < 0) return;  // uniform in the workgroup
-
-  const float *nw = is_v ? nullptr : is_q ? a.nwq : a.nwk;
-  if (a.nwq || a.nwk) {
-    float s = __fadd_rn(__fadd_rn(__fmul_rn(x[0], x[0]), __fmul_rn(x[1], x[1])),
-                        __fadd_rn(__fmul_rn(x[2], x[2]), __fmul_rn(x[3], x[3])));
-    s = __fadd_rn(s, lane_xor<1>(s));
-    s = __fadd_rn(s, lane_xor<2>(s));
-    s = __fadd_rn(s, lane_xor<4>(s));
-    float ss = 0.0f;
+  for (int r = 0; r < ROWS; ++r) {
+    const int row = min(row0 + r, a.seqs.rows - 1);
 #pragma unroll
-    for (int b = 0; b < 4; ++b) ss = __fadd_rn(ss, __shfl(s, (lane & 32) + 8 * b));
-    if (nw && live) {
-      const float rinv = rms_factor(ss, a.inv_hd);
-      const int64_t ws = is_q ? a.nwq_stride : a.nwk_stride;
+    for (int i = 0; i < 4; ++i) x[r][i] = 0.0f;
+    if (live) {
+      if constexpr (VEC) {
+        const float4 t = *reinterpret_cast<const float4 *>(src + row * ldx);
+        x[r][0] = t.x, x[r][1] = t.y, x[r][2] = t.z, x[r][3] = t.w;
+      } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = __fmul_rn(__fmul_rn(x[i], rinv), nw[(c0 + i) * ws]);
-    }
-  }
-
-  if (a.rot > 0) {
-    const int h = a.rot / 2;
-    const float *cs = a.cos_t + pos * a.ld_cs, *sn = a.sin_t + pos * a.ld_cs;
-    *reinterpret_cast<float4 *>(&ex[slot][c0]) = make_float4(x[0], x[1], x[2], x[3]);
-    // the 32 lanes of a head are in one wave: its own LDS writes are done
-    // before its reads
-    __builtin_amdgcn_wave_barrier();
-    if (!is_v) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int c = c0 + i;
-        if (c < a.rot) {
-          const bool first = a.interleaved ? !(c & 1) : c < h;
-          const int at = a.interleaved ? c >> 1 : first ? c : c - h;
-          const float o = ex[slot][a.interleaved ? c ^ 1 : first ? c + h : c - h];
-          x[i] = first ? __fsub_rn(__fmul_rn(x[i], cs[at]), __fmul_rn(o, sn[at]))
-                       : __fadd_rn(__fmul_rn(o, sn[at]), __fmul_rn(x[i], cs[at]));
-        }
+        for (int i = 0; i < 4; ++i) x[r][i] = src[row * ldx + i];
       }
     }
   }
 
-  const float m = max32(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
-  if (!live) return;
-  const float scale = __fmul_rn(m, inv127());
-  const double y = rcp64(scale);
-  char4 q;
-  q.x = static_cast<signed char>(quant_rcp(x[0], y));
-  q.y = static_cast<signed char>(quant_rcp(x[1], y));
-  q.z = static_cast<signed char>(quant_rcp(x[2], y));
-  q.w = static_cast<signed char>(quant_rcp(x[3], y));
-  int8_t *dst;
-  float *sdst;
-  if (is_q) {
-    dst = a.q8 + static_cast<int64_t>(row) * a.ldq8;
-    sdst = a.qs + static_cast<int64_t>(row) * a.ldqs + static_cast<int64_t>(head) * a.qs_col;
-  } else {
-    const int logical = pos / a.pool.page_tokens, t = pos % a.pool.page_tokens;
-    const int page = seq_page(a.seqs, a.pool, seq, logical);
-    if (page < 0) return;
-    dst = (is_v ? a.pool.v : a.pool.k) + page * a.pool.page_bytes + t * a.pool.row_bytes;
-    sdst = (is_v ? a.pool.vs : a.pool.ks) + page * a.pool.spage + t * a.pool.srow + head;
+  // each row's sequence and position; -1: behind the last sequence, or left out
+  int seq[ROWS], pos[ROWS];
+  seqs_of_rows<ROWS>(a.seqs, row0, seq);
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    pos[r] = -1;
+    if (row0 + r < a.seqs.rows && seq[r] < a.seqs.n_seq) {
+      const SeqSpan sp = seq_span(a.seqs, seq[r]);
+      if (row0 + r >= sp.r0 && row0 + r < sp.r0 + sp.n) pos[r] = sp.pos(row0 + r);
+    }
   }
-  *reinterpret_cast<char4 *>(dst + static_cast<int64_t>(head) * HD + c0) = q;
-  if ((lane & 31) == 0) *sdst = scale;
+
+  int page[ROWS], slot_of[ROWS];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    page[r] = -1, slot_of[r] = 0;
+    if (pos[r] < 0) continue;
+    slot_of[r] = pos[r] % a.pool.page_tokens;
+    page[r] = seq_page(a.seqs, a.pool, seq[r], pos[r] / a.pool.page_tokens);
+  }
+
+  float w[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+  const float *nw = is_v || !live ? nullptr : is_q ? a.nwq : a.nwk;
+  if (nw) {
+    const int64_t ws = is_q ? a.nwq_stride : a.nwk_stride;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = nw[(c0 + i) * ws];
+  }
+  const int h = a.rot / 2;
+  const bool first = c0 < h, turns = !is_v && live && c0 < a.rot;
+  float cs[ROWS][4], sn[ROWS][4];
+  if (angles) {  // (rot is a multiple of 8)
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      if (!turns || pos[r] < 0) continue;
+      const float *c = a.cos_t + pos[r] * a.ld_cs, *s = a.sin_t + pos[r] * a.ld_cs;
+      if (a.interleaved) {
+        const float2 u = *reinterpret_cast<const float2 *>(c + (c0 >> 1)), v = *reinterpret_cast<const float2 *>(s + (c0 >> 1));
+        cs[r][0] = cs[r][1] = u.x, cs[r][2] = cs[r][3] = u.y;
+        sn[r][0] = sn[r][1] = v.x, sn[r][2] = sn[r][3] = v.y;
+      } else {
+        const float4 u = *reinterpret_cast<const float4 *>(c + (first ? c0 : c0 - h));
+        const float4 v = *reinterpret_cast<const float4 *>(s + (first ? c0 : c0 - h));
+        cs[r][0] = u.x, cs[r][1] = u.y, cs[r][2] = u.z, cs[r][3] = u.w;
+        sn[r][0] = v.x, sn[r][1] = v.y, sn[r][2] = v.z, sn[r][3] = v.w;
+      }
+    }
+  }
+
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    if (pos[r] < 0) continue;  // uniform in the workgroup
+    const int row = row0 + r;
+    float (&y)[4] = x[r];
+    if (a.nwq || a.nwk) {
+      float s = __fadd_rn(__fadd_rn(__fmul_rn(y[0], y[0]), __fmul_rn(y[1], y[1])),
+                          __fadd_rn(__fmul_rn(y[2], y[2]), __fmul_rn(y[3], y[3])));
+      s = __fadd_rn(s, lane_xor<1>(s));
+      s = __fadd_rn(s, lane_xor<2>(s));
+      s = __fadd_rn(s, lane_xor<4>(s));
+      const float ss = ordered_sum4(s, lane);
+      if (nw) {
+        const float rinv = rms_factor(ss, a.inv_hd);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = __fmul_rn(__fmul_rn(y[i], rinv), w[i]);
+      }
+    }
+    if (a.rot > 0) {
+      // (a head's 32 lanes are in one wave, which finishes its LDS writes before its
+      // reads, and those before the next row's writes)
+      *reinterpret_cast<float4 *>(&ex[slot][c0]) = make_float4(y[0], y[1], y[2], y[3]);
+      __builtin_amdgcn_wave_barrier();
+      if (turns && angles) {
+        float o[4] = {y[1], y[0], y[3], y[2]};
+        if (!a.interleaved) {
+          const float4 t = *reinterpret_cast<const float4 *>(&ex[slot][first ? c0 + h : c0 - h]);
+          o[0] = t.x, o[1] = t.y, o[2] = t.z, o[3] = t.w;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool f = a.interleaved ? !(i & 1) : first;
+          const float u = __fmul_rn(y[i], cs[r][i]), v = __fmul_rn(o[i], sn[r][i]);
+          y[i] = f ? __fsub_rn(u, v) : __fadd_rn(v, u);
+        }
+      } else if (turns) {
+        const float *c = a.cos_t + pos[r] * a.ld_cs, *s = a.sin_t + pos[r] * a.ld_cs;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int col = c0 + i;
+          if (col < a.rot) {
+            const bool f = a.interleaved ? !(col & 1) : col < h;
+            const int at = a.interleaved ? col >> 1 : f ? col : col - h;
+            const float o = ex[slot][a.interleaved ? col ^ 1 : f ? col + h : col - h];
+            const float u = __fmul_rn(y[i], c[at]), v = __fmul_rn(o, s[at]);
+            y[i] = f ? __fsub_rn(u, v) : __fadd_rn(v, u);
+          }
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+    const float m = max32(fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3]))));
+    if (!live) continue;
+    const float scale = __fmul_rn(m, inv127());
+    const char4 q = quant4(y, scale);
+    int8_t *dst;
+    float *sdst;
+    if (is_q) {
+      dst = a.q8 + row * a.ldq8;
+      sdst = a.qs + row * a.ldqs + head * a.qs_col;
+    } else {
+      if (page[r] < 0) continue;
+      dst = (is_v ? a.pool.v : a.pool.k) + page[r] * a.pool.page_bytes + slot_of[r] * a.pool.row_bytes;
+      sdst = (is_v ? a.pool.vs : a.pool.ks) + page[r] * a.pool.spage + slot_of[r] * a.pool.srow + head;
+    }
+    *reinterpret_cast<char4 *>(dst + static_cast<int64_t>(head) * HD + c0) = q;
+    if ((lane & 31) == 0) *sdst = scale;
+  }
 }
 
 // Channel bounds of one page and KV head: over the page's cached keys the least
@@ -199,11 +294,18 @@ hipError_t launch_seq_append(const SeqAppendArgs &a, hipStream_t s) {
   const int groups = (a.heads + 2 * a.kv_heads + 7) / 8;
   const auto al16 = [](const void *p, int64_t ld_) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld_ & 3) == 0; };
   const bool vec = (!a.q || al16(a.q, a.ldq)) && al16(a.k, a.ldk) && al16(a.v, a.ldv);
-  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.seqs.rows) * groups));
-  if (vec)
-    hipLaunchKernelGGL(seq_append_kernel<true>, grid, dim3(256), 0, s, a, groups);
+  const bool angles = a.rot > 0 && a.rot % 8 == 0 && al16(a.cos_t, a.ld_cs) && al16(a.sin_t, a.ld_cs);
+  // four rows a workgroup once one a workgroup would leave some waiting for a CU
+  const bool four = static_cast<int64_t>(a.seqs.rows) * groups > APPEND_WGS;
+  const int64_t wgs = (four ? (a.seqs.rows + 3) / 4 : a.seqs.rows) * static_cast<int64_t>(groups);
+  if (wgs > INT32_MAX / 256) return hipErrorInvalidValue;
+  const dim3 grid(static_cast<unsigned>(wgs));
+  if (vec && four)
+    hipLaunchKernelGGL((seq_append_kernel<true, 4>), grid, dim3(256), 0, s, a, groups, angles);
+  else if (vec)
+    hipLaunchKernelGGL((seq_append_kernel<true, 1>), grid, dim3(256), 0, s, a, groups, angles);
   else
-    hipLaunchKernelGGL(seq_append_kernel<false>, grid, dim3(256), 0, s, a, groups);
+    hipLaunchKernelGGL((seq_append_kernel<false, 1>), dim3(static_cast<unsigned>(a.seqs.rows * groups)), dim3(256), 0, s, a, groups, angles);
   return hipGetLastError();
 }
 

@@ -47,18 +47,26 @@ __device__ __forceinline__ SeqSpan seq_span(const Seqs &q, int s) {
   return o;
 }
 
-// The sequence that holds a wave-uniform row: as many sequences end at or
-// before it (64 ends a step, one per lane).  n_seq: behind the last one.
-__device__ __forceinline__ int seq_of_row(const Seqs &q, int row) {
+// The sequences that hold the wave-uniform rows row0 .. row0 + ROWS - 1: of each as
+// many as end at or before it (64 ends a step, one per lane).  n_seq: behind the
+// last one.
+template <int ROWS>
+__device__ __forceinline__ void seqs_of_rows(const Seqs &q, int row0, int (&seq)[ROWS]) {
   const int lane = threadIdx.x & 63;
-  int s = 0;
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) seq[r] = 0;
 #pragma unroll 4
   for (int b = 0; b < q.n_seq; b += 64) {
     const int j = b + lane;
-    const bool before = j < q.n_seq && q.start[min(j, q.n_seq - 1) + 1] <= row;
-    s += __popcll(__ballot(before));
+    const int end = j < q.n_seq ? q.start[j + 1] : INT32_MAX;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) seq[r] += __popcll(__ballot(end <= row0 + r));
   }
-  return s;
+}
+__device__ __forceinline__ int seq_of_row(const Seqs &q, int row) {
+  int seq[1];
+  seqs_of_rows<1>(q, row, seq);
+  return seq[0];
 }
 
 // Physical page of a sequence's logical page (0 <= logical * page_tokens <

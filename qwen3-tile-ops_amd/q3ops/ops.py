@@ -241,18 +241,39 @@ def _on_device(t, like) -> None:
         raise ValueError(f"tensors on {t.device} and {like.device}")
 
 
-def _launch_stream(pool: PagedKV, stream, *tensors) -> int:
-    """The stream of a call on the pool's device, which has to be the current
-    one (kernels launch there) and to hold every tensor."""
+def _views(pool: PagedKV, tensors) -> list:
+    """view() of each tensor, all on the pool's device (one loop over them: at one
+    row the wrapper is most of a call's time, and a call per tensor half of that)."""
+    index, out = pool.device.index, []
+    for t in tensors:
+        if t is None:
+            out.append(None)
+            continue
+        if t.get_device() != index:
+            raise ValueError("operator views must point at device memory" if not t.is_cuda
+                             else f"tensors on {t.device} and {pool.device}")
+        known = _DT.get(t.dtype)
+        stride = t.stride()
+        if known is None or len(stride) != 2 or stride[1] != 1:
+            out.append(view(t))  # a vector, or an error
+            continue
+        es, code = known
+        rows, cols = t.shape
+        out.append(byref(View(t.data_ptr(), (stride[0] if rows > 1 else cols) * es, es, rows, cols, code)))
+    return out
+
+
+def _launch_stream(pool: PagedKV, stream) -> int:
+    """The stream of a call on the pool's device, which has to be the current one
+    (kernels launch there)."""
     dev = pool.device
     if dev.index != torch.cuda.current_device():
         raise ValueError(f"the pool is on {dev}, the current device is cuda:{torch.cuda.current_device()}")
-    for t in tensors:
-        if t is not None and t.device != dev:
-            raise ValueError(f"tensors on {t.device} and {dev}")
-    if stream is not None and stream.device != dev:
+    if stream is None:
+        return _raw_stream(dev.index)
+    if stream.device != dev:
         raise ValueError(f"a stream of {stream.device} for a pool on {dev}")
-    return _stream(stream)
+    return stream.cuda_stream
 
 
 def rope_append_paged(q, k, v, pool: PagedKV, seqs: Seqs, q8=None, qs=None, nwq=None, nwk=None, inv_hd=0.0,
@@ -261,11 +282,11 @@ def rope_append_paged(q, k, v, pool: PagedKV, seqs: Seqs, q8=None, qs=None, nwq=
     sequence, normed (gains nwq / nwk), rotated at their positions (cos / sin
     [position, rot_dim / 2], e.g. rope_tables'; None: not rotated), quantised; K
     and V into their pages, Q into q8 / qs (q None: K and V alone)."""
-    check(lib().q3_rope_append_paged(view(q), view(k), view(v), view(nwq), view(nwk), inv_hd, view(cos), view(sin),
-                                     rot_dim if cos is not None else 0, int(interleaved), view(q8), view(qs),
-                                     byref(pool), byref(seqs), 0 if q is None else q.shape[1] // 128, pool.kv_heads,
-                                     _launch_stream(pool, stream, q, k, v, nwq, nwk, cos, sin, q8, qs)),
-          "rope_append_paged")
+    vq, vk, vv, vnq, vnk, vc, vs, v8, vqs = _views(pool, (q, k, v, nwq, nwk, cos, sin, q8, qs))
+    check(lib().q3_rope_append_paged(vq, vk, vv, vnq, vnk, inv_hd, vc, vs, rot_dim if cos is not None else 0,
+                                     int(interleaved), v8, vqs, byref(pool), byref(seqs),
+                                     0 if q is None else q.shape[1] // 128, pool.kv_heads,
+                                     _launch_stream(pool, stream)), "rope_append_paged")
 
 
 def page_bounds(pool: PagedKV, seqs: Seqs, bounds, bscale, rows: int | None = None, stream=None):
@@ -273,8 +294,9 @@ def page_bounds(pool: PagedKV, seqs: Seqs, bounds, bscale, rows: int | None = No
     largest; f32 [pages, kv_heads]) of the pages that the sequences' new rows lie
     in (rows: the call's row count, n_seq * max_rows if not given)."""
     rows = seqs.n_seq * seqs.max_rows if rows is None else rows
-    check(lib().q3_page_bounds(byref(pool), byref(seqs), rows, pool.kv_heads, view(bounds), view(bscale),
-                               _launch_stream(pool, stream, bounds, bscale)), "page_bounds")
+    vb, vs = _views(pool, (bounds, bscale))
+    check(lib().q3_page_bounds(byref(pool), byref(seqs), rows, pool.kv_heads, vb, vs, _launch_stream(pool, stream)),
+          "page_bounds")
 
 
 def seqs_workspace_bytes(pool: PagedKV, seqs: Seqs, rows: int, heads: int, n_sel: int = 0) -> int:
@@ -291,12 +313,15 @@ def _workspace_on(ws, stream, pool, seqs, q8, n_sel):
     memory out again in the order of the current stream)."""
     if ws is None:
         n = seqs_workspace_bytes(pool, seqs, q8.shape[0], q8.shape[1] // 128, n_sel)
-        if n and stream is not None and stream != torch.cuda.current_stream(pool.device):
+        if n == 0:
+            return None, None, 0
+        if stream is not None and stream != torch.cuda.current_stream(pool.device):
             raise ValueError("a call on a stream that is not the current one needs its workspace given")
-        ws = torch.empty(n, dtype=torch.uint8, device=pool.device) if n else None
-    elif not ws.is_contiguous():
-        raise ValueError("the workspace must be contiguous")
-    return (ws, None, 0) if ws is None else (ws, ws.data_ptr(), ws.numel() * ws.element_size())
+        ws = torch.empty(n, dtype=torch.uint8, device=pool.device)
+        return ws, ws.data_ptr(), n
+    if not ws.is_contiguous() or ws.device != pool.device:
+        raise ValueError("the workspace must be contiguous and on the pool's device")
+    return ws, ws.data_ptr(), ws.numel() * ws.element_size()
 
 
 def attention_varlen_paged(q8, q_scale, pool: PagedKV, seqs: Seqs, out=None, o8=None, os=None, causal=True,
@@ -305,31 +330,33 @@ def attention_varlen_paged(q8, q_scale, pool: PagedKV, seqs: Seqs, out=None, o8=
     cached keys; the result in f32 (out) or int8 with a scale per head (o8, os).
     workspace: a device tensor of seqs_workspace_bytes, needed on a stream that
     is not the current one; otherwise one is allocated."""
-    st = _launch_stream(pool, stream, q8, q_scale, out, o8, os, workspace)
+    vq, vs, vo, v8, vos = _views(pool, (q8, q_scale, out, o8, os))
+    st = _launch_stream(pool, stream)
     keep, ws, n = _workspace_on(workspace, stream, pool, seqs, q8, 0)
-    check(lib().q3_attention_varlen_paged(view(q8), view(q_scale), byref(pool), byref(seqs), view(out), view(o8),
-                                          view(os), q8.shape[1] // 128, pool.kv_heads, 128, int(causal), qk_scale,
-                                          ws, n, st), "attention_varlen_paged")
+    check(lib().q3_attention_varlen_paged(vq, vs, byref(pool), byref(seqs), vo, v8, vos, q8.shape[1] // 128,
+                                          pool.kv_heads, 128, int(causal), qk_scale, ws, n, st),
+          "attention_varlen_paged")
 
 
 def select_pages(q8, q_scale, pool: PagedKV, seqs: Seqs, bounds, bscale, ids, n_sel, workspace=None, stream=None):
     """q3_select_pages: the n_sel pages of each row and KV head with the largest
     bounds of a score, into ids (int32 [rows, kv_heads * n_sel])."""
-    st = _launch_stream(pool, stream, q8, q_scale, bounds, bscale, ids, workspace)
+    vq, vs, vb, vbs, vi = _views(pool, (q8, q_scale, bounds, bscale, ids))
+    st = _launch_stream(pool, stream)
     keep, ws, n = _workspace_on(workspace, stream, pool, seqs, q8, n_sel)
-    check(lib().q3_select_pages(view(q8), view(q_scale), byref(pool), byref(seqs), view(bounds), view(bscale),
-                                view(ids), n_sel, q8.shape[1] // 128, pool.kv_heads, ws, n, st), "select_pages")
+    check(lib().q3_select_pages(vq, vs, byref(pool), byref(seqs), vb, vbs, vi, n_sel, q8.shape[1] // 128,
+                                pool.kv_heads, ws, n, st), "select_pages")
 
 
 def attention_pages(q8, q_scale, pool: PagedKV, seqs: Seqs, ids, n_sel, out=None, o8=None, os=None,
                     qk_scale=128 ** -0.5, workspace=None, stream=None):
     """q3_attention_pages: attention_varlen_paged over the keys of each row's
     listed pages (select_pages' ids, or the caller's own)."""
-    st = _launch_stream(pool, stream, q8, q_scale, ids, out, o8, os, workspace)
+    vq, vs, vi, vo, v8, vos = _views(pool, (q8, q_scale, ids, out, o8, os))
+    st = _launch_stream(pool, stream)
     keep, ws, n = _workspace_on(workspace, stream, pool, seqs, q8, n_sel)
-    check(lib().q3_attention_pages(view(q8), view(q_scale), byref(pool), byref(seqs), view(ids), n_sel, view(out),
-                                   view(o8), view(os), q8.shape[1] // 128, pool.kv_heads, 128, qk_scale, ws, n, st),
-          "attention_pages")
+    check(lib().q3_attention_pages(vq, vs, byref(pool), byref(seqs), vi, n_sel, vo, v8, vos, q8.shape[1] // 128,
+                                   pool.kv_heads, 128, qk_scale, ws, n, st), "attention_pages")
 
 
 __all__ = ["Q3Error", "view", "paged_kv", "embedding_rmsnorm_rows", "rmsnorm_rows", "quant_rows_heads",
