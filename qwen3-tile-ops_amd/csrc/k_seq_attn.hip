@@ -227,30 +227,27 @@ __device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, F
   if (split >= p.part.splits) return;
   const int tile = unit % p.tiles;
 
-  int seq, row0 = 0;
-  if constexpr (LIST) {
-    row0 = unit / p.tiles;
-    seq = seq_of_row(a.seqs, row0);
-    if (seq >= a.seqs.n_seq) return;
-  } else {
-    seq = unit / p.tiles;
-  }
-  const SeqSpan sp = seq_span(a.seqs, seq);
   const int pt = a.pool.page_tokens;
 
   // this lane's column, and how many keys it sees
   const int c = tile * FEW_COLS + col;
-  int row, g, cols;
+  int seq, row0, row, g, cols, sees;
   if constexpr (LIST) {
-    if (row0 < sp.r0 || row0 >= sp.r0 + sp.n) return;
-    row = row0, g = c, cols = group_heads;
+    row0 = row = unit / p.tiles, g = c, cols = group_heads;
+    const SeqRow at = row_at(a.seqs, row);
+    if (at.seq < 0) return;
+    seq = at.seq;
+    sees = max(at.pos + 1, 0);
   } else {
+    seq = unit / p.tiles;
+    const SeqSpan sp = seq_span(a.seqs, seq);
     cols = sp.n * group_heads;
     if (cols > p.most || tile * FEW_COLS >= cols) return;
-    row = sp.r0 + c / group_heads, g = c % group_heads;
+    row0 = sp.r0, row = sp.r0 + c / group_heads, g = c % group_heads;
+    sees = a.causal ? max(sp.pos(row) + 1, 0) : sp.kv;
   }
   const bool live = c < cols;
-  const int sees = !live ? 0 : a.causal ? max(sp.pos(row) + 1, 0) : sp.kv;
+  if (!live) sees = 0;
   // the tile's first column sees the fewest keys, its last the most
   const int vmin = __builtin_amdgcn_readlane(sees, 0);
   const int vmax = __builtin_amdgcn_readlane(sees, min(cols - tile * FEW_COLS, FEW_COLS) - 1);
@@ -430,7 +427,7 @@ __device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, F
 #pragma unroll
     for (int i = 0; i < 8; ++i) r[i] += f * src[i];
   }
-  const int jrow = LIST ? row0 : sp.r0 + cc / group_heads;
+  const int jrow = LIST ? row0 : row0 + cc / group_heads;
   const int jhead = kvh * group_heads + (LIST ? cc : cc % group_heads);
   if (p.part.splits == 1) {
 #pragma unroll
@@ -920,16 +917,14 @@ __global__ void __launch_bounds__(256) seq_attn_join_kernel(SeqAttnArgs a, std::
   const int cell = blockIdx.x / blocks;
   const int c = blockIdx.x % blocks * PER + (GROUPS == 1 ? group : 0);  // column of the cell
   const int group_heads = a.heads / a.kv_heads;
-  int seq, row, head, span = p.span;
-  SeqSpan sp;
+  int row, head, n;
   if (!WIDE && a.ids) {
     row = cell, head = c;
-    seq = seq_of_row(a.seqs, row);
-    if (seq >= a.seqs.n_seq) return;
-    sp = seq_span(a.seqs, seq);
-    if (row < sp.r0 || row >= sp.r0 + sp.n || c >= a.heads) return;
+    if (row_at(a.seqs, row).seq < 0 || c >= a.heads) return;
+    n = p.splits;
   } else {
-    int col = c, cols;
+    int col = c, cols, seq, span = p.span;
+    SeqSpan sp;
     if constexpr (WIDE) {
       int nth;
       seq = wide_tile(a, plan, cell / a.kv_heads, &nth, &span, &sp);
@@ -946,9 +941,9 @@ __global__ void __launch_bounds__(256) seq_attn_join_kernel(SeqAttnArgs a, std::
     if (c >= cell_cols || col >= cols) return;
     row = sp.r0 + col / group_heads;
     head = cell % a.kv_heads * group_heads + col % group_heads;
+    const int sees = a.causal ? max(sp.pos(row) + 1, 0) : sp.kv;
+    n = (sees + span - 1) / span;
   }
-  const int sees = a.causal ? max(sp.pos(row) + 1, 0) : sp.kv;
-  const int n = !WIDE && a.ids ? p.splits : (sees + span - 1) / span;
   const int64_t at = (static_cast<int64_t>(cell) * cell_cols + c) * p.splits;
   float top = -INFINITY;
   for (int s = threadIdx.x & 15; s < n; s += 16) top = fmaxf(top, p.ml[at + s].x);

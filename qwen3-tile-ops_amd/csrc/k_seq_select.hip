@@ -112,12 +112,10 @@ __global__ void __launch_bounds__(256) page_pick_kernel(SelectArgs a) {
   __shared__ uint32_t total_s[2][4];
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
   const int row = blockIdx.x / a.kv_heads, head = blockIdx.x % a.kv_heads;
-  const int seq = seq_of_row(a.seqs, row);
-  if (seq >= a.seqs.n_seq) return;
-  const SeqSpan sp = seq_span(a.seqs, seq);
-  if (row < sp.r0 || row >= sp.r0 + sp.n) return;
+  const SeqRow at = row_at(a.seqs, row);
+  if (at.seq < 0) return;
   int32_t *ids = a.ids + row * a.ld_ids + static_cast<int64_t>(head) * a.n_sel;
-  const int last = sp.pos(row) < 0 ? -1 : sp.pos(row) / a.pool.page_tokens;
+  const int last = at.pos < 0 ? -1 : at.pos / a.pool.page_tokens;
   if (last < a.n_sel) {  // every page fits
     for (int i = tid; i < a.n_sel; i += 256) ids[i] = i <= last ? i : -1;
     return;

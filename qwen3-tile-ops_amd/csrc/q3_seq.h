@@ -39,34 +39,46 @@ struct SeqSpan {
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return max(lo, min(x, hi)); }
 
-__device__ __forceinline__ SeqSpan seq_span(const Seqs &q, int s) {
+__device__ __forceinline__ SeqSpan seq_span(const Seqs &q, int begin, int end, int kv) {
   SeqSpan o;
-  o.r0 = clampi(q.start[s], 0, q.rows);
-  o.n = clampi(clampi(q.start[s + 1], 0, q.rows) - o.r0, 0, q.max_rows);
-  o.kv = clampi(q.kv_len[s], 0, q.max_kv);
+  o.r0 = clampi(begin, 0, q.rows);
+  o.n = clampi(clampi(end, 0, q.rows) - o.r0, 0, q.max_rows);
+  o.kv = clampi(kv, 0, q.max_kv);
   return o;
 }
+__device__ __forceinline__ SeqSpan seq_span(const Seqs &q, int s) { return seq_span(q, q.start[s], q.start[s + 1], q.kv_len[s]); }
 
-// The sequences that hold the wave-uniform rows row0 .. row0 + ROWS - 1: of each as
-// many as end at or before it (64 ends a step, one per lane).  n_seq: behind the
-// last one.
+// The sequence of a row (-1: of none) and the row's position in it.
+struct SeqRow {
+  int seq, pos;
+};
+
+// Of the wave-uniform rows row0 .. row0 + ROWS - 1: each is in the sequence behind
+// as many as end at or before it.  64 sequences a step, one per lane, whose starts
+// and lengths come with their ends: one round trip to memory.
 template <int ROWS>
-__device__ __forceinline__ void seqs_of_rows(const Seqs &q, int row0, int (&seq)[ROWS]) {
+__device__ __forceinline__ void rows_at(const Seqs &q, int row0, SeqRow (&at)[ROWS]) {
   const int lane = threadIdx.x & 63;
 #pragma unroll
-  for (int r = 0; r < ROWS; ++r) seq[r] = 0;
-#pragma unroll 4
+  for (int r = 0; r < ROWS; ++r) at[r] = {-1, 0};
+#pragma unroll 2
   for (int b = 0; b < q.n_seq; b += 64) {
-    const int j = b + lane;
-    const int end = j < q.n_seq ? q.start[j + 1] : INT32_MAX;
+    const int j = min(b + lane, q.n_seq - 1);
+    const int begin = q.start[j], end = b + lane < q.n_seq ? q.start[j + 1] : INT32_MAX, kv = q.kv_len[j];
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) seq[r] += __popcll(__ballot(end <= row0 + r));
+    for (int r = 0; r < ROWS; ++r) {
+      const int before = __popcll(__ballot(end <= row0 + r));
+      if (at[r].seq >= 0 || before >= 64 || b + before >= q.n_seq) continue;
+      const SeqSpan sp = seq_span(q, __builtin_amdgcn_readlane(begin, before), __builtin_amdgcn_readlane(end, before),
+                                  __builtin_amdgcn_readlane(kv, before));
+      if (row0 + r >= sp.r0 && row0 + r < sp.r0 + sp.n) at[r] = {b + before, sp.pos(row0 + r)};
+    }
   }
 }
-__device__ __forceinline__ int seq_of_row(const Seqs &q, int row) {
-  int seq[1];
-  seqs_of_rows<1>(q, row, seq);
-  return seq[0];
+__device__ __forceinline__ SeqRow row_at(const Seqs &q, int row) {
+  SeqRow at[1];
+  rows_at<1>(q, row, at);
+  return at[0];
 }
 
 // Physical page of a sequence's logical page (0 <= logical * page_tokens <
