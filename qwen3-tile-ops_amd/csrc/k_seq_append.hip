@@ -58,15 +58,17 @@ __device__ __forceinline__ float ordered_sum4(float s, int lane) {
 // head, 4 columns a lane: a head's reads and writes are then whole 16- and 4-byte
 // words, its 32-column norm blocks 8 lanes each, and a decoding row of 16 + 2 x 8
 // heads is 4 workgroups.  At one row bound by the chain start -> length -> page and
-// angles -> store (4.1 us), at many by how many rows' reads are under way: with one row
-// a workgroup 2048 rows took 24 us, with four, whose loads go out together, 22.
+// angles -> store (4.1 us), at many by the same chain of each workgroup beside what is
+// in flight: 2048 rows (43 MB) take 20.9 us, 24.3 with one row a workgroup, 22.3 with four
+// (more registers, fewer waves); with no arithmetic at all it is 19.
 // VEC: x rows may be read as 16-byte words; angles: so may a lane's angles (and its
 // four columns are rotated alike).
 template <bool VEC, int ROWS>
-__global__ void __launch_bounds__(256) seq_append_kernel(SeqAppendArgs a, int groups, bool angles) {
+__global__ void __launch_bounds__(256, 8) seq_append_kernel(SeqAppendArgs a, int groups, bool angles) {
   __shared__ __align__(16) float ex[8][HD];
   const int lane = threadIdx.x & 63, wave = wave_id();
-  const int row0 = blockIdx.x / groups * ROWS, group = blockIdx.x % groups;
+  const int row_blocks = (a.seqs.rows + ROWS - 1) / ROWS;
+  const int row0 = blockIdx.x % row_blocks * ROWS, group = blockIdx.x / row_blocks;
   const int slot = wave * 2 + (lane >> 5), item = group * 8 + slot;
   const int c0 = 4 * (lane & 31);
   const bool is_q = item < a.heads, is_v = item >= a.heads + a.kv_heads;
@@ -286,17 +288,17 @@ hipError_t launch_seq_append(const SeqAppendArgs &a, hipStream_t s) {
   const auto al16 = [](const void *p, int64_t ld_) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld_ & 3) == 0; };
   const bool vec = (!a.q || al16(a.q, a.ldq)) && al16(a.k, a.ldk) && al16(a.v, a.ldv);
   const bool angles = a.rot > 0 && a.rot % 8 == 0 && al16(a.cos_t, a.ld_cs) && al16(a.sin_t, a.ld_cs);
-  // four rows a workgroup once one a workgroup would leave some waiting for a CU
-  const bool four = static_cast<int64_t>(a.seqs.rows) * groups > APPEND_WGS;
-  const int64_t wgs = (four ? (a.seqs.rows + 3) / 4 : a.seqs.rows) * static_cast<int64_t>(groups);
+  // two rows a workgroup once one a workgroup would leave some waiting for a CU
+  const bool two = vec && static_cast<int64_t>(a.seqs.rows) * groups > APPEND_WGS;
+  const int64_t wgs = (two ? (a.seqs.rows + 1) / 2 : a.seqs.rows) * static_cast<int64_t>(groups);
   if (wgs > INT32_MAX / 256) return hipErrorInvalidValue;
   const dim3 grid(static_cast<unsigned>(wgs));
-  if (vec && four)
-    hipLaunchKernelGGL((seq_append_kernel<true, 4>), grid, dim3(256), 0, s, a, groups, angles);
+  if (two)
+    hipLaunchKernelGGL((seq_append_kernel<true, 2>), grid, dim3(256), 0, s, a, groups, angles);
   else if (vec)
     hipLaunchKernelGGL((seq_append_kernel<true, 1>), grid, dim3(256), 0, s, a, groups, angles);
   else
-    hipLaunchKernelGGL((seq_append_kernel<false, 1>), dim3(static_cast<unsigned>(a.seqs.rows * groups)), dim3(256), 0, s, a, groups, angles);
+    hipLaunchKernelGGL((seq_append_kernel<false, 1>), grid, dim3(256), 0, s, a, groups, angles);
   return hipGetLastError();
 }
 

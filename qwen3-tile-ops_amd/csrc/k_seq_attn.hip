@@ -209,8 +209,10 @@ struct FewLds {
   float m[FEW_WAVES][FEW_COLS], l[FEW_WAVES][FEW_COLS];
 };
 
-// (block: of the workgroups that the plan asks for)
-template <bool LIST>
+// (block: of the workgroups that the plan asks for.)  ONCE: no other workgroup reads
+// these keys, so they are read past the caches (one row at 131072 keys 71 -> 62 us, 64 rows
+// at 2048 keys 71 -> 65; where rows share pages that costs: 92 rows' listed pages 68 -> 83).
+template <bool LIST, bool ONCE>
 __device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, FewLds &lds) {
   const int lane = threadIdx.x & 63, wave = wave_id();
   const int col = lane & 15, quarter = lane >> 4;
@@ -304,9 +306,9 @@ __device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, F
     const int8_t *k = a.pool.k + at, *v = a.pool.v + at;
     const int64_t eight = 8 * a.pool.row_bytes;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) lds_copy16(k + q * eight + lane_k, st + FEW_K + q * 1024);
+    for (int q = 0; q < 4; ++q) lds_copy16<ONCE>(k + q * eight + lane_k, st + FEW_K + q * 1024);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) lds_copy16(v + q * eight + (q < 2 ? lane_v : lane_v4), st + FEW_V + q * 1024);
+    for (int q = 0; q < 4; ++q) lds_copy16<ONCE>(v + q * eight + (q < 2 ? lane_v : lane_v4), st + FEW_V + q * 1024);
     const int64_t sat = page * a.pool.spage + (t0 + (lane & 31)) * a.pool.srow + kvh;
     lds_copy4((lane < 32 ? a.pool.ks : a.pool.vs) + sat, st + FEW_S);
   };
@@ -883,10 +885,10 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
 
 // ---- launches -------------------------------------------------------------------
 
-template <bool LIST>
+template <bool LIST, bool ONCE>
 __global__ void __launch_bounds__(256, 2) seq_attn_few_kernel(SeqAttnArgs a, FewPlan p) {
   __shared__ FewLds lds;
-  few_columns<LIST>(a, p, blockIdx.x, lds);
+  few_columns<LIST, ONCE>(a, p, blockIdx.x, lds);
 }
 
 // Both kinds of sequences in one launch, so that short ones fill the CUs beside the
@@ -899,23 +901,25 @@ __global__ void __launch_bounds__(256, 2) seq_attn_mixed_kernel(SeqAttnArgs a, F
   if (static_cast<int>(blockIdx.x) < wide)
     wide_columns(a, wp, blockIdx.x, lds.wide);
   else
-    few_columns<false>(a, fp, blockIdx.x - wide, lds.few);
+    few_columns<false, true>(a, fp, blockIdx.x - wide, lds.few);
 }
 
 // Joins the splits of slots: 16 lanes of 8 channels a slot, of many splits 16 such
 // groups over the splits in turn (GROUPS; 16 slots a workgroup otherwise).  A cell is
 // what slots are counted in: (sequence, KV head) or row of the 16-column kernel,
 // (tile, KV head) of the 128-column one.
-template <int GROUPS, bool WIDE>
-__global__ void __launch_bounds__(256) seq_attn_join_kernel(SeqAttnArgs a, std::conditional_t<WIDE, WidePlan, FewPlan> plan, int cell_cols) {
+struct JoinLds {
+  float o[4][HD], sum[4];
+};
+
+template <int GROUPS, bool WIDE, class Plan>
+__device__ void join_slots(const SeqAttnArgs &a, const Plan &plan, int cell_cols, int block, JoinLds &lds) {
   const Partials &p = plan.part;
-  __shared__ float o_s[4][HD];
-  __shared__ float sum_s[4];
   constexpr int PER = 16 / GROUPS;
   const int group = threadIdx.x >> 4, d0 = 8 * (threadIdx.x & 15);
   const int blocks = (cell_cols + PER - 1) / PER;
-  const int cell = blockIdx.x / blocks;
-  const int c = blockIdx.x % blocks * PER + (GROUPS == 1 ? group : 0);  // column of the cell
+  const int cell = block / blocks;
+  const int c = block % blocks * PER + (GROUPS == 1 ? group : 0);  // column of the cell
   const int group_heads = a.heads / a.kv_heads;
   int row, head, n;
   if (!WIDE && a.ids) {
@@ -970,33 +974,46 @@ __global__ void __launch_bounds__(256) seq_attn_join_kernel(SeqAttnArgs a, std::
     const int wave = threadIdx.x >> 6;
     if ((threadIdx.x & 63) < 16) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o_s[wave][d0 + i] = r[i];
-      if (d0 == 0) sum_s[wave] = sum;
+      for (int i = 0; i < 8; ++i) lds.o[wave][d0 + i] = r[i];
+      if (d0 == 0) lds.sum[wave] = sum;
     }
     __syncthreads();
     if (threadIdx.x >= 16) return;
-    sum = (sum_s[0] + sum_s[1]) + (sum_s[2] + sum_s[3]);
+    sum = (lds.sum[0] + lds.sum[1]) + (lds.sum[2] + lds.sum[3]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = (o_s[0][d0 + i] + o_s[1][d0 + i]) + (o_s[2][d0 + i] + o_s[3][d0 + i]);
+    for (int i = 0; i < 8; ++i) r[i] = (lds.o[0][d0 + i] + lds.o[1][d0 + i]) + (lds.o[2][d0 + i] + lds.o[3][d0 + i]);
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) r[i] = top == -INFINITY ? 0.0f : r[i] / sum;
   store_row8(a, row, head, d0, r);
 }
 
-template <bool WIDE, class P>
-hipError_t launch_join(const SeqAttnArgs &a, const P &plan, int cell_cols, hipStream_t s) {
-  const Partials &p = plan.part;
-  if (p.slots == 0) return hipSuccess;
-  const int64_t cells = p.slots / cell_cols;
-  const bool many = p.splits > 12;
-  const int64_t wgs = cells * (many ? cell_cols : (cell_cols + 15) / 16);
-  if (wgs > INT32_MAX / 256) return hipErrorInvalidValue;
-  if (many)
-    hipLaunchKernelGGL((seq_attn_join_kernel<16, WIDE>), dim3(static_cast<unsigned>(wgs)), dim3(256), 0, s, a, plan, cell_cols);
-  else
-    hipLaunchKernelGGL((seq_attn_join_kernel<1, WIDE>), dim3(static_cast<unsigned>(wgs)), dim3(256), 0, s, a, plan, cell_cols);
-  return hipGetLastError();
+constexpr int JOIN_MANY = 12;  // splits from which 16 groups share a slot
+
+int join_cols(const SeqAttnArgs &a, const FewPlan &p) { return a.ids ? a.heads : p.most; }
+int join_cols(const SeqAttnArgs &, const WidePlan &) { return WIDE_COLS; }
+
+template <class P>
+int64_t join_wgs(const SeqAttnArgs &a, const P &plan) {
+  const int cols = join_cols(a, plan);
+  return plan.part.slots / cols * (plan.part.splits > JOIN_MANY ? cols : (cols + 15) / 16);
+}
+
+// The first `few` workgroups join the 16-column kernel's slots.
+__global__ void __launch_bounds__(256) seq_attn_join_kernel(SeqAttnArgs a, FewPlan fp, WidePlan wp, int few) {
+  __shared__ JoinLds lds;
+  const int block = blockIdx.x;
+  if (block < few) {
+    const int cols = a.ids ? a.heads : fp.most;
+    if (fp.part.splits > JOIN_MANY)
+      join_slots<16, false>(a, fp, cols, block, lds);
+    else
+      join_slots<1, false>(a, fp, cols, block, lds);
+  } else if (wp.part.splits > JOIN_MANY) {
+    join_slots<16, true>(a, wp, WIDE_COLS, block - few, lds);
+  } else {
+    join_slots<1, true>(a, wp, WIDE_COLS, block - few, lds);
+  }
 }
 
 // ---- plans --------------------------------------------------------------------
@@ -1028,7 +1045,7 @@ void plan_splits(int64_t units, int64_t keys, int64_t want, int step, int least,
 // 40 / 35.
 constexpr int FEW_MOST = 16;
 constexpr int64_t FEW_PAIRS = 6 << 20;
-constexpr int FEW_WANT = 2048, WIDE_WANT = 1536;  // workgroups
+constexpr int FEW_WANT = 1024, WIDE_WANT = 1536;  // workgroups
 
 struct Plan {
   FewPlan few;
@@ -1040,7 +1057,7 @@ Plan plan_attn(const SeqAttnArgs &a) {
   Plan p{};
   const int64_t g = a.heads / a.kv_heads, rows = a.seqs.rows, n_seq = a.seqs.n_seq;
   const int64_t cols = a.ids ? g : a.seqs.max_rows * g;  // of a sequence (listed pages: of a row), at most
-  const bool small = rows * a.heads * a.seqs.max_kv <= FEW_PAIRS && n_seq * cdiv(cols, FEW_COLS) * a.kv_heads <= 4 * FEW_WANT;
+  const bool small = rows * a.heads * a.seqs.max_kv <= FEW_PAIRS && n_seq * cdiv(cols, FEW_COLS) * a.kv_heads <= 8 * FEW_WANT;
   p.any_wide = !a.ids && cols > FEW_MOST && !small;
   const int64_t few_cols = p.any_wide ? FEW_MOST : cols < 1 ? 1 : cols;
   p.few.most = static_cast<int>(few_cols);
@@ -1086,12 +1103,18 @@ hipError_t launch_seq_attn(const SeqAttnArgs &args, hipStream_t s) {
     hipLaunchKernelGGL(seq_attn_mixed_kernel, dim3(static_cast<unsigned>(wide + few)), dim3(256), 0, s, a, p.few, p.wide,
                        static_cast<int>(wide));
   else if (a.ids)
-    hipLaunchKernelGGL(seq_attn_few_kernel<true>, dim3(static_cast<unsigned>(few)), dim3(256), 0, s, a, p.few);
+    hipLaunchKernelGGL((seq_attn_few_kernel<true, false>), dim3(static_cast<unsigned>(few)), dim3(256), 0, s, a, p.few);
+  else if (p.few.tiles == 1)
+    hipLaunchKernelGGL((seq_attn_few_kernel<false, true>), dim3(static_cast<unsigned>(few)), dim3(256), 0, s, a, p.few);
   else
-    hipLaunchKernelGGL(seq_attn_few_kernel<false>, dim3(static_cast<unsigned>(few)), dim3(256), 0, s, a, p.few);
+    hipLaunchKernelGGL((seq_attn_few_kernel<false, false>), dim3(static_cast<unsigned>(few)), dim3(256), 0, s, a, p.few);
   if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  if (const hipError_t e = launch_join<true>(a, p.wide, WIDE_COLS, s); e != hipSuccess) return e;
-  return launch_join<false>(a, p.few, a.ids ? a.heads : p.few.most, s);
+  const int64_t join_few = join_wgs(a, p.few), join = join_few + join_wgs(a, p.wide);
+  if (join == 0) return hipSuccess;
+  if (join > kMaxGrid) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(seq_attn_join_kernel, dim3(static_cast<unsigned>(join)), dim3(256), 0, s, a, p.few, p.wide,
+                     static_cast<int>(join_few));
+  return hipGetLastError();
 }
 
 }  // namespace q3
