@@ -39,10 +39,10 @@ class Batch:
         self.ks = np.full(shape, np.nan, F)
         self.vs = np.full(shape, np.nan, F)
         for i in range(len(lens)):
-            for t in range(max(int(self.kv_len[i]), 0)):
-                p = self.tables[i, t // page]
-                self.ks[p, t % page] = rng.uniform(0.01, 0.03, kv_heads)
-                self.vs[p, t % page] = rng.uniform(0.01, 0.03, kv_heads)
+            t = np.arange(max(int(self.kv_len[i]), 0))
+            p = self.tables[i, t // page]
+            self.ks[p, t % page] = rng.uniform(0.01, 0.03, (len(t), kv_heads))
+            self.vs[p, t % page] = rng.uniform(0.01, 0.03, (len(t), kv_heads))
         self.max_rows = max(n + [0])
         self.max_kv = int(max(list(self.kv_len) + [0]))
 
@@ -75,15 +75,32 @@ def attend(b: Batch, q8, qs, heads, scale, causal=True, ids=None, n_sel=0):
     out = np.zeros((b.rows, heads, 128))
     mag = np.zeros((b.rows, heads, 128))
     top = np.zeros((b.rows, heads))
-    for row, s, pos in b.row_positions():
-        visible = pos + 1 if causal else int(b.kv_len[s])
+    if ids is None:  # a sequence's rows and a KV head's query heads at once
+        for s, (n, _) in enumerate(b.lens):
+            r0, kv = int(b.start[s]), max(int(b.kv_len[s]), 0)
+            if n == 0 or kv == 0:
+                continue
+            pos = int(b.kv_len[s]) - n + np.arange(n)
+            for kvh in range(b.kv_heads):
+                k, v, ok = b.keys(s, kvh, np.arange(kv))
+                k[~ok], v[~ok] = 0, 0
+                sees = ok[None] & ((np.arange(kv)[None] <= pos[:, None]) if causal else True)
+                any_ = sees.any(1)
+                vsum = sees @ (np.abs(v) + 128)
+                for h in range(kvh * g, kvh * g + g):
+                    q = q8[r0:r0 + n, h * 128:(h + 1) * 128].astype(np.float64) * qs[r0:r0 + n, h, None].astype(np.float64)
+                    x = np.where(sees, (q @ k.T) * float(F(scale)), -np.inf)
+                    p = np.exp(x - np.where(any_, x.max(1), 0)[:, None])
+                    p /= np.maximum(p.sum(1), 1e-300)[:, None]
+                    out[r0:r0 + n, h], mag[r0:r0 + n, h] = p @ v, p @ np.abs(v) + 2.0 ** -109 * vsum
+                    top[r0:r0 + n, h] = np.where(any_, np.abs(np.where(sees, x, 0)).max(1), 0)
+        return out.reshape(b.rows, -1), mag.reshape(b.rows, -1), np.repeat(top, 128, 1)
+    for row, s, pos in b.row_positions():  # listed pages, row by row
+        visible = pos + 1
         for kvh in range(b.kv_heads):
-            if ids is None:
-                tok = np.arange(max(visible, 0))
-            else:
-                pages = [p for p in ids[row, kvh * n_sel:(kvh + 1) * n_sel] if 0 <= p < b.tables.shape[1]]
-                tok = np.concatenate([np.arange(p * b.page, (p + 1) * b.page) for p in pages] or [np.zeros(0, int)]).astype(int)
-                tok = tok[tok < visible]
+            pages = [p for p in ids[row, kvh * n_sel:(kvh + 1) * n_sel] if 0 <= p < b.tables.shape[1]]
+            tok = np.concatenate([np.arange(p * b.page, (p + 1) * b.page) for p in pages] or [np.zeros(0, int)]).astype(int)
+            tok = tok[tok < visible]
             k, v, ok = b.keys(s, kvh, tok)
             k, v = k[ok], v[ok]
             if len(k) == 0:

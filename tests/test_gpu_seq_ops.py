@@ -92,6 +92,101 @@ def test_attention_not_causal(cuda, lens):
     check_attention(Batch(LENS[lens], 4, 32, seed=5), 8, causal=False)
 
 
+# more than 6 << 20 (row, head, key) triples: the 128-column tiles, beside 16-column
+# ones for the sequences of few rows
+WIDE = {
+    "prompt": ([(640, 0), (1, 700)], 16, 8, 32),
+    "chunk": ([(600, 101)], 16, 8, 128),
+    "mixed": ([(1, 3000), (200, 51), (0, 5), (33, 900), (2, 40), (9, 0)], 16, 8, 32),
+    "group_of_three": ([(300, 3300), (43, 7)], 6, 2, 96),
+    "one_kv_head": ([(130, 3000), (1, 64)], 16, 1, 32),
+    "group_of_33": ([(70, 2800)], 33, 1, 64),
+    "negative_positions": ([(200, -150), (64, 6400), (40, -40)], 16, 2, 32),
+    "many_splits": ([(20, 9000)], 64, 2, 256),
+    "no_groups": ([(700, 500), (17, 33)], 16, 16, 32),
+}
+
+
+@pytest.mark.parametrize("name", WIDE)
+def test_attention_wide(cuda, name):
+    lens, heads, kv_heads, page = WIDE[name]
+    b = Batch(lens, kv_heads, page, seed=len(name), before=1, behind=2)
+    assert b.rows * heads * b.max_kv > 6 << 20
+    check_attention(b, heads)
+
+
+@pytest.mark.parametrize("name", ["mixed", "negative_positions", "many_splits"])
+def test_attention_wide_not_causal(cuda, name):
+    lens, heads, kv_heads, page = WIDE[name]
+    check_attention(Batch(lens, kv_heads, page, seed=8), heads, causal=False)
+
+
+def test_attention_wide_bad_pages(cuda):
+    b = Batch([(300, 500), (250, 1000), (60, 1000)], 2, 32, seed=1)
+    b.tables[0, [0, 3, 24]] = [b.n_pages, 65535, b.n_pages + 7]
+    b.tables[1, 4:30] = 65535
+    b.tables[2] = 65535
+    assert b.rows * 16 * b.max_kv > 6 << 20
+    check_attention(b, 16)
+
+
+@pytest.mark.parametrize("what", ["wide", "zeros", "tiny", "huge", "negative", "queries"])
+def test_attention_wide_scales(cuda, what):
+    """V scales both sides of what the f16 terms take: a range of 2^4 and more, zeros,
+    near either end of the floats, negative; query scales of zero and below."""
+    b = Batch([(500, 300), (1, 40), (100, 700)], 2, 32, seed=3)
+    assert b.rows * 16 * b.max_kv > 6 << 20
+    scale = {"wide": lambda u: np.exp2(np.floor(u * 9) - 4), "zeros": lambda u: np.where(u < 0.3, 0, 1), "tiny": lambda u: np.full_like(u, 2.0 ** -90),
+             "huge": lambda u: np.full_like(u, 2.0 ** 90), "negative": lambda u: np.where(u < 0.5, -1, 1), "queries": np.ones_like}[what]
+    b.vs *= scale(b.rng.random(b.vs.shape)).astype(F)
+    q8, qs = queries(b.rng, b.rows, 16)
+    if what == "queries":
+        qs[::3] = 0
+        qs[1::3] *= -1
+        qs[2::9, ::3] *= -1
+    want, mag, top = attend(b, q8, qs, 16, QK)
+    pool, seqs = on_device(b)
+    out = torch.empty((b.rows, 2048), device="cuda")
+    ops.attention_varlen_paged(dev(q8), dev(qs), pool, seqs, out, qk_scale=QK)
+    got = out.cpu().numpy()
+    err, bound = np.abs(got - want), attend_bound(mag, top, b.max_kv)
+    assert np.isfinite(got).all() and (err <= bound).all(), float((err / bound).max())
+
+
+def test_attention_wide_strided(cuda):
+    """Result rows that 16-byte words do not fit."""
+    b = Batch([(500, 300), (1, 40)], 2, 32, seed=3)
+    q8, qs = queries(b.rng, b.rows, 16)
+    want, mag, top = attend(b, q8, qs, 16, QK)
+    pool, seqs = on_device(b)
+    wo = torch.full((b.rows, 2048 + 7), 7.5, device="cuda")
+    ops.attention_varlen_paged(dev(q8), dev(qs), pool, seqs, wo[:, 3:2051], qk_scale=QK)
+    got = wo.cpu().numpy()
+    assert (np.abs(got[:, 3:2051] - want) <= attend_bound(mag, top, b.max_kv)).all()
+    assert (got[:, :3] == 7.5).all() and (got[:, 2051:] == 7.5).all()
+
+
+def test_attention_wide_bad_lengths(cuda):
+    b = Batch([(300, 900), (300, 500)], 2, 32, behind=4)
+    assert b.rows * 16 * b.max_kv > 6 << 20
+    q8, qs = queries(b.rng, b.rows, 16)
+    want, mag, top = attend(b, q8, qs, 16, QK)
+    pool, _ = on_device(b)
+    kv_len = b.kv_len.copy()
+    for wrong in (1 << 30, 2147483647, -5, -2147483648):
+        kv_len[0] = wrong
+        seqs = ops.sequences(pool, dev(b.tables), dev(b.start), dev(kv_len), b.max_rows, b.max_kv)
+        out = torch.full((b.rows, 2048), 7.5, device="cuda")
+        ops.attention_varlen_paged(dev(q8), dev(qs), pool, seqs, out, qk_scale=QK)
+        got = out.cpu().numpy()
+        assert (np.abs(got - want) <= attend_bound(mag, top, b.max_kv))[300:600].all() and (got[600:] == 7.5).all()
+    for start in ([0, 300, 1 << 30], [-7, 300, 600], [-2147483648, 2147483647, 600], [600, 300, 0]):
+        seqs = ops.sequences(pool, dev(b.tables), dev(np.array(start, np.int32)), dev(b.kv_len), b.max_rows, b.max_kv)
+        out = torch.full((b.rows + 8, 2048), 7.5, device="cuda")
+        ops.attention_varlen_paged(dev(q8), dev(qs), pool, seqs, out, qk_scale=QK)
+        assert (out.cpu().numpy()[b.rows:] == 7.5).all()
+
+
 def test_attention_rows_around_the_sequences(cuda):
     check_attention(Batch([(3, 100), (1, 50), (40, 8)], 8, 32, before=5, behind=9), 16)
     check_attention(Batch([(1, 100), (1, 50)], 8, 32, before=2, behind=3), 16)
@@ -500,13 +595,13 @@ def test_steps_together(cuda):
                 b.tables[s, (int(b.kv_len[s]) - 1) // page] = free.pop()
 
 
-@pytest.mark.parametrize("rows", [1, 33])
-def test_captured_and_replayed(cuda, rows):
+@pytest.mark.parametrize("rows,context", [(1, 500), (33, 500), (200, 1600)])
+def test_captured_and_replayed(cuda, rows, context):
     """A step captured once and replayed on other lengths, tables and rows, with
     eager calls of the same operators between the replays; two graphs that share
     a workspace, replayed in turn."""
-    heads, kvh, page, n_sel, n = 8, 4, 32, 4, 3
-    b = Batch([(rows, 500)] * n, kvh, page, seed=30, smooth=True)
+    heads, kvh, page, n_sel, n = 8, 4, 32, 4, 3  # (200 rows: the 128-column tiles too)
+    b = Batch([(rows, context)] * n, kvh, page, seed=30, smooth=True)
     pool, _ = on_device(b)
     tk, tv, tks, tvs = pool._keep
     total, max_kv = n * rows, b.max_kv
@@ -532,7 +627,7 @@ def test_captured_and_replayed(cuda, rows):
         with torch.cuda.graph(g, stream=side):
             step(*s, ws)
         graphs.append(g)
-    for lens in ([(rows, 400)] * n, [(rows, 0), (rows, 90), (rows, 500)], [(0, 40), (rows, 33), (1, 31)], [(rows, 500)] * n):
+    for lens in ([(rows, 400)] * n, [(rows, 0), (rows, 90), (rows, 500)], [(0, 40), (rows, 33), (1, 31)], [(rows, context)] * n):
         kv_len.copy_(torch.tensor([r + c for r, c in lens], dtype=torch.int32))
         start.copy_(torch.tensor(np.cumsum([0] + [r for r, _ in lens]).astype(np.int32)))
         eager = new()
