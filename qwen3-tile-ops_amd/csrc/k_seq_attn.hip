@@ -458,19 +458,24 @@ __device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, F
 // in flight: one barrier a step.
 //
 // A matrix instruction takes 33 cycles of its SIMD, under which four to five vector
-// instructions go for nothing; each further one costs 2.5, a conversion from int32 4
-// and an exponential 8 (measured).  So the number of vector instructions counts as
-// much as that of the 20 matrix ones a step: two terms of P instead of three, keys'
-// scales in the scores but the column's in the exponent's FMA, a reference that moves
-// by steps of 2^8, whole steps without a mask in a loop of their own.
+// instructions go for nothing; each further one costs 2.5, a conversion, a packing or
+// a maximum of three 4.5 and an exponential 8.4 (measured).  So the number of vector
+// instructions counts as much as that of the 20 matrix ones a step: two terms of P
+// instead of three, keys' scales in the scores but the column's in the exponent's FMA,
+// a reference that moves by steps of 2^8, whole steps without a mask in a loop of
+// their own, integer scores read as floats.  A wave's step is some 700 cycles of vector
+// and 660 of matrix instructions and takes 1800 of its SIMD: what a step waits
+// beyond its issue is the barrier and the LDS reads.  1700 rows of each of 3 sequences, 32 heads
+// on 8: 128 us, 0.40 of what a large bf16 matrix product reaches for the
+// products that the causal mask leaves.  Runs of matrix and of vector instructions set
+// apart by hand, a wave's priority over its products, 64 keys a step, eight waves that halve the
+// keys and a third workgroup a CU (spills) were not faster.
 //
 // P: where the split's V scales lie within a factor of 16 of each other (as they do
 // but for crafted caches) p * vs fits two f16 numbers, with a reference that puts
-// the largest at 2^7 .. 2^15: 22 bits down to 2^-10 of it, and nothing is off by more
-// than 2^-25 / 2^7.  Otherwise the three bf16 numbers of the 16-column kernel.
-//
-// Two workgroups a CU: a third would fit LDS, but not the registers (spills cost more
-// than it gives), and eight waves that halve the keys were slower for whole prompts.
+// the largest p times the largest vs at 2^6 .. 2^15: 22 bits down to 2^-9 of that, and
+// nothing is off by more than 2^-25 / 2^6 of it.  Otherwise the three bf16 numbers of
+// the 16-column kernel.
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef int v16i __attribute__((ext_vector_type(16)));
 
@@ -493,6 +498,17 @@ struct WidePlan {
 // transposing read (two runs of four, 8 apart) meet 8 chunks.
 __device__ __forceinline__ int vswz_wide(int key) { return (key & 3) | ((key >> 1) & 4); }
 
+__device__ __forceinline__ int wave_sum(int x) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) x += static_cast<int>(lane_xor_m(static_cast<uint32_t>(x), d));
+  return __builtin_amdgcn_readfirstlane(x);
+}
+__device__ __forceinline__ int wave_max(int x) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) x = max(x, static_cast<int>(lane_xor_m(static_cast<uint32_t>(x), d)));
+  return __builtin_amdgcn_readfirstlane(x);
+}
+
 // The sequence of the unit-th tile of 128 columns, -1 behind the last, and which of
 // its tiles it is: tiles are counted 64 sequences at a time, one per lane.  *span:
 // the keys of a split, the plan's or more: with splits as long as the work for each
@@ -513,24 +529,28 @@ __device__ __forceinline__ int wide_tile(const SeqAttnArgs &a, const WidePlan &p
       steps += static_cast<float>(tiles) * static_cast<float>(keys / WIDE_KEYS + 1);
     }
     if (found >= 0) continue;
-    int upto = tiles;  // inclusive sum over the lanes
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int t = __shfl_up(upto, d);
-      upto += lane >= d ? t : 0;
-    }
-    const uint64_t holds = __ballot(upto > unit);
-    if (holds) {
-      const int at = __builtin_ctzll(holds);
-      // a sequence's last rows see the most keys: its tiles start with them
-      *nth = __builtin_amdgcn_readlane(upto, at) - 1 - unit;
+    const int total = wave_sum(tiles);
+    if (unit < total) {
+      // Each sequence's r-th tile from its end comes before any's (r + 1)-th: the last
+      // rows see the most keys, and long tiles are to start first.  r is the largest
+      // number of rounds that are over before this unit.
+      int r = 0;
+      for (int bit = 31 - __builtin_clz(wave_max(tiles)); bit >= 0; --bit) {
+        const int to = r | (1 << bit);
+        if (wave_sum(min(tiles, to)) <= unit) r = to;
+      }
+      const int k = unit - wave_sum(min(tiles, r));  // the k-th sequence with more than r tiles
+      const uint64_t left = __ballot(tiles > r);
+      const bool is = tiles > r && __popcll(left & ((1ull << lane) - 1)) == k;
+      const int at = __builtin_ctzll(__ballot(is));
+      *nth = __builtin_amdgcn_readlane(tiles, at) - 1 - r;
       *seq = {__builtin_amdgcn_readlane(sp.r0, at), __builtin_amdgcn_readlane(sp.n, at), __builtin_amdgcn_readlane(sp.kv, at)};
       found = b + at;
     }
-    unit -= __builtin_amdgcn_readlane(upto, 63);
+    unit -= total;
   }
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) steps += __shfl_xor(steps, d);
+  for (int d = 1; d < 64; d *= 2) steps += __uint_as_float(lane_xor_m(__float_as_uint(steps), d));
   const float each = steps * static_cast<float>(a.kv_heads) / WIDE_SLOTS;
   const int even = static_cast<int>(fminf(each, static_cast<float>(WIDE_SPAN / WIDE_KEYS))) * WIDE_KEYS;
   *span = __builtin_amdgcn_readfirstlane(max(p.part.span, even));
@@ -666,23 +686,31 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
   for (int t = 0; t < 4; ++t)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
-  const float size = fabsf(cs);
+  const float size = fabsf(cs), sign = __builtin_copysignf(1.0f, cs);
   const bool turned = __ballot(cs < 0.0f) != 0;  // some column's scale is negative
 
-  // S of a step, as int32.
-  auto products = [&](int step, v16i &s) {
+  // S of a step, |S| <= 2^21, on top of the bits of 1.5 * 2^23: as f32, that plus S (a
+  // subtraction then instead of a conversion, which takes twice its time).
+  constexpr int kOnTop = 0x4B400000;
+  v16i on_top;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = 0;
+  for (int i = 0; i < 16; ++i) on_top[i] = kOnTop;
+  asm volatile("" : "+v"(on_top));  // kept in registers, not made anew in every step
+  auto products = [&](const v4i_d (&kf)[4], v16i &s) {
+    s = __builtin_amdgcn_mfma_i32_32x32x32_i8(kf[0], qf[0], on_top, 0, 0, 0);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const v4i_d kf = *reinterpret_cast<const v4i_d *>(st.k[step % WIDE_DEPTH] + n32 * HD + 16 * ((2 * i + half) ^ (n32 & 7)));
-      s = __builtin_amdgcn_mfma_i32_32x32x32_i8(kf, qf[i], s, 0, 0, 0);
-    }
+    for (int i = 1; i < 4; ++i) s = __builtin_amdgcn_mfma_i32_32x32x32_i8(kf[i], qf[i], s, 0, 0, 0);
+  };
+  auto keys_of = [&](int step, v4i_d (&kf)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      kf[i] = *reinterpret_cast<const v4i_d *>(st.k[step % WIDE_DEPTH] + n32 * HD + 16 * ((2 * i + half) ^ (n32 & 7)));
   };
 
   // Their scores but for the column's scale: register i is key 8 (i / 4) + 4 half +
-  // i % 4.  EDGE: some column does not see some key; `seen` keeps which, since
-  // nothing of that key may enter the sums, not even a scale's NaN.
+  // i % 4.  EDGE: some column does not see some key, or has a negative scale; `seen`
+  // keeps which, since nothing of that key may enter the sums, not even a scale's NaN.  Returns the
+  // column's largest score in base 2, less lift.
   float x[16];
   uint32_t seen = ~0u;
   auto scores = [&](int step, const v16i &s, auto edge_tag) {
@@ -691,16 +719,14 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
     for (int i = 0; i < 4; ++i) {
       const v4f ks = *reinterpret_cast<const v4f *>(lds.sc[step % (2 * WIDE_DEPTH)] + 8 * i + 4 * half);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[4 * i + j] = static_cast<float>(s[4 * i + j]) * ks[j];
-    }
-    if (turned) {
-      const float sign = __builtin_copysignf(1.0f, cs);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] *= sign;
-      asm volatile("");  // a branch, not sixteen selects in every step
+      for (int j = 0; j < 4; ++j) x[4 * i + j] = (__int_as_float(s[4 * i + j]) - __int_as_float(kOnTop)) * ks[j];
     }
     seen = ~0u;
     if constexpr (EDGE) {
+      if (turned) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] *= sign;
+      }
       seen = 0;
       const int limit = lds.block[step].x < 0 ? 0 : sees - (first + step * WIDE_KEYS + 4 * half);
 #pragma unroll
@@ -713,11 +739,11 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
     float mb = x[0];
 #pragma unroll
     for (int i = 1; i < 16; ++i) mb = fmaxf(mb, x[i]);
-    {
-      const LanePair pr = lane_pair32(__float_as_uint(mb));
-      mb = fmaxf(__uint_as_float(pr.a), __uint_as_float(pr.b));
-    }
-    const float top = mb == -INFINITY ? -INFINITY : mb * size - lift;
+    const LanePair pr = lane_pair32(__float_as_uint(mb));
+    mb = fmaxf(__uint_as_float(pr.a), __uint_as_float(pr.b));
+    return mb == -INFINITY ? -INFINITY : mb * size - lift;
+  };
+  auto refer = [&](float top) {
     if (__ballot(top > base + WIDE_ROOM)) {
       const float to = fmaxf(top, base);
       const float alpha = base == -INFINITY ? 0.0f : exp2_from(base, to);
@@ -728,39 +754,41 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
     }
   };
 
-  // P and O += P V of the step whose scores are at hand.
-  auto values = [&](int step, auto edge_tag, auto narrow_tag) {
+  // P of 16 keys (registers 8 r .. 8 r + 7) times their V scales, in the terms that
+  // the matrix cores take.
+  auto weights = [&](int step, int r, auto edge_tag, auto narrow_tag) {
     constexpr bool EDGE = decltype(edge_tag)::value;
+    const float *vs = lds.sc[step % (2 * WIDE_DEPTH)] + KB + 16 * r + 4 * half;
+    const v4f va = *reinterpret_cast<const v4f *>(vs), vc = *reinterpret_cast<const v4f *>(vs + 8);
+    float e[8], pv[8];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {  // 16 keys: registers 8 r .. 8 r + 7
-      const float *vs = lds.sc[step % (2 * WIDE_DEPTH)] + KB + 16 * r + 4 * half;
-      const v4f va = *reinterpret_cast<const v4f *>(vs), vc = *reinterpret_cast<const v4f *>(vs + 8);
-      float e[8], pv[8];
+    for (int j = 0; j < 8; ++j) {
+      e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * r + j], size, -base));
+      const bool in = !EDGE || (seen >> (8 * r + j) & 1);
+      if (!in) e[j] = 0.0f;
+      pv[j] = e[j] * (j < 4 ? va[j] : vc[j - 4]);
+      if (!in) pv[j] = 0.0f;
+    }
+    l += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+    if constexpr (decltype(narrow_tag)::value)
+      return split_f16(pv);
+    else
+      return split_bf16(pv);
+  };
+  auto values = [&](int step, int r, const auto &pb) {
+    const uint8_t *vt = st.vt[step & 1] + (r * 4 * 64 + lane) * 16;
+    if constexpr (std::is_same_v<std::decay_t<decltype(pb)>, F16x2>) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * r + j], size, -base));
-        const bool in = !EDGE || (seen >> (8 * r + j) & 1);
-        if (!in) e[j] = 0.0f;
-        pv[j] = e[j] * (j < 4 ? va[j] : vc[j - 4]);
-        if (!in) pv[j] = 0.0f;
-      }
-      l += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
-      const uint8_t *vt = st.vt[step & 1] + (r * 4 * 64 + lane) * 16;
-      if constexpr (decltype(narrow_tag)::value) {
-        const F16x2 pb = split_f16(pv);
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int t = 0; t < 4; ++t)
+          o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const v8h *>(vt + t * 1024), pb.part[u], o[t], 0, 0, 0);
+    } else {
 #pragma unroll
-          for (int t = 0; t < 4; ++t)
-            o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const v8h *>(vt + t * 1024), pb.part[u], o[t], 0, 0, 0);
-      } else {
-        const Bf16x3 pb = split_bf16(pv);
+      for (int u = 0; u < 3; ++u)
 #pragma unroll
-        for (int u = 0; u < 3; ++u)
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-            o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const v8bf *>(vt + t * 1024), pb.part[u], o[t], 0, 0, 0);
-      }
+        for (int t = 0; t < 4; ++t)
+          o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const v8bf *>(vt + t * 1024), pb.part[u], o[t], 0, 0, 0);
     }
   };
 
@@ -787,12 +815,15 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
       const bool more = !decltype(edge_tag)::value || step + 1 < steps;
       if (step + WIDE_DEPTH < steps) copy(step + WIDE_DEPTH);
       v16i s;
-      if (more) {
-        products(step + 1, s);
-        turn(step + 1, narrow_tag);
-      }
-      values(step, edge_tag, narrow_tag);
-      if (more) scores(step + 1, s, edge_tag);
+      v4i_d kf[4];
+      if (more) keys_of(step + 1, kf);
+      const auto p0 = weights(step, 0, edge_tag, narrow_tag);
+      if (more) products(kf, s);
+      const auto p1 = weights(step, 1, edge_tag, narrow_tag);
+      values(step, 0, p0);
+      if (more) turn(step + 1, narrow_tag);
+      values(step, 1, p1);
+      if (more) refer(scores(step + 1, s, edge_tag));
       // the step after next is needed now; those behind it may be on their way, as
       // many copies as a wave issues for them (fewer where a page is missing)
       if (missing || step + WIDE_DEPTH >= steps)
@@ -807,13 +838,16 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
   auto all = [&](auto narrow_tag) {
     turn(0, narrow_tag);
     v16i s;
-    products(0, s);
-    scores(0, s, std::true_type{});
+    v4i_d kf[4];
+    keys_of(0, kf);
+    products(kf, s);
+    refer(scores(0, s, std::true_type{}));
     lds_barrier();
     // Steps that every column sees whole, then the others (all, where a page is
-    // missing): two loops, since one with both forms of a step keeps O twice.
+    // missing or a scale negative): two loops, since one with both forms of a step
+    // keeps O twice.
     if constexpr (decltype(narrow_tag)::value)
-      run(missing ? 0 : clampi((tile_min - first) / WIDE_KEYS, 0, steps) - 1, std::false_type{}, narrow_tag);
+      run(missing || turned ? 0 : clampi((tile_min - first) / WIDE_KEYS, 0, steps) - 1, std::false_type{}, narrow_tag);
     run(steps, std::true_type{}, narrow_tag);
   };
   if (steps > 0) {
