@@ -462,20 +462,21 @@ __device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, F
 // a maximum of three 4.5 and an exponential 8.4 (measured).  So the number of vector
 // instructions counts as much as that of the 20 matrix ones a step: two terms of P
 // instead of three, keys' scales in the scores but the column's in the exponent's FMA,
-// a reference that moves by steps of 2^8, whole steps without a mask in a loop of
+// a reference that moves by steps of 2^4, whole steps without a mask in a loop of
 // their own, integer scores read as floats.  A wave's step is some 700 cycles of vector
 // and 660 of matrix instructions and takes 1800 of its SIMD: what a step waits
-// beyond its issue is the barrier and the LDS reads.  1700 rows of each of 3 sequences, 32 heads
-// on 8: 128 us, 0.40 of what a large bf16 matrix product reaches for the
-// products that the causal mask leaves.  Runs of matrix and of vector instructions set
-// apart by hand, a wave's priority over its products, 64 keys a step, eight waves that halve the
-// keys and a third workgroup a CU (spills) were not faster.
+// beyond its issue is the barrier and the LDS reads.  Three prompts of 1700 rows, 32
+// heads on 8: 129 us, 0.40 of the rate of a large bf16 matrix product for the products
+// that the causal mask leaves.  Matrix and vector instructions set apart by hand, a
+// wave's priority over its products, 64 keys a step, eight waves that halve the keys
+// and a third workgroup a CU (spills) were not faster.
 //
-// P: where the split's V scales lie within a factor of 16 of each other (as they do
-// but for crafted caches) p * vs fits two f16 numbers, with a reference that puts
-// the largest p times the largest vs at 2^6 .. 2^15: 22 bits down to 2^-9 of that, and
-// nothing is off by more than 2^-25 / 2^6 of it.  Otherwise the three bf16 numbers of
-// the 16-column kernel.
+// P: where the split's V scales lie within a factor of 2^8 of each other p * vs fits
+// two f16 numbers, with a reference that puts the largest p times the largest vs at
+// 2^10 .. 2^15, so the key of the largest p at 2^2 or above: 22 bits from 2^-3 up, and
+// below nothing is off by more than 2^-25, 2^-27 of that key.  Otherwise the three bf16
+// numbers of the 16-column kernel, with a third more time (three prompts of 1700 rows
+// 170 us).
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef int v16i __attribute__((ext_vector_type(16)));
 
@@ -486,7 +487,7 @@ constexpr int WIDE_WAVES = 4;
 constexpr int WIDE_DEPTH = 4;      // steps whose K and V lie in LDS or on their way
 constexpr int WIDE_SPAN = 8192;   // keys of a split: its blocks' places lie in LDS
 constexpr int WIDE_OROW = 32 + 4;  // floats of a column's row where the results turn
-constexpr float WIDE_ROOM = 8.0f;  // P may reach 2^8 of its reference before O is scaled down
+constexpr float WIDE_ROOM = 4.0f;  // P may reach 2^4 of its reference before O is scaled down
 
 struct WidePlan {
   Partials part;  // slots: (tile, KV head, column)
@@ -672,11 +673,11 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
   wait_copies<0>();
   lds_barrier();
   const uint32_t most = __builtin_amdgcn_readfirstlane(lds.range[0]), least = __builtin_amdgcn_readfirstlane(lds.range[1]);
-  // Narrow: exponents 4 apart at most, and no closer to the ends than 2^64.
+  // Narrow: within a factor of 2^8, and no closer to the ends than 2^64.
   const int expo = static_cast<int>(most >> 23) - 127;
-  const bool narrow = most == 0 || (expo >= -64 && expo <= 64 && least >= most - (4u << 23));
-  // with p = 2^(x - base), base = the largest x less `lift`: p vs <= 2^7 there
-  const float lift = narrow && most ? static_cast<float>(6 - expo) : 0.0f;
+  const bool narrow = most == 0 || (expo >= -64 && expo <= 64 && least >= most - (8u << 23));
+  // with p = 2^(x - base), base = the largest x less `lift`: p vs < 2^11 there
+  const float lift = narrow && most ? static_cast<float>(10 - expo) : 0.0f;
 
   // The softmax's reference (base 2), at most WIDE_ROOM short of the largest score
   // less lift, so that O is scaled down a few times in all, not at every new maximum.

@@ -130,13 +130,14 @@ def test_attention_wide_bad_pages(cuda):
     check_attention(b, 16)
 
 
-@pytest.mark.parametrize("what", ["wide", "zeros", "tiny", "huge", "negative", "queries"])
+@pytest.mark.parametrize("what", ["wide", "within", "zeros", "tiny", "huge", "negative", "queries"])
 def test_attention_wide_scales(cuda, what):
-    """V scales both sides of what the f16 terms take: a range of 2^4 and more, zeros,
+    """V scales both sides of what the f16 terms take: a range of 2^8 and more, one of 2^7, zeros,
     near either end of the floats, negative; query scales of zero and below."""
     b = Batch([(500, 300), (1, 40), (100, 700)], 2, 32, seed=3)
     assert b.rows * 16 * b.max_kv > 6 << 20
-    scale = {"wide": lambda u: np.exp2(np.floor(u * 9) - 4), "zeros": lambda u: np.where(u < 0.3, 0, 1), "tiny": lambda u: np.full_like(u, 2.0 ** -90),
+    scale = {"wide": lambda u: np.exp2(np.floor(u * 9) - 4), "within": lambda u: np.exp2(np.floor(u * 7) - 3),
+             "zeros": lambda u: np.where(u < 0.3, 0, 1), "tiny": lambda u: np.full_like(u, 2.0 ** -90),
              "huge": lambda u: np.full_like(u, 2.0 ** 90), "negative": lambda u: np.where(u < 0.5, -1, 1), "queries": np.ones_like}[what]
     b.vs *= scale(b.rng.random(b.vs.shape)).astype(F)
     q8, qs = queries(b.rng, b.rows, 16)
