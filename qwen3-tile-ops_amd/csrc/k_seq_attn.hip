@@ -221,8 +221,8 @@ __device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, F
   // XCD, whose L2 then holds the lines of scales that they share.
   const int group_heads = a.heads / a.kv_heads;
   const int rest = block >> 3;
-  const int kvh = rest % a.kv_heads;
-  const int us = (rest / a.kv_heads) * 8 + (block & 7);
+  const int kvh = ONCE ? rest % a.kv_heads : block % a.kv_heads;
+  const int us = ONCE ? (rest / a.kv_heads) * 8 + (block & 7) : block / a.kv_heads;
   // Split by split: the dispatcher goes round the CUs' groups strictly, so a pattern
   // of splits with work and without would leave some of them idle.
   const int unit = us % static_cast<int>(p.units), split = us / static_cast<int>(p.units);
@@ -1137,6 +1137,8 @@ hipError_t launch_seq_attn(const SeqAttnArgs &args, hipStream_t s) {
   if (wide)
     hipLaunchKernelGGL(seq_attn_mixed_kernel, dim3(static_cast<unsigned>(wide + few)), dim3(256), 0, s, a, p.few, p.wide,
                        static_cast<int>(wide));
+  else if (a.ids && a.seqs.max_rows <= 1)
+    hipLaunchKernelGGL((seq_attn_few_kernel<true, true>), dim3(static_cast<unsigned>(few)), dim3(256), 0, s, a, p.few);
   else if (a.ids)
     hipLaunchKernelGGL((seq_attn_few_kernel<true, false>), dim3(static_cast<unsigned>(few)), dim3(256), 0, s, a, p.few);
   else if (p.few.tiles == 1)
