@@ -182,20 +182,24 @@ __device__ __forceinline__ float exp2_from(float x, float base) { return __built
 // A workgroup takes one tile of 16 columns, one KV head and one split of the keys;
 // its four waves take 32-key blocks in turn, each with its own running maximum and
 // sum, and join at the end.  A block is K [32][128] and V [32][128] int8 and their
-// 64 scales, 8.25 KiB: copied straight into the wave's own LDS stage while the block
-// before is worked on, so no wave waits for another and what is in flight costs no
-// registers.  16-byte chunk c of key r lies at chunk c ^ (r & 7) (V: c ^ vswz(r)),
-// so that neither the K operand's reads (16 keys, one chunk) nor the transposing
-// reads of V (8 keys, one chunk) meet in a bank.
+// 64 scales, 8.25 KiB, copied straight into the wave's own LDS, so no wave waits for
+// another and what is in flight costs no registers: K into its one place once the block's
+// scores are formed, V and the scales beside those of the block before.  12.5 KiB a
+// wave then, and three workgroups a CU (with two places for K two: 92 rows' lists of
+// pages 58 us instead of 49, 256 rows at 1000 keys 110 instead of 101; K straight to
+// registers, four a CU, reads half lines: 32 rows at 16000 keys 233 us instead of 208).  16-byte chunk
+// c of key r lies at chunk c ^ (r & 7) (V: c ^ vswz(r)), so that neither the K
+// operand's reads (16 keys, one chunk) nor the transposing reads of V (8 keys, one
+// chunk) meet in a bank.
 constexpr int KB = 32;
 constexpr int FEW_COLS = 16;
 constexpr int FEW_WAVES = 4;
-constexpr int FEW_STAGES = 2;
-constexpr int FEW_COPIES = 9;  // of a block: 4 K, 4 V, 1 scales
-constexpr int FEW_K = 0, FEW_V = KB * HD, FEW_S = 2 * KB * HD, FEW_STAGE = 2 * KB * HD + 2 * KB * 4;
+constexpr int FEW_STAGES = 2;  // of V and the scales
+constexpr int FEW_V = 0, FEW_S = KB * HD, FEW_STAGE = KB * HD + 2 * KB * 4;
+constexpr int FEW_K = FEW_STAGES * FEW_STAGE, FEW_WAVE = FEW_K + KB * HD;  // bytes of a wave
 constexpr int FEW_ROW = HD + 4;  // floats of a column's row where the waves join
 constexpr int FEW_SPAN = 64 * KB * FEW_WAVES;  // keys of a split: a lane of each wave names one block
-static_assert(FEW_WAVES * FEW_COLS * FEW_ROW * 4 <= FEW_WAVES * FEW_STAGES * FEW_STAGE, "the join fits the stages");
+static_assert(FEW_WAVES * FEW_COLS * FEW_ROW * 4 <= FEW_WAVES * FEW_WAVE, "the join fits the stages");
 
 struct FewPlan {
   Partials part;  // slots: (sequence, KV head, column), of listed pages (row, head)
@@ -205,20 +209,22 @@ struct FewPlan {
 };
 
 struct FewLds {
-  __align__(16) uint8_t stage[FEW_WAVES * FEW_STAGES * FEW_STAGE];
+  __align__(16) uint8_t stage[FEW_WAVES * FEW_WAVE];
   float m[FEW_WAVES][FEW_COLS], l[FEW_WAVES][FEW_COLS];
 };
 
 // (block: of the workgroups that the plan asks for.)  ONCE: no other workgroup reads
-// these keys, so they are read past the caches (one row at 131072 keys 71 -> 62 us, 64 rows
-// at 2048 keys 71 -> 65; where rows share pages that costs: 92 rows' listed pages 68 -> 83).
+// these keys, so they are read past the caches (one row at 131072 keys 69 -> 62 us, 32
+// rows at 16000 232 -> 208; where rows share pages that costs: 92 rows' lists 48 -> 58).
 template <bool LIST, bool ONCE>
 __device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, FewLds &lds) {
   const int lane = threadIdx.x & 63, wave = wave_id();
   const int col = lane & 15, quarter = lane >> 4;
 
-  // Workgroups go round the 8 XCDs: the KV heads of one (unit, split) share an
-  // XCD, whose L2 then holds the lines of scales that they share.
+  // Workgroups go round the 8 XCDs.  Keys read once: the KV heads of one (unit, split)
+  // share an XCD, whose L2 then holds the lines of scales that they share.  Others: a KV
+  // head keeps to its XCD, whose L2 then holds the pages that rows share (92 rows' lists
+  // 59 -> 48 us; 64 lists of one row each 83 -> 95).
   const int group_heads = a.heads / a.kv_heads;
   const int rest = block >> 3;
   const int kvh = ONCE ? rest % a.kv_heads : block % a.kv_heads;
@@ -294,7 +300,7 @@ __device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, F
     cs = a.qs[row * a.ldqs + (kvh * group_heads + g) * a.qs_col] * a.qk_scale * kLog2e;
   }
 
-  uint8_t *const stages = lds.stage + wave * FEW_STAGES * FEW_STAGE;
+  uint8_t *const stages = lds.stage + wave * FEW_WAVE;
   const int r8 = lane >> 3, ch = lane & 7;
   const int64_t lane_k = r8 * a.pool.row_bytes + 16 * (ch ^ r8);
   const int64_t lane_v = r8 * a.pool.row_bytes + 16 * (ch ^ (r8 & 3));
@@ -306,7 +312,7 @@ __device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, F
     const int8_t *k = a.pool.k + at, *v = a.pool.v + at;
     const int64_t eight = 8 * a.pool.row_bytes;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) lds_copy16<ONCE>(k + q * eight + lane_k, st + FEW_K + q * 1024);
+    for (int q = 0; q < 4; ++q) lds_copy16<ONCE>(k + q * eight + lane_k, stages + FEW_K + q * 1024);
 #pragma unroll
     for (int q = 0; q < 4; ++q) lds_copy16<ONCE>(v + q * eight + (q < 2 ? lane_v : lane_v4), st + FEW_V + q * 1024);
     const int64_t sat = page * a.pool.spage + (t0 + (lane & 31)) * a.pool.srow + kvh;
@@ -329,23 +335,13 @@ __device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, F
     const int now = ahead;
     uint8_t *const st = stages + buf * FEW_STAGE;
     buf ^= 1;
-    ahead = -1;
-    if (todo) {
-      ahead = __builtin_ctzll(todo);
-      todo &= todo - 1;
-      // the reads of the block that lay there have been used
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      issue(ahead, stages + buf * FEW_STAGE);
-      wait_copies<FEW_COPIES>();
-    } else {
-      wait_copies<0>();
-    }
+    wait_copies<0>();
 
     // S^T of two 16-key tiles: lane holds keys 4 quarter + i of each
     float x[8], vsc[8];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const uint8_t *kr = st + FEW_K + (t * 16 + col) * HD;
+      const uint8_t *kr = stages + FEW_K + (t * 16 + col) * HD;
       const v4i_d k0 = *reinterpret_cast<const v4i_d *>(kr + 16 * (quarter ^ (col & 7)));
       const v4i_d k1 = *reinterpret_cast<const v4i_d *>(kr + 16 * ((4 + quarter) ^ (col & 7)));
       v4i_d s = {0, 0, 0, 0};
@@ -358,6 +354,14 @@ __device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, F
         x[4 * t + i] = static_cast<float>(s[i]) * ks[i] * cs;
         vsc[4 * t + i] = vs[i];
       }
+    }
+    ahead = -1;
+    if (todo) {
+      ahead = __builtin_ctzll(todo);
+      todo &= todo - 1;
+      // the reads of this block's K, and of the block before, have been used
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      issue(ahead, stages + buf * FEW_STAGE);
     }
     const int key0 = __builtin_amdgcn_readlane(bkey, now);
     const bool edge = key0 + KB > vmin;  // some column does not see the whole block
@@ -921,7 +925,7 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
 // ---- launches -------------------------------------------------------------------
 
 template <bool LIST, bool ONCE>
-__global__ void __launch_bounds__(256, 2) seq_attn_few_kernel(SeqAttnArgs a, FewPlan p) {
+__global__ void __launch_bounds__(256, 3) seq_attn_few_kernel(SeqAttnArgs a, FewPlan p) {
   __shared__ FewLds lds;
   few_columns<LIST, ONCE>(a, p, blockIdx.x, lds);
 }
@@ -1080,7 +1084,9 @@ void plan_splits(int64_t units, int64_t keys, int64_t want, int step, int least,
 // 40 / 35.
 constexpr int FEW_MOST = 16;
 constexpr int64_t FEW_PAIRS = 6 << 20;
-constexpr int FEW_WANT = 1024, WIDE_WANT = 1536;  // workgroups
+// Workgroups to split for: equal lists of pages 1024, sequences, whose lengths differ,
+// more (64 rows at 500 .. 4000 keys 1024: 62 us, 1536: 56, 2304: 56; 92 rows' lists 49, 53, 56).
+constexpr int LIST_WANT = 1024, FEW_WANT = 1536, WIDE_WANT = 1536;
 
 struct Plan {
   FewPlan few;
@@ -1098,8 +1104,8 @@ Plan plan_attn(const SeqAttnArgs &a) {
   p.few.most = static_cast<int>(few_cols);
   p.few.tiles = static_cast<int>(cdiv(few_cols, FEW_COLS));
   p.few.units = (a.ids ? rows : n_seq) * p.few.tiles;
-  plan_splits(p.few.units * a.kv_heads, a.ids ? int64_t(a.n_sel) * a.pool.page_tokens : a.seqs.max_kv, FEW_WANT, FEW_WAVES * KB, 256,
-              FEW_SPAN, p.few.part);
+  plan_splits(p.few.units * a.kv_heads, a.ids ? int64_t(a.n_sel) * a.pool.page_tokens : a.seqs.max_kv,
+              a.ids ? LIST_WANT : FEW_WANT, FEW_WAVES * KB, 256, FEW_SPAN, p.few.part);
   if (p.few.part.splits > 1) p.few.part.slots = a.ids ? rows * a.heads : n_seq * a.kv_heads * few_cols;
   if (p.any_wide) {
     p.wide.least = FEW_MOST + 1;
