@@ -433,11 +433,12 @@ __device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, F
 #pragma unroll
     for (int i = 0; i < 8; ++i) r[i] += f * src[i];
   }
+  // (no key at all: zeros; scores that are all NaN leave a sum of NaN)
   const int jrow = LIST ? row0 : row0 + cc / group_heads;
   const int jhead = kvh * group_heads + (LIST ? cc : cc % group_heads);
   if (p.part.splits == 1) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = top == -INFINITY ? 0.0f : r[i] / sum;
+    for (int i = 0; i < 8; ++i) r[i] = sum == 0.0f ? 0.0f : r[i] / sum;
     store_row8(a, jrow, jhead, d0, r);
     return;
   }
@@ -1023,7 +1024,7 @@ __device__ void join_slots(const SeqAttnArgs &a, const Plan &plan, int cell_cols
     for (int i = 0; i < 8; ++i) r[i] = (lds.o[0][d0 + i] + lds.o[1][d0 + i]) + (lds.o[2][d0 + i] + lds.o[3][d0 + i]);
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = top == -INFINITY ? 0.0f : r[i] / sum;
+  for (int i = 0; i < 8; ++i) r[i] = sum == 0.0f ? 0.0f : r[i] / sum;
   store_row8(a, row, head, d0, r);
 }
 

@@ -255,6 +255,53 @@ def test_attention_scales(cuda):
     assert (err <= bound).all(), float((err / bound).max())
 
 
+@pytest.mark.parametrize("kind", ["few", "many", "listed"])
+def test_attention_nan(cuda, kind):
+    """A NaN query, key or value scale reaches the results that it enters, whole rows of
+    a head, and no other."""
+    lens, page = ([(500, 300), (1, 40), (100, 700)] if kind == "many" else [(5, 700), (1, 40), (3, 2)]), 32
+    b = Batch(lens, 2, page, seed=4)
+    heads = 16 if kind == "many" else 4
+    assert (b.rows * heads * b.max_kv > 6 << 20) == (kind == "many")
+    q8, qs = queries(b.rng, b.rows, heads)
+    n_sel = 4
+    ids = np.tile(np.arange(n_sel, dtype=np.int32), (b.rows, 2))
+    pool, seqs = on_device(b)
+    tq = dev(q8)
+
+    def run(pool, qs):
+        out = torch.empty((b.rows, heads * 128), device="cuda")
+        if kind == "listed":
+            ops.attention_pages(tq, dev(qs), pool, seqs, dev(ids), n_sel, out, qk_scale=QK)
+        else:
+            ops.attention_varlen_paged(tq, dev(qs), pool, seqs, out, qk_scale=QK)
+        return out.cpu().numpy().reshape(b.rows, heads, 128)
+
+    plain = run(pool, qs)
+    assert np.isfinite(plain).all()
+    _, mag, top = attend(b, q8, qs, heads, QK, True, ids if kind == "listed" else None, n_sel)
+    # both runs are within the bound of the same value
+    twice = 2 * attend_bound(mag, top, b.max_kv).reshape(plain.shape)
+    bad = qs.copy()
+    bad[::2, 1] = np.nan
+    got, want = run(pool, bad), plain.copy()
+    want[::2, 1] = np.nan
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    assert (np.abs(got - want) <= twice)[~np.isnan(want)].all()
+    rows = {r: (s, p) for r, s, p in b.row_positions()}
+    for name in ("ks", "vs"):
+        t = 33  # of sequence 0, KV head 1: the heads of the upper half
+        keep = getattr(b, name).copy()
+        getattr(b, name)[b.tables[0, t // page], t % page, 1] = np.nan
+        got, want = run(on_device(b)[0], qs), plain.copy()
+        sees = [r for r, (s, p) in rows.items() if s == 0 and p >= t]
+        want[sees, heads // 2:] = np.nan
+        same = np.isnan(got) == np.isnan(want)
+        assert same.all(), np.argwhere(~same)[:4].tolist()
+        assert (np.abs(got - want) <= twice)[~np.isnan(want)].all()
+        getattr(b, name)[:] = keep
+
+
 def test_attention_strided(cuda):
     """Query and result rows inside wider ones."""
     b = Batch([(5, 60), (1, 700), (50, 0)], 2, 32, seed=4)
