@@ -257,7 +257,10 @@ int q3_argmax_logits(const q3_view *logits, int32_t *out_id, void *stream);
  * row_start[n_seq] on are left as they are.  What the arrays may hold wrongly is
  * clamped: a sequence's rows to max_rows, kv_len to [0, max_kv]; a page id
  * outside the pool is a page whose keys are never attended to or written.
- * row_start must not decrease. */
+ * row_start must not decrease.  At most 2^21 rows, 512 heads and max_kv 2^30
+ * (Q3_ERR_RANGE / Q3_ERR_ARG), and no more work than one launch's grid holds
+ * (Q3_ERR_HIP).  The same call gives the same bits; a row's last bits may hang on
+ * what else the batch holds. */
 typedef struct q3_seqs {
   const int32_t *row_start; /* device [n_seq + 1]                            */
   const int32_t *kv_len;    /* device [n_seq]: cached tokens, new ones included */

@@ -306,6 +306,7 @@ hipError_t launch_page_bounds(const PageBoundsArgs &a, hipStream_t s) {
   if (a.seqs.rows == 0 || a.seqs.n_seq == 0) return hipSuccess;
   const int pt = a.pool.page_tokens;
   const int per = (min(a.seqs.max_rows, a.seqs.max_kv) + pt - 2) / pt + 1;  // pages that max_rows tokens can lie in
+  if (static_cast<int64_t>(per) * a.kv_heads * a.seqs.n_seq > INT32_MAX / 256) return hipErrorInvalidValue;
   hipLaunchKernelGGL(page_bounds_kernel, dim3(static_cast<unsigned>(per * a.kv_heads), a.seqs.n_seq), dim3(256), 0, s, a, per);
   return hipGetLastError();
 }

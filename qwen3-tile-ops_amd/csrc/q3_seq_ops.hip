@@ -24,7 +24,7 @@ bool aligned(const void *p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p)
 // The pool and the sequences of a call over `rows` rows.
 int seq_common(const q3_paged_kv *kv, const q3_seqs *q, uint32_t rows, int kv_heads, q3::Pool &p, q3::Seqs &s) {
   if (!kv || !kv->k || !kv->v || !kv->ks || !kv->vs || !q) return Q3_ERR_ARG;
-  if (kv_heads <= 0) return Q3_ERR_ARG;
+  if (kv_heads <= 0 || kv_heads > kMaxHeads) return Q3_ERR_ARG;
   if (kv->page_tokens == 0 || kv->page_tokens % 32 != 0) return Q3_ERR_UNSUPPORTED;
   const uint64_t pt = kv->page_tokens;
   if (kv->page_bytes < pt * kv->row_bytes || kv->scale_page_bytes < pt * kv->scale_row_bytes) return Q3_ERR_VIEW;
@@ -60,7 +60,7 @@ int check_out(const q3_view *out, const q3_view *o8, const q3_view *os, uint32_t
   if (!out == !o8 || !o8 != !os) return Q3_ERR_ARG;  // one of the two forms
   if (out) {
     Q3_TRY(check_view(out, Q3_DT_F32));
-    if (out->rows < rows || out->cols < cols) return Q3_ERR_VIEW;
+    if (out->rows < rows || out->cols < cols || !aligned(out->data, 4)) return Q3_ERR_VIEW;
     a.out = static_cast<float *>(out->data);
     a.ldo = ld(out);
   } else {
@@ -97,7 +97,7 @@ int attn_common(const q3_view *q8, const q3_view *q_scale, const q3_paged_kv *kv
 int check_ids(const q3_view *ids, uint32_t rows, int kv_heads, uint32_t n_sel) {
   Q3_TRY(check_view(ids, Q3_DT_I32));
   if (n_sel == 0 || n_sel > 65536) return Q3_ERR_RANGE;
-  if (ids->rows < rows || ids->cols < static_cast<uint64_t>(kv_heads) * n_sel) return Q3_ERR_VIEW;
+  if (ids->rows < rows || ids->cols < static_cast<uint64_t>(kv_heads) * n_sel || !aligned(ids->data, 4)) return Q3_ERR_VIEW;
   return Q3_OK;
 }
 

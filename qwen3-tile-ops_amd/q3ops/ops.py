@@ -189,6 +189,9 @@ def argmax_logits(logits, out_id, stream=None):
 # ---- batches of sequences over one paged cache ------------------------------
 
 
+MAX_ROWS = 1 << 21  # of a call on a batch of sequences
+
+
 def kv_pool(k: torch.Tensor, v: torch.Tensor, ks: torch.Tensor, vs: torch.Tensor) -> PagedKV:
     """The pool of K/V pages that the batch operators below share: k/v
     [pages, page_tokens, kv_heads * 128] int8, ks/vs [pages, page_tokens,
@@ -231,6 +234,7 @@ def sequences(pool: PagedKV, tables, row_start, kv_len, max_rows: int, max_kv: i
     s = Seqs(row_start.data_ptr(), kv_len.data_ptr(), tables.data_ptr(), n_seq, tables.shape[1],
              pool.n_pages, max_rows, max_kv)
     s._keep = (tables, row_start, kv_len)
+    s.index = pool.device.index
     return s
 
 
@@ -263,10 +267,13 @@ def _views(pool: PagedKV, tensors) -> list:
     return out
 
 
-def _launch_stream(pool: PagedKV, stream) -> int:
+def _launch_stream(pool: PagedKV, seqs: Seqs, stream) -> int:
     """The stream of a call on the pool's device, which has to be the current one
-    (kernels launch there)."""
+    (kernels launch there).  Sequences of another pool do as well (a layer's), if
+    their tables' pages are this one's too."""
     dev = pool.device
+    if seqs.n_pages > pool.n_pages or seqs.index != dev.index:
+        raise ValueError(f"sequences over {seqs.n_pages} pages on cuda:{seqs.index} for a pool of {pool.n_pages} on {dev}")
     if dev.index != torch.cuda.current_device():
         raise ValueError(f"the pool is on {dev}, the current device is cuda:{torch.cuda.current_device()}")
     if stream is None:
@@ -286,16 +293,16 @@ def rope_append_paged(q, k, v, pool: PagedKV, seqs: Seqs, q8=None, qs=None, nwq=
     check(lib().q3_rope_append_paged(vq, vk, vv, vnq, vnk, inv_hd, vc, vs, rot_dim if cos is not None else 0,
                                      int(interleaved), v8, vqs, byref(pool), byref(seqs),
                                      0 if q is None else q.shape[1] // 128, pool.kv_heads,
-                                     _launch_stream(pool, stream)), "rope_append_paged")
+                                     _launch_stream(pool, seqs, stream)), "rope_append_paged")
 
 
 def page_bounds(pool: PagedKV, seqs: Seqs, bounds, bscale, rows: int | None = None, stream=None):
     """q3_page_bounds: channel bounds (int8 [pages * kv_heads, 256], least then
     largest; f32 [pages, kv_heads]) of the pages that the sequences' new rows lie
-    in (rows: the call's row count, n_seq * max_rows if not given)."""
-    rows = seqs.n_seq * seqs.max_rows if rows is None else rows
+    in (rows: the call's row count; without it row_start is taken as it is)."""
+    rows = MAX_ROWS if rows is None else rows
     vb, vs = _views(pool, (bounds, bscale))
-    check(lib().q3_page_bounds(byref(pool), byref(seqs), rows, pool.kv_heads, vb, vs, _launch_stream(pool, stream)),
+    check(lib().q3_page_bounds(byref(pool), byref(seqs), rows, pool.kv_heads, vb, vs, _launch_stream(pool, seqs, stream)),
           "page_bounds")
 
 
@@ -331,7 +338,7 @@ def attention_varlen_paged(q8, q_scale, pool: PagedKV, seqs: Seqs, out=None, o8=
     workspace: a device tensor of seqs_workspace_bytes, needed on a stream that
     is not the current one; otherwise one is allocated."""
     vq, vs, vo, v8, vos = _views(pool, (q8, q_scale, out, o8, os))
-    st = _launch_stream(pool, stream)
+    st = _launch_stream(pool, seqs, stream)
     keep, ws, n = _workspace_on(workspace, stream, pool, seqs, q8, 0)
     check(lib().q3_attention_varlen_paged(vq, vs, byref(pool), byref(seqs), vo, v8, vos, q8.shape[1] // 128,
                                           pool.kv_heads, 128, int(causal), qk_scale, ws, n, st),
@@ -342,7 +349,7 @@ def select_pages(q8, q_scale, pool: PagedKV, seqs: Seqs, bounds, bscale, ids, n_
     """q3_select_pages: the n_sel pages of each row and KV head with the largest
     bounds of a score, into ids (int32 [rows, kv_heads * n_sel])."""
     vq, vs, vb, vbs, vi = _views(pool, (q8, q_scale, bounds, bscale, ids))
-    st = _launch_stream(pool, stream)
+    st = _launch_stream(pool, seqs, stream)
     keep, ws, n = _workspace_on(workspace, stream, pool, seqs, q8, n_sel)
     check(lib().q3_select_pages(vq, vs, byref(pool), byref(seqs), vb, vbs, vi, n_sel, q8.shape[1] // 128,
                                 pool.kv_heads, ws, n, st), "select_pages")
@@ -353,7 +360,7 @@ def attention_pages(q8, q_scale, pool: PagedKV, seqs: Seqs, ids, n_sel, out=None
     """q3_attention_pages: attention_varlen_paged over the keys of each row's
     listed pages (select_pages' ids, or the caller's own)."""
     vq, vs, vi, vo, v8, vos = _views(pool, (q8, q_scale, ids, out, o8, os))
-    st = _launch_stream(pool, stream)
+    st = _launch_stream(pool, seqs, stream)
     keep, ws, n = _workspace_on(workspace, stream, pool, seqs, q8, n_sel)
     check(lib().q3_attention_pages(vq, vs, byref(pool), byref(seqs), vi, n_sel, vo, v8, vos, q8.shape[1] // 128,
                                    pool.kv_heads, 128, qk_scale, ws, n, st), "attention_pages")

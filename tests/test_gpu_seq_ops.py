@@ -447,8 +447,9 @@ def test_append_equals_norm_rope_quant_heads(cuda):
     cos, sin = (dev(t) for t in rope_tables(b.max_kv))
     pool, seqs = on_device(b)
     q8, qs = torch.empty((60, 2048), dtype=torch.int8, device="cuda"), torch.empty((60, 16), device="cuda")
-    ops.rope_append_paged(x[:, :2048], x[:, 2048:3072], x[:, 3072:], pool, seqs, q8, qs, nwq=w, nwk=w, inv_hd=1 / 128, cos=cos, sin=sin)
-    for heads, rows, got, gs in ((16, x[:, :2048], q8, qs), (8, x[:, 2048:3072], None, None)):
+    q, k, v = x.split([2048, 1024, 1024], 1)
+    ops.rope_append_paged(q, k, v, pool, seqs, q8, qs, nwq=w, nwk=w, inv_hd=1 / 128, cos=cos, sin=sin)
+    for heads, rows, got, gs in ((16, q, q8, qs), (8, k, None, None)):
         r8, rs = torch.empty((60, heads * 128), dtype=torch.int8, device="cuda"), torch.empty((60, heads), device="cuda")
         ops.norm_rope_quant_heads(rows, w, cos[77:], sin[77:], r8, rs, heads, 1 / 128)
         if got is None:
@@ -691,6 +692,83 @@ def test_captured_and_replayed(cuda, rows, context):
                 assert torch.equal(got, want), lens
 
 
+@pytest.mark.parametrize("rows", [1, 70])
+def test_append_captured_and_replayed(cuda, rows):
+    """Rows appended, and their pages bounded, by a graph on other lengths, rows and
+    inputs, step after step, beside eager calls on a pool of the same contents."""
+    heads, kvh, page, n = 4, 2, 32, 3
+    b = Batch([(rows, 400)] * n, kvh, page, seed=31)
+    b.ks[:], b.vs[:] = np.nan_to_num(b.ks), np.nan_to_num(b.vs)
+    pools = [on_device(b)[0] for _ in range(2)]
+    total = n * rows
+    start, kv_len = dev(b.start), dev(b.kv_len)
+    seqs = ops.sequences(pools[0], dev(b.tables), start, kv_len, rows, b.max_kv)
+    cos, sin = (dev(t) for t in rope_tables(b.max_kv))
+    x = [torch.randn((total, h * 128), device="cuda") for h in (heads, kvh, kvh)]
+    res = [(torch.zeros((total, heads * 128), dtype=torch.int8, device="cuda"), torch.zeros((total, heads), device="cuda"),
+            torch.zeros((b.n_pages * kvh, 256), dtype=torch.int8, device="cuda"), torch.zeros((b.n_pages, kvh), device="cuda")) for _ in pools]
+
+    def step(i):
+        ops.rope_append_paged(*x, pools[i], seqs, *res[i][:2], cos=cos, sin=sin)
+        ops.page_bounds(pools[i], seqs, *res[i][2:], total)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        step(0)
+    for lens in ([(rows, 300)] * n, [(rows, 0), (0, 31), (rows, 90)], [(1, 31), (rows, 331), (1, 0)], [(rows, 400)] * n):
+        kv_len.copy_(torch.tensor([r + c for r, c in lens], dtype=torch.int32))
+        start.copy_(torch.tensor(np.cumsum([0] + [r for r, _ in lens]).astype(np.int32)))
+        for t in x:
+            t.normal_()
+        g.replay()
+        step(1)
+        torch.cuda.synchronize()
+        for got, want in zip((*pools[0]._keep, *res[0]), (*pools[1]._keep, *res[1])):
+            assert torch.equal(got, want), lens
+
+
+def test_selection_on_two_streams(cuda):
+    """The selection and the attention over its pages on two streams at once, each with
+    its own workspace, which all their calls share in turn."""
+    heads, kvh, n_sel = 8, 4, 5
+    b = Batch([(1, 3000), (20, 1000)], kvh, 32, seed=41, smooth=True)
+    pool, seqs = on_device(b)
+    hb, hs, _ = bounds_on_host(b)
+    bounds, scale = dev(hb), dev(hs)
+    q8, qs = (dev(t) for t in queries(b.rng, b.rows, heads))
+    n = ops.seqs_workspace_bytes(pool, seqs, b.rows, heads, n_sel)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    sets = [[(torch.zeros((b.rows, kvh * n_sel), dtype=torch.int32, device="cuda"), torch.zeros((b.rows, heads * 128), device="cuda"))
+             for _ in range(4)] for _ in range(3)]
+    ws = [torch.empty(n, dtype=torch.uint8, device="cuda") for _ in sets]
+    torch.cuda.synchronize()
+    for i in range(4):
+        for st, w, o in zip([*streams, None], ws, sets):
+            ops.select_pages(q8, qs, pool, seqs, bounds, scale, o[i][0], n_sel, workspace=w, stream=st)
+            ops.attention_pages(q8, qs, pool, seqs, o[i][0], n_sel, o[i][1], qk_scale=QK, workspace=w, stream=st)
+    torch.cuda.synchronize()
+    want = seqref.select(b, q8.cpu().numpy(), qs.cpu().numpy(), heads, hb, hs, n_sel)
+    assert np.array_equal(sets[2][0][0].cpu().numpy(), want)
+    for o in sets:
+        for ids, out in o:
+            assert torch.equal(ids, sets[2][0][0]) and torch.equal(out, sets[2][0][1])
+
+
+def test_page_bounds_rows_given_or_not(cuda):
+    """Row starts that do not begin at 0, with and without the call's row count."""
+    b = Batch([(1, 40), (33, 31)], 2, 32, before=50)
+    pool, seqs = on_device(b)
+    want, wscale, touched = bounds_on_host(b)
+    for rows in (None, b.rows):
+        bounds = torch.full((b.n_pages * 2, 256), 99, dtype=torch.int8, device="cuda")
+        scale = torch.full(wscale.shape, 7.5, device="cuda")
+        ops.page_bounds(pool, seqs, bounds, scale, rows)
+        assert bits_equal(bounds.cpu().numpy().reshape(b.n_pages, -1)[touched], want.reshape(b.n_pages, -1)[touched])
+        assert bits_equal(scale.cpu().numpy()[touched], wscale[touched])
+
+
 def test_two_streams(cuda):
     """Calls of one pool on two streams at once, each with its own workspace."""
     b = Batch([(1, 3000), (40, 100)], 2, 32, seed=40)
@@ -742,3 +820,21 @@ def test_refused_on_the_device(cuda):
         ops.kv_pool(*(t[:, :, ::2] for t in pool._keep))
     with pytest.raises(TypeError):
         ops.sequences(pool, seqs._keep[0].int(), *seqs._keep[1:], 1, 41)
+    fewer = ops.kv_pool(*(t[:-1] for t in pool._keep))  # not all pages that the tables may name
+    with pytest.raises(ValueError):
+        ops.attention_varlen_paged(q8, qs, fewer, seqs, out)
+    with pytest.raises(ValueError):
+        ops.rope_append_paged(None, out[:, :256], out[:, :256], fewer, seqs)
+    with pytest.raises(ops.Q3Error):
+        ops.attention_varlen_paged(q8, qs, pool, ops.sequences(pool, *seqs._keep, -1, 41), out)
+    with pytest.raises(ops.Q3Error):
+        ops.attention_varlen_paged(q8, qs, pool, ops.sequences(pool, *seqs._keep, 1, 65), out)
+    long = Batch([(1, 3000)], 2, 32)
+    pool, seqs = on_device(long)
+    with pytest.raises(ValueError):  # whose workspace?
+        ops.attention_varlen_paged(q8, qs, pool, seqs, out, stream=torch.cuda.Stream())
+    for ws in (torch.empty(64, dtype=torch.uint8, device="cuda"), torch.empty(1 << 20, dtype=torch.uint8, device="cuda")[4:]):
+        with pytest.raises(ops.Q3Error):
+            ops.attention_varlen_paged(q8, qs, pool, seqs, out, workspace=ws)
+    with pytest.raises(ValueError):
+        ops.attention_varlen_paged(q8, qs, pool, seqs, out, workspace=torch.empty(1 << 20, dtype=torch.uint8))

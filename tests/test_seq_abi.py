@@ -108,6 +108,7 @@ def test_results_refused(lib):
                    (dict(out=None, o8=V(ROWS, H * 128, DT_I8)), ARG), (dict(out=None, os=V(ROWS, H, DT_F32)), ARG),
                    (dict(out=V(ROWS - 1, H * 128, DT_F32)), VIEW), (dict(out=V(ROWS, H * 128 - 1, DT_F32)), VIEW),
                    (dict(out=V(ROWS, H * 128, DT_I8)), DTYPE), (dict(hd=64), UNSUPPORTED),
+                   (dict(out=C.byref(_lib.View(_ADDR + 2, H * 512, 4, ROWS, H * 128, DT_F32))), VIEW),
                    (dict(out=None, o8=V(ROWS, H * 128, DT_I8), os=V(ROWS, H - 1, DT_F32)), VIEW)]:
         assert attend(lib, **kw) == rc, kw
     assert pages(lib, hd=64) == UNSUPPORTED
@@ -116,8 +117,15 @@ def test_results_refused(lib):
 @pytest.mark.parametrize("call", [pages, select])
 def test_ids_refused(lib, call):
     for kw, rc in [(dict(ids=None), ARG), (dict(ids=V(ROWS, KV * 3, DT_F32)), DTYPE), (dict(ids=V(ROWS, KV * 3 - 1, DT_I32)), VIEW),
-                   (dict(ids=V(ROWS - 1, KV * 3, DT_I32)), VIEW), (dict(n_sel=0), RANGE), (dict(n_sel=65537), RANGE), (dict(n_sel=4), VIEW)]:
+                   (dict(ids=V(ROWS - 1, KV * 3, DT_I32)), VIEW), (dict(n_sel=0), RANGE), (dict(n_sel=65537), RANGE), (dict(n_sel=4), VIEW),
+                   (dict(ids=C.byref(_lib.View(_ADDR + 1, KV * 12, 4, ROWS, KV * 3, DT_I32))), VIEW)]:
         assert call(lib, **kw) == rc, kw
+
+
+def test_heads_refused(lib):
+    wide = pool(row_bytes=513 * 128, page_bytes=32 * 513 * 128, scale_row_bytes=513 * 4, scale_page_bytes=32 * 513 * 4)
+    assert bounds(lib, kv=wide, kvh=513, b=V(16 * 513, 256, DT_I8), bs=V(16, 513, DT_F32)) == ARG
+    assert attend(lib, q8=V(ROWS, 513 * 128, DT_I8), qs=V(ROWS, 513, DT_F32), out=V(ROWS, 513 * 128, DT_F32), heads=513, kvh=513, kv=wide) == ARG
 
 
 @pytest.mark.parametrize("call", ["select", "bounds"])
