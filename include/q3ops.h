@@ -255,7 +255,8 @@ int q3_argmax_logits(const q3_view *logits, int32_t *out_id, void *stream);
  * by the kernels alone, so a call may be captured into a graph and replayed on
  * other lengths, within max_rows and max_kv.  Rows before row_start[0] and from
  * row_start[n_seq] on are left as they are.  What the arrays may hold wrongly is
- * clamped: a sequence's rows to max_rows, kv_len to [0, max_kv]; a page id
+ * clamped: a sequence's rows to max_rows, kv_len to [0, max_kv] (limits well
+ * above the lengths cost little time, but workspace); a page id
  * outside the pool is a page whose keys are never attended to or written.
  * row_start must not decrease.  At most 2^21 rows, 512 heads and max_kv 2^30
  * (Q3_ERR_RANGE / Q3_ERR_ARG), and no more work than one launch's grid holds

@@ -172,8 +172,14 @@ struct Partials {
   float *o;    // [slot][split][128]
   float2 *ml;  // [slot][split]
   int64_t slots;
-  int splits, span;  // keys of a split (listed pages: of the list's keys)
+  int splits, span;  // of a list's keys; a sequence's: split_span
 };
+
+// The keys of each of at most `splits` parts of a sequence: its length is known on the
+// device alone, and max_kv may be far above it.
+__device__ __forceinline__ int split_span(int keys, int splits, int least, int step) {
+  return max(least, ((keys + splits - 1) / splits + step - 1) / step * step);
+}
 
 __device__ __forceinline__ float exp2_from(float x, float base) { return __builtin_amdgcn_exp2f(x - base); }
 
@@ -198,7 +204,8 @@ constexpr int FEW_STAGES = 2;  // of V and the scales
 constexpr int FEW_V = 0, FEW_S = KB * HD, FEW_STAGE = KB * HD + 2 * KB * 4;
 constexpr int FEW_K = FEW_STAGES * FEW_STAGE, FEW_WAVE = FEW_K + KB * HD;  // bytes of a wave
 constexpr int FEW_ROW = HD + 4;  // floats of a column's row where the waves join
-constexpr int FEW_SPAN = 64 * KB * FEW_WAVES;  // keys of a split: a lane of each wave names one block
+constexpr int FEW_BLOCKS = 64 * FEW_WAVES;  // named at a time, one by a lane of each wave
+constexpr int FEW_STEP = KB * FEW_WAVES, FEW_LEAST = 256;  // keys of a split: a multiple, at least
 static_assert(FEW_WAVES * FEW_COLS * FEW_ROW * 4 <= FEW_WAVES * FEW_WAVE, "the join fits the stages");
 
 struct FewPlan {
@@ -239,7 +246,8 @@ __device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, F
 
   // this lane's column, and how many keys it sees
   const int c = tile * FEW_COLS + col;
-  int seq, row0, row, g, cols, sees;
+  int seq, row0, row, g, cols, sees, span = p.part.span;
+  bool whole = p.part.splits == 1;
   if constexpr (LIST) {
     row0 = row = unit / p.tiles, g = c, cols = group_heads;
     const SeqRow at = row_at(a.seqs, row);
@@ -251,6 +259,8 @@ __device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, F
     const SeqSpan sp = seq_span(a.seqs, seq);
     cols = sp.n * group_heads;
     if (cols > p.most || tile * FEW_COLS >= cols) return;
+    span = split_span(sp.kv, p.part.splits, FEW_LEAST, FEW_STEP);
+    whole = sp.kv <= span;
     row0 = sp.r0, row = sp.r0 + c / group_heads, g = c % group_heads;
     sees = a.causal ? max(sp.pos(row) + 1, 0) : sp.kv;
   }
@@ -260,32 +270,8 @@ __device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, F
   const int vmin = __builtin_amdgcn_readlane(sees, 0);
   const int vmax = __builtin_amdgcn_readlane(sees, min(cols - tile * FEW_COLS, FEW_COLS) - 1);
 
-  // Lane i names the wave's block i: its page, its place there, its first key.
-  const int span_blocks = p.part.span / KB;
+  const int span_blocks = span / KB;
   const int first = split * span_blocks;  // blocks from 0, or of the list
-  int bpage = -1, bkey = 0, bt = 0;
-  {
-    const int b = first + lane * FEW_WAVES + wave;
-    if (lane * FEW_WAVES + wave < span_blocks) {
-      const int per_page = pt / KB;
-      const int nth = b / per_page;
-      bt = (b % per_page) * KB;
-      if constexpr (LIST) {
-        if (nth < a.n_sel) {
-          const int id = a.ids[row0 * a.ld_ids + static_cast<int64_t>(kvh) * a.n_sel + nth];
-          // a page of the row's: its first key is seen, so it lies in the table
-          if (vmax > 0 && id >= 0 && id <= (vmax - 1) / pt) {
-            bkey = id * pt + bt;
-            if (bkey < vmax) bpage = seq_page(a.seqs, a.pool, seq, id);
-          }
-        }
-      } else {
-        bkey = b * KB;
-        if (bkey < vmax) bpage = seq_page(a.seqs, a.pool, seq, nth);
-      }
-    }
-  }
-  uint64_t todo = __ballot(bpage >= 0);
   if constexpr (!LIST) {
     if (split > 0 && first * KB >= vmax) return;  // behind the tile's last key: nobody joins this split
   }
@@ -306,8 +292,7 @@ __device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, F
   const int64_t lane_v = r8 * a.pool.row_bytes + 16 * (ch ^ (r8 & 3));
   const int64_t lane_v4 = r8 * a.pool.row_bytes + 16 * (ch ^ ((r8 & 3) | 4));
 
-  auto issue = [&](int i, uint8_t *st) {
-    const int page = __builtin_amdgcn_readlane(bpage, i), t0 = __builtin_amdgcn_readlane(bt, i);
+  auto issue = [&](int page, int t0, uint8_t *st) {
     const int64_t at = page * a.pool.page_bytes + t0 * a.pool.row_bytes + kvh * HD;
     const int8_t *k = a.pool.k + at, *v = a.pool.v + at;
     const int64_t eight = 8 * a.pool.row_bytes;
@@ -324,87 +309,112 @@ __device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, F
 #pragma unroll
   for (int t = 0; t < 8; ++t) o[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 
-  int ahead = -1;  // the block in flight
-  if (todo) {
-    ahead = __builtin_ctzll(todo);
-    todo &= todo - 1;
-    issue(ahead, stages);
-  }
   int buf = 0;
-  while (ahead >= 0) {
-    const int now = ahead;
-    uint8_t *const st = stages + buf * FEW_STAGE;
-    buf ^= 1;
-    wait_copies<0>();
-
-    // S^T of two 16-key tiles: lane holds keys 4 quarter + i of each
-    float x[8], vsc[8];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const uint8_t *kr = stages + FEW_K + (t * 16 + col) * HD;
-      const v4i_d k0 = *reinterpret_cast<const v4i_d *>(kr + 16 * (quarter ^ (col & 7)));
-      const v4i_d k1 = *reinterpret_cast<const v4i_d *>(kr + 16 * ((4 + quarter) ^ (col & 7)));
-      v4i_d s = {0, 0, 0, 0};
-      s = __builtin_amdgcn_mfma_i32_16x16x64_i8(k0, qf[0], s, 0, 0, 0);
-      s = __builtin_amdgcn_mfma_i32_16x16x64_i8(k1, qf[1], s, 0, 0, 0);
-      const v4f ks = *reinterpret_cast<const v4f *>(st + FEW_S + 4 * (t * 16 + 4 * quarter));
-      const v4f vs = *reinterpret_cast<const v4f *>(st + FEW_S + 4 * (KB + t * 16 + 4 * quarter));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[4 * t + i] = static_cast<float>(s[i]) * ks[i] * cs;
-        vsc[4 * t + i] = vs[i];
+  for (int part = 0; part < span_blocks; part += FEW_BLOCKS) {
+    if constexpr (!LIST) {
+      if ((first + part) * KB >= vmax) break;
+    }
+    // Lane i names the wave's block i of this part: its page, its place there, its first key.
+    int bpage = -1, bkey = 0, bt = 0;
+    const int nth_block = part + lane * FEW_WAVES + wave;
+    if (nth_block < span_blocks) {
+      const int per_page = pt / KB;
+      const int b = first + nth_block;
+      const int nth = b / per_page;
+      bt = (b % per_page) * KB;
+      if constexpr (LIST) {
+        if (nth < a.n_sel) {
+          const int id = a.ids[row0 * a.ld_ids + static_cast<int64_t>(kvh) * a.n_sel + nth];
+          // a page of the row's: its first key is seen, so it lies in the table
+          if (vmax > 0 && id >= 0 && id <= (vmax - 1) / pt) {
+            bkey = id * pt + bt;
+            if (bkey < vmax) bpage = seq_page(a.seqs, a.pool, seq, id);
+          }
+        }
+      } else {
+        bkey = b * KB;
+        if (bkey < vmax) bpage = seq_page(a.seqs, a.pool, seq, nth);
       }
     }
-    ahead = -1;
-    if (todo) {
-      ahead = __builtin_ctzll(todo);
+    uint64_t todo = __ballot(bpage >= 0);
+    auto next = [&]() {  // starts the next block's copies; -1: there is none
+      if (todo == 0) return -1;
+      const int i = __builtin_ctzll(todo);
       todo &= todo - 1;
       // the reads of this block's K, and of the block before, have been used
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      issue(ahead, stages + buf * FEW_STAGE);
-    }
-    const int key0 = __builtin_amdgcn_readlane(bkey, now);
-    const bool edge = key0 + KB > vmin;  // some column does not see the whole block
-    if (edge) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (key0 + (j >> 2) * 16 + 4 * quarter + (j & 3) >= sees) x[j] = -INFINITY;
-    }
-    float mb = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-    mb = fmaxf(col_max(mb), m);
-    const float base = mb == -INFINITY ? 0.0f : mb;
-    if (__ballot(mb != m)) {
-      const float alpha = exp2_from(m, base);
-      l *= alpha;
-#pragma unroll
-      for (int t = 0; t < 8; ++t) o[t] *= alpha;
-      m = mb;
-    }
-    float pv[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float e = exp2_from(x[j], base);
-      l += e;
-      pv[j] = e * vsc[j];
-    }
-    if (edge) {  // a scale behind the sequence's end may be anything
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (key0 + (j >> 2) * 16 + 4 * quarter + (j & 3) >= sees) pv[j] = 0.0f;
-    }
-    const Bf16x3 pb = split_bf16(pv);
+      issue(__builtin_amdgcn_readlane(bpage, i), __builtin_amdgcn_readlane(bt, i), stages + buf * FEW_STAGE);
+      return i;
+    };
+    int ahead = next();  // the block in flight
+    while (ahead >= 0) {
+      const int now = ahead;
+      uint8_t *const st = stages + buf * FEW_STAGE;
+      buf ^= 1;
+      wait_copies<0>();
 
-    // the key that this lane's address names for the transposing read: the 16
-    // lanes of a row take 8 keys, two halves of a 16-byte chunk each
-    const int rj = (lane & 15) >> 1;
-    const int key = 4 * quarter + (rj & 3) + 16 * (rj >> 2);
-    const uint8_t *vq = st + FEW_V + key * HD + 8 * (lane & 1);
+      // S^T of two 16-key tiles: lane holds keys 4 quarter + i of each
+      float x[8], vsc[8];
 #pragma unroll
-    for (int t = 0; t < 8; ++t) {
-      const v2i_d w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(reinterpret_cast<lds_v2i_ptr_d>(to_lds(vq + 16 * (t ^ vswz(key)))));
-      const v8bf vt = int8_bf16(w);
+      for (int t = 0; t < 2; ++t) {
+        const uint8_t *kr = stages + FEW_K + (t * 16 + col) * HD;
+        const v4i_d k0 = *reinterpret_cast<const v4i_d *>(kr + 16 * (quarter ^ (col & 7)));
+        const v4i_d k1 = *reinterpret_cast<const v4i_d *>(kr + 16 * ((4 + quarter) ^ (col & 7)));
+        v4i_d s = {0, 0, 0, 0};
+        s = __builtin_amdgcn_mfma_i32_16x16x64_i8(k0, qf[0], s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_i32_16x16x64_i8(k1, qf[1], s, 0, 0, 0);
+        const v4f ks = *reinterpret_cast<const v4f *>(st + FEW_S + 4 * (t * 16 + 4 * quarter));
+        const v4f vs = *reinterpret_cast<const v4f *>(st + FEW_S + 4 * (KB + t * 16 + 4 * quarter));
 #pragma unroll
-      for (int u = 0; u < 3; ++u) o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt, pb.part[u], o[t], 0, 0, 0);
+        for (int i = 0; i < 4; ++i) {
+          x[4 * t + i] = static_cast<float>(s[i]) * ks[i] * cs;
+          vsc[4 * t + i] = vs[i];
+        }
+      }
+      ahead = next();
+      const int key0 = __builtin_amdgcn_readlane(bkey, now);
+      const bool edge = key0 + KB > vmin;  // some column does not see the whole block
+      if (edge) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (key0 + (j >> 2) * 16 + 4 * quarter + (j & 3) >= sees) x[j] = -INFINITY;
+      }
+      float mb = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+      mb = fmaxf(col_max(mb), m);
+      const float base = mb == -INFINITY ? 0.0f : mb;
+      if (__ballot(mb != m)) {
+        const float alpha = exp2_from(m, base);
+        l *= alpha;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) o[t] *= alpha;
+        m = mb;
+      }
+      float pv[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float e = exp2_from(x[j], base);
+        l += e;
+        pv[j] = e * vsc[j];
+      }
+      if (edge) {  // a scale behind the sequence's end may be anything
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (key0 + (j >> 2) * 16 + 4 * quarter + (j & 3) >= sees) pv[j] = 0.0f;
+      }
+      const Bf16x3 pb = split_bf16(pv);
+
+      // the key that this lane's address names for the transposing read: the 16
+      // lanes of a row take 8 keys, two halves of a 16-byte chunk each
+      const int rj = (lane & 15) >> 1;
+      const int key = 4 * quarter + (rj & 3) + 16 * (rj >> 2);
+      const uint8_t *vq = st + FEW_V + key * HD + 8 * (lane & 1);
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        const v2i_d w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(reinterpret_cast<lds_v2i_ptr_d>(to_lds(vq + 16 * (t ^ vswz(key)))));
+        const v8bf vt = int8_bf16(w);
+#pragma unroll
+        for (int u = 0; u < 3; ++u) o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt, pb.part[u], o[t], 0, 0, 0);
+      }
     }
   }
 
@@ -436,7 +446,7 @@ __device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, F
   // (no key at all: zeros; scores that are all NaN leave a sum of NaN)
   const int jrow = LIST ? row0 : row0 + cc / group_heads;
   const int jhead = kvh * group_heads + (LIST ? cc : cc % group_heads);
-  if (p.part.splits == 1) {
+  if (whole) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) r[i] = sum == 0.0f ? 0.0f : r[i] / sum;
     store_row8(a, jrow, jhead, d0, r);
@@ -490,7 +500,8 @@ constexpr int WIDE_SLOTS = 512;    // workgroups at a time, two a CU
 constexpr int WIDE_KEYS = KB;      // of a step
 constexpr int WIDE_WAVES = 4;
 constexpr int WIDE_DEPTH = 4;      // steps whose K and V lie in LDS or on their way
-constexpr int WIDE_SPAN = 8192;   // keys of a split: its blocks' places lie in LDS
+constexpr int WIDE_RING = 256;     // steps whose blocks' places lie in LDS
+constexpr int WIDE_LEAST = 512;    // keys of a split
 constexpr int WIDE_OROW = 32 + 4;  // floats of a column's row where the results turn
 constexpr float WIDE_ROOM = 4.0f;  // P may reach 2^4 of its reference before O is scaled down
 
@@ -517,8 +528,7 @@ __device__ __forceinline__ int wave_max(int x) {
 
 // The sequence of the unit-th tile of 128 columns, -1 behind the last, and which of
 // its tiles it is: tiles are counted 64 sequences at a time, one per lane.  *span:
-// the keys of a split, the plan's or more: with splits as long as the work for each
-// of WIDE_SLOTS workgroups (the plan knows no sequence's length, only limits).
+// the keys of a split, no fewer than the work for each of WIDE_SLOTS workgroups.
 __device__ __forceinline__ int wide_tile(const SeqAttnArgs &a, const WidePlan &p, int unit, int *nth, int *span, SeqSpan *seq) {
   const int lane = threadIdx.x & 63;
   const int group_heads = a.heads / a.kv_heads;
@@ -558,8 +568,8 @@ __device__ __forceinline__ int wide_tile(const SeqAttnArgs &a, const WidePlan &p
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) steps += __uint_as_float(lane_xor_m(__float_as_uint(steps), d));
   const float each = steps * static_cast<float>(a.kv_heads) / WIDE_SLOTS;
-  const int even = static_cast<int>(fminf(each, static_cast<float>(WIDE_SPAN / WIDE_KEYS))) * WIDE_KEYS;
-  *span = __builtin_amdgcn_readfirstlane(max(p.part.span, even));
+  const int even = static_cast<int>(fminf(each, static_cast<float>(1 << 25))) * WIDE_KEYS;
+  *span = __builtin_amdgcn_readfirstlane(max(split_span(found < 0 ? 0 : seq->kv, p.part.splits, WIDE_LEAST, WIDE_KEYS), even));
   return found;
 }
 
@@ -578,7 +588,7 @@ struct WideLds {
   static_assert(sizeof(Stages) >= 4 * 32 * WIDE_OROW * 4, "the results fit where the steps were");
   __align__(16) Stages st;
   __align__(16) float sc[2 * WIDE_DEPTH][2 * WIDE_KEYS];  // of a step's block ks, then vs
-  int2 block[WIDE_SPAN / KB];                             // page, first token
+  int2 block[WIDE_RING];                                  // of step % WIDE_RING: page, first token
   uint32_t range[2];
 };
 
@@ -608,8 +618,7 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
   const int tile_min = a.causal ? max(sp.pos(first_row) + 1, 0) : sp.kv;
   const int tile_max = tile_keys(a, sp, col0, cols);
   if (split > 0 && split * static_cast<int64_t>(span) >= tile_max) return;
-  const int first = split * span;
-  const int end = min(tile_max, first + span);
+  const int first = split * span, end = min(tile_max, first + span);
   const int steps = (end - first + WIDE_KEYS - 1) / WIDE_KEYS;  // <= 0: none
 
   v4i_d qf[4];
@@ -623,23 +632,17 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
     cs = a.qs[row * a.ldqs + head * a.qs_col] * a.qk_scale * kLog2e;
   }
 
-  // the split's blocks
-  if (tid < 2) lds.range[tid] = tid == 0 ? 0u : 0x7f800000u;
-  bool hole = false;
-  for (int i = tid; i < steps; i += 256) {
-    const int key = first + i * KB;
-    const int2 at = make_int2(seq_page(a.seqs, a.pool, seq, key / pt), key % pt);
-    hole |= at.x < 0;
-    lds.block[i] = at;
-  }
-  const bool missing = __syncthreads_or(hole);
+  auto place = [&](int step) {
+    const int key = first + step * WIDE_KEYS;
+    return make_int2(seq_page(a.seqs, a.pool, seq, key / pt), key % pt);
+  };
 
   // Copies: wave w takes keys 8 w .. 8 w + 7 of a step (of block w / 4).
   const int r8 = lane >> 3, ch = lane & 7;
   const int64_t my_row = (8 * wave + r8) * a.pool.row_bytes + kvh * HD;
   const int64_t lane_k = my_row + 16 * (ch ^ r8), lane_v = my_row + 16 * (ch ^ vswz_wide(8 * wave + r8));
   auto copy = [&](int step) {
-    int2 at = lds.block[step];
+    int2 at = lds.block[step % WIDE_RING];
     at = make_int2(__builtin_amdgcn_readfirstlane(at.x), __builtin_amdgcn_readfirstlane(at.y));
     if (at.x < 0) return;
     const int64_t bytes = at.x * a.pool.page_bytes + at.y * a.pool.row_bytes;
@@ -649,35 +652,50 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
       lds_copy4((half ? a.pool.vs : a.pool.ks) + at.x * a.pool.spage + (at.y + n32) * a.pool.srow + kvh, lds.sc[step % (2 * WIDE_DEPTH)]);
   };
 
-  // the first steps' copies, and beside them the range of the V scales' magnitudes
-  // (as integers; zeros aside), 32 lanes a block
+  // The blocks' places, and the range of the V scales' magnitudes (as integers; zeros
+  // aside), 32 lanes a block: of the whole split, its start last, beside whose scales
+  // the first steps' copies are under way.
+  bool missing = false;
+  uint32_t most = 0, least = 0x7f800000u;
+  if (tid < 2) lds.range[tid] = tid == 0 ? most : least;
+  for (int part = (max(steps, 1) - 1) / WIDE_RING * WIDE_RING;; part -= WIDE_RING) {
+    const int n = min(steps - part, WIDE_RING);
+    bool hole = false;
+    if (tid < n) {
+      const int2 at = place(part + tid);
+      hole = at.x < 0;
+      lds.block[tid] = at;
+    }
+    missing |= __syncthreads_or(hole) != 0;
+    if (part == 0) {
 #pragma unroll
-  for (int i = 0; i < WIDE_DEPTH; ++i)
-    if (i < steps) copy(i);
-  {
-    uint32_t most = 0, least = 0x7f800000u;
+      for (int i = 0; i < WIDE_DEPTH; ++i)
+        if (i < steps) copy(i);
+    }
 #pragma unroll 4
-    for (int i = tid >> 5; i < steps; i += 2 * WIDE_WAVES) {
+    for (int i = tid >> 5; i < n; i += 2 * WIDE_WAVES) {
       const int2 at = lds.block[i];
-      if (at.x >= 0 && first + i * KB + n32 < end) {
+      if (at.x >= 0 && first + (part + i) * KB + n32 < end) {
         const uint32_t v = __float_as_uint(a.pool.vs[at.x * a.pool.spage + (at.y + n32) * a.pool.srow + kvh]) & 0x7fffffffu;
         most = max(most, v);
         if (v) least = min(least, v);
       }
     }
+    if (part == 0) break;
+    __syncthreads();
+  }
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      most = max(most, lane_xor_m(most, d));
-      least = min(least, lane_xor_m(least, d));
-    }
-    if (lane == 0) {
-      atomicMax(&lds.range[0], most);
-      atomicMin(&lds.range[1], least);
-    }
+  for (int d = 1; d < 64; d *= 2) {
+    most = max(most, lane_xor_m(most, d));
+    least = min(least, lane_xor_m(least, d));
+  }
+  if (lane == 0) {
+    atomicMax(&lds.range[0], most);
+    atomicMin(&lds.range[1], least);
   }
   wait_copies<0>();
   lds_barrier();
-  const uint32_t most = __builtin_amdgcn_readfirstlane(lds.range[0]), least = __builtin_amdgcn_readfirstlane(lds.range[1]);
+  most = __builtin_amdgcn_readfirstlane(lds.range[0]), least = __builtin_amdgcn_readfirstlane(lds.range[1]);
   // Narrow: within a factor of 2^8, and no closer to the ends than 2^64.
   const int expo = static_cast<int>(most >> 23) - 127;
   const bool narrow = most == 0 || (expo >= -64 && expo <= 64 && least >= most - (8u << 23));
@@ -734,7 +752,7 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
         for (int i = 0; i < 16; ++i) x[i] *= sign;
       }
       seen = 0;
-      const int limit = lds.block[step].x < 0 ? 0 : sees - (first + step * WIDE_KEYS + 4 * half);
+      const int limit = lds.block[step % WIDE_RING].x < 0 ? 0 : sees - (first + step * WIDE_KEYS + 4 * half);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const bool in = 8 * (i >> 2) + (i & 3) < limit;
@@ -818,6 +836,10 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
   int step = 0;
   auto run = [&](int to, auto edge_tag, auto narrow_tag) {
     for (; step < to; ++step) {
+      if (step % (WIDE_RING / 2) == 0 && step > 0) {  // the places after the next, over those gone by
+        const int next = step + WIDE_RING / 2 + tid;
+        if (tid < WIDE_RING / 2 && next < steps) lds.block[next % WIDE_RING] = place(next);
+      }
       const bool more = !decltype(edge_tag)::value || step + 1 < steps;
       if (step + WIDE_DEPTH < steps) copy(step + WIDE_DEPTH);
       v16i s;
@@ -967,7 +989,7 @@ __device__ void join_slots(const SeqAttnArgs &a, const Plan &plan, int cell_cols
     if (row_at(a.seqs, row).seq < 0 || c >= a.heads) return;
     n = p.splits;
   } else {
-    int col = c, cols, seq, span = p.span;
+    int col = c, cols, seq, span;
     SeqSpan sp;
     if constexpr (WIDE) {
       int nth;
@@ -980,7 +1002,8 @@ __device__ void join_slots(const SeqAttnArgs &a, const Plan &plan, int cell_cols
       seq = cell / a.kv_heads;
       sp = seq_span(a.seqs, seq);
       cols = sp.n * group_heads;
-      if (cols > plan.most) return;
+      span = split_span(sp.kv, p.splits, FEW_LEAST, FEW_STEP);
+      if (cols > plan.most || sp.kv <= span) return;  // elsewhere; written as it is
     }
     if (c >= cell_cols || col >= cols) return;
     row = sp.r0 + col / group_heads;
@@ -1028,7 +1051,10 @@ __device__ void join_slots(const SeqAttnArgs &a, const Plan &plan, int cell_cols
   store_row8(a, row, head, d0, r);
 }
 
-constexpr int JOIN_MANY = 12;  // splits from which 16 groups share a slot
+// 16 groups share a slot from 13 splits on, where slots are few: at many the launch's
+// workgroups would cost more than the splits one after another.
+constexpr int JOIN_MANY = 12, JOIN_SLOTS = 2048;
+__host__ __device__ inline bool join_wide(const Partials &p) { return p.splits > JOIN_MANY && p.slots <= JOIN_SLOTS; }
 
 int join_cols(const SeqAttnArgs &a, const FewPlan &p) { return a.ids ? a.heads : p.most; }
 int join_cols(const SeqAttnArgs &, const WidePlan &) { return WIDE_COLS; }
@@ -1036,7 +1062,7 @@ int join_cols(const SeqAttnArgs &, const WidePlan &) { return WIDE_COLS; }
 template <class P>
 int64_t join_wgs(const SeqAttnArgs &a, const P &plan) {
   const int cols = join_cols(a, plan);
-  return plan.part.slots / cols * (plan.part.splits > JOIN_MANY ? cols : (cols + 15) / 16);
+  return plan.part.slots / cols * (join_wide(plan.part) ? cols : (cols + 15) / 16);
 }
 
 // The first `few` workgroups join the 16-column kernel's slots.
@@ -1045,11 +1071,11 @@ __global__ void __launch_bounds__(256) seq_attn_join_kernel(SeqAttnArgs a, FewPl
   const int block = blockIdx.x;
   if (block < few) {
     const int cols = a.ids ? a.heads : fp.most;
-    if (fp.part.splits > JOIN_MANY)
+    if (join_wide(fp.part))
       join_slots<16, false>(a, fp, cols, block, lds);
     else
       join_slots<1, false>(a, fp, cols, block, lds);
-  } else if (wp.part.splits > JOIN_MANY) {
+  } else if (join_wide(wp.part)) {
     join_slots<16, true>(a, wp, WIDE_COLS, block - few, lds);
   } else {
     join_slots<1, true>(a, wp, WIDE_COLS, block - few, lds);
@@ -1062,17 +1088,18 @@ constexpr int64_t kMaxGrid = (int64_t(1) << 32) / 256 - 1;  // workgroups of 256
 
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Splits `keys` over workgroups, `units` of which would run without a split, until
-// there are about `want` of them: spans of a multiple of `step` keys, from `least`
-// to `most`, and at most 64 splits within that.
-void plan_splits(int64_t units, int64_t keys, int64_t want, int step, int least, int most, Partials &p) {
+// Splits `keys` at most over workgroups, `units` of which would run without a split,
+// until there are about `want` of them: 64 splits at most, of `least` keys or more.  A
+// max_kv far above the lengths adds workgroups that end at once, no longer splits: 16 rows
+// at 500 .. 2000 keys take 19.5 us with a max_kv of 2000 and of 131072 (26 where the spans
+// followed max_kv), 512 rows behind 1500 keys 48 both ways (116).
+void plan_splits(int64_t units, int64_t keys, int64_t want, int step, int least, Partials &p) {
   if (keys < 1) keys = 1;
   if (units < 1) units = 1;
   int64_t splits = units >= want ? 1 : want / units;
   if (splits > 64) splits = 64;
   int64_t span = cdiv(cdiv(keys, splits), step) * step;
   if (span < least) span = least;
-  if (span > most) span = most;
   p.span = static_cast<int>(span);
   p.splits = static_cast<int>(cdiv(keys, span));
 }
@@ -1106,13 +1133,13 @@ Plan plan_attn(const SeqAttnArgs &a) {
   p.few.tiles = static_cast<int>(cdiv(few_cols, FEW_COLS));
   p.few.units = (a.ids ? rows : n_seq) * p.few.tiles;
   plan_splits(p.few.units * a.kv_heads, a.ids ? int64_t(a.n_sel) * a.pool.page_tokens : a.seqs.max_kv,
-              a.ids ? LIST_WANT : FEW_WANT, FEW_WAVES * KB, 256, FEW_SPAN, p.few.part);
+              a.ids ? LIST_WANT : FEW_WANT, FEW_STEP, FEW_LEAST, p.few.part);
   if (p.few.part.splits > 1) p.few.part.slots = a.ids ? rows * a.heads : n_seq * a.kv_heads * few_cols;
   if (p.any_wide) {
     p.wide.least = FEW_MOST + 1;
     const int64_t wide_seqs = rows * g / p.wide.least;
     p.wide.tiles = rows * g / WIDE_COLS + (n_seq < wide_seqs ? n_seq : wide_seqs);
-    plan_splits(p.wide.tiles * a.kv_heads, a.seqs.max_kv, WIDE_WANT, WIDE_KEYS, 512, WIDE_SPAN, p.wide.part);
+    plan_splits(p.wide.tiles * a.kv_heads, a.seqs.max_kv, WIDE_WANT, WIDE_KEYS, WIDE_LEAST, p.wide.part);
     if (p.wide.part.splits > 1) p.wide.part.slots = p.wide.tiles * a.kv_heads * WIDE_COLS;
   }
   return p;

@@ -255,6 +255,55 @@ def test_attention_scales(cuda):
     assert (err <= bound).all(), float((err / bound).max())
 
 
+@pytest.mark.parametrize("kind", ["few", "many", "hole", "wide", "listed"])
+def test_attention_unsplit(cuda, kind):
+    """So many sequences (of the same pages) that their 17000 keys are not split: more
+    blocks than are named at a time."""
+    kvh, n_sel = 16, 300
+    n, rows = (100, 1) if kind in ("few", "listed") else (49, 17)
+    b = Batch([(rows, 17000 - rows)], kvh, 32, seed=6)
+    if kind == "hole":
+        b.tables[0, 300:310] = 65535
+    if kind == "wide":
+        b.vs *= np.exp2(np.floor(b.rng.random(b.vs.shape) * 12) - 6).astype(F)
+    q8, qs = queries(b.rng, n * rows, kvh)
+    lens = 17000 - 7 * np.arange(n)
+    ids = np.sort(np.stack([b.rng.permutation(531)[:n_sel] for _ in range(kvh)]), 1).astype(np.int32).reshape(1, -1)
+    pool, _ = on_device(b)
+    seqs = ops.sequences(pool, dev(np.repeat(b.tables, n, 0)), dev((rows * np.arange(n + 1)).astype(np.int32)),
+                         dev(lens.astype(np.int32)), rows, 17000)
+    out = torch.empty((n * rows, kvh * 128), device="cuda")
+    if kind == "listed":
+        ops.attention_pages(dev(q8), dev(qs), pool, seqs, dev(np.repeat(ids, n, 0)), n_sel, out, qk_scale=QK)
+    else:
+        ops.attention_varlen_paged(dev(q8), dev(qs), pool, seqs, out, qk_scale=QK)
+    got = out.cpu().numpy()
+    assert np.isfinite(got).all()
+    for i in (0, n // 2, n - 1):
+        b.lens, b.kv_len, b.rows = [(rows, int(lens[i]) - rows)], lens[i:i + 1], rows
+        at = slice(i * rows, (i + 1) * rows)
+        want, mag, top = attend(b, q8[at], qs[at], kvh, QK, True, ids if kind == "listed" else None, n_sel)
+        assert (np.abs(got[at] - want) <= attend_bound(mag, top, 17000)).all(), i
+
+
+@pytest.mark.parametrize("lens,heads,kv_heads", [([(1, 543)], 16, 8), ([(1, 700), (1, 5), (1, 1300)], 16, 8), ([(33, 500), (1, 90)], 16, 8),
+                                                 ([(300, 500), (1, 40)], 16, 2)])
+def test_attention_loose_limits(cuda, lens, heads, kv_heads):
+    """max_kv far above the lengths, tables as wide: the same results, and a workspace
+    that does not grow with it without end."""
+    b = Batch(lens, kv_heads, 32, seed=12)
+    q8, qs = queries(b.rng, b.rows, heads)
+    pool, seqs = on_device(b)
+    wide = np.full((len(lens), 8192), 65535, np.uint16)
+    wide[:, :b.tables.shape[1]] = b.tables
+    loose = ops.sequences(pool, dev(wide), *seqs._keep[1:], b.max_rows, 8192 * 32)
+    assert ops.seqs_workspace_bytes(pool, loose, b.rows, heads) <= 65 * (b.rows + 128 * len(lens)) * heads * 520
+    want, mag, top = attend(b, q8, qs, heads, QK)
+    out = torch.empty((b.rows, heads * 128), device="cuda")
+    ops.attention_varlen_paged(dev(q8), dev(qs), pool, loose, out, qk_scale=QK)
+    assert (np.abs(out.cpu().numpy() - want) <= attend_bound(mag, top, b.max_kv)).all()
+
+
 @pytest.mark.parametrize("kind", ["few", "many", "listed"])
 def test_attention_nan(cuda, kind):
     """A NaN query, key or value scale reaches the results that it enters, whole rows of
