@@ -156,6 +156,7 @@ __global__ void __launch_bounds__(256, 8) seq_append_kernel(SeqAppendArgs a, int
       // (a head's 32 lanes are in one wave, which finishes its LDS writes before its
       // reads, and those before the next row's writes)
       *reinterpret_cast<float4 *>(&ex[slot][c0]) = make_float4(y[0], y[1], y[2], y[3]);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
       if (turns && angles) {
         float o[4] = {y[1], y[0], y[3], y[2]};
@@ -183,6 +184,7 @@ __global__ void __launch_bounds__(256, 8) seq_append_kernel(SeqAppendArgs a, int
           }
         }
       }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
     }
     const float m = max32(fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3]))));
@@ -211,7 +213,8 @@ __global__ void __launch_bounds__(256, 8) seq_append_kernel(SeqAppendArgs a, int
 // and the page is read anew on every call: rewritten slots leave no trace.
 // One workgroup per (page, head): 8 lanes a key (16 bytes each), 32 keys a step.
 // A page written by this call has just left the caches' write path, so the 4 KiB
-// of a 32-token page and head come from L2.
+// of a 32-token page and head come from L2.  781 rows of 7 sequences, 8 heads: 5.9 us, the
+// chain length -> table -> keys and two barriers.
 __global__ void __launch_bounds__(256) page_bounds_kernel(PageBoundsArgs a, int pages_per_seq) {
   __shared__ float lo_s[4][HD], hi_s[4][HD];
   __shared__ float peak[2];

@@ -196,7 +196,9 @@ __device__ __forceinline__ float exp2_from(float x, float base) { return __built
 // registers, four a CU, reads half lines: 32 rows at 16000 keys 233 us instead of 208).  16-byte chunk
 // c of key r lies at chunk c ^ (r & 7) (V: c ^ vswz(r)), so that neither the K
 // operand's reads (16 keys, one chunk) nor the transposing reads of V (8 keys, one
-// chunk) meet in a bank.
+// chunk) meet in a bank.  Bound by the K/V stream once there are keys enough: one row at
+// 131072 keys 56 us (4.9 TB/s), 32 rows at 16000, eight heads a KV head, 208 with the join
+// (5.2); one row at 543 keys 6.7, a launch and the chain length -> table -> keys.
 constexpr int KB = 32;
 constexpr int FEW_COLS = 16;
 constexpr int FEW_WAVES = 4;
@@ -967,9 +969,9 @@ __global__ void __launch_bounds__(256, 2) seq_attn_mixed_kernel(SeqAttnArgs a, F
 }
 
 // Joins the splits of slots: 16 lanes of 8 channels a slot, of many splits 16 such
-// groups over the splits in turn (GROUPS; 16 slots a workgroup otherwise).  A cell is
-// what slots are counted in: (sequence, KV head) or row of the 16-column kernel,
-// (tile, KV head) of the 128-column one.
+// groups over the splits in turn (GROUPS; 16 slots a workgroup otherwise): 4 to 5 us,
+// most of it the launch.  A cell is what slots are counted in: (sequence, KV head) or
+// row of the 16-column kernel, (tile, KV head) of the 128-column one.
 struct JoinLds {
   float o[4][HD], sum[4];
 };
