@@ -215,7 +215,15 @@ struct FewPlan {
   int64_t units;  // (sequence or row) x tiles of 16 columns
   int tiles;
   int most;       // columns of a sequence that are taken here
+  int each;       // workgroups of a sequence and KV head to aim at
 };
+
+// The keys of a split of a sequence, whose tiles share its part of the workgroups (so a
+// decoding row beside short chunks is split as finely as among its like).
+__device__ __forceinline__ int few_span(const FewPlan &p, int keys, int cols) {
+  const int tiles = (cols + FEW_COLS - 1) / FEW_COLS;
+  return split_span(keys, clampi(p.each / max(tiles, 1), 1, p.part.splits), FEW_LEAST, FEW_STEP);
+}
 
 struct FewLds {
   __align__(16) uint8_t stage[FEW_WAVES * FEW_WAVE];
@@ -261,7 +269,7 @@ __device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, F
     const SeqSpan sp = seq_span(a.seqs, seq);
     cols = sp.n * group_heads;
     if (cols > p.most || tile * FEW_COLS >= cols) return;
-    span = split_span(sp.kv, p.part.splits, FEW_LEAST, FEW_STEP);
+    span = few_span(p, sp.kv, cols);
     whole = sp.kv <= span;
     row0 = sp.r0, row = sp.r0 + c / group_heads, g = c % group_heads;
     sees = a.causal ? max(sp.pos(row) + 1, 0) : sp.kv;
@@ -288,6 +296,7 @@ __device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, F
     cs = a.qs[row * a.ldqs + (kvh * group_heads + g) * a.qs_col] * a.qk_scale * kLog2e;
   }
 
+  const bool once = ONCE || (!LIST && cols <= FEW_COLS);  // (a sequence of one tile)
   uint8_t *const stages = lds.stage + wave * FEW_WAVE;
   const int r8 = lane >> 3, ch = lane & 7;
   const int64_t lane_k = r8 * a.pool.row_bytes + 16 * (ch ^ r8);
@@ -298,10 +307,17 @@ __device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, F
     const int64_t at = page * a.pool.page_bytes + t0 * a.pool.row_bytes + kvh * HD;
     const int8_t *k = a.pool.k + at, *v = a.pool.v + at;
     const int64_t eight = 8 * a.pool.row_bytes;
+    auto copy = [&](auto nt_tag) {
+      constexpr bool NT = decltype(nt_tag)::value;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) lds_copy16<ONCE>(k + q * eight + lane_k, stages + FEW_K + q * 1024);
+      for (int q = 0; q < 4; ++q) lds_copy16<NT>(k + q * eight + lane_k, stages + FEW_K + q * 1024);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) lds_copy16<ONCE>(v + q * eight + (q < 2 ? lane_v : lane_v4), st + FEW_V + q * 1024);
+      for (int q = 0; q < 4; ++q) lds_copy16<NT>(v + q * eight + (q < 2 ? lane_v : lane_v4), st + FEW_V + q * 1024);
+    };
+    if (once)
+      copy(std::true_type{});
+    else
+      copy(std::false_type{});
     const int64_t sat = page * a.pool.spage + (t0 + (lane & 31)) * a.pool.srow + kvh;
     lds_copy4((lane < 32 ? a.pool.ks : a.pool.vs) + sat, st + FEW_S);
   };
@@ -1004,7 +1020,7 @@ __device__ void join_slots(const SeqAttnArgs &a, const Plan &plan, int cell_cols
       seq = cell / a.kv_heads;
       sp = seq_span(a.seqs, seq);
       cols = sp.n * group_heads;
-      span = split_span(sp.kv, p.splits, FEW_LEAST, FEW_STEP);
+      span = few_span(plan, sp.kv, cols);
       if (cols > plan.most || sp.kv <= span) return;  // elsewhere; written as it is
     }
     if (c >= cell_cols || col >= cols) return;
@@ -1055,7 +1071,7 @@ __device__ void join_slots(const SeqAttnArgs &a, const Plan &plan, int cell_cols
 
 // 16 groups share a slot from 13 splits on, where slots are few: at many the launch's
 // workgroups would cost more than the splits one after another.
-constexpr int JOIN_MANY = 12, JOIN_SLOTS = 2048;
+constexpr int JOIN_MANY = 12, JOIN_SLOTS = 1024;
 __host__ __device__ inline bool join_wide(const Partials &p) { return p.splits > JOIN_MANY && p.slots <= JOIN_SLOTS; }
 
 int join_cols(const SeqAttnArgs &a, const FewPlan &p) { return a.ids ? a.heads : p.most; }
@@ -1107,12 +1123,15 @@ void plan_splits(int64_t units, int64_t keys, int64_t want, int step, int least,
 }
 
 // Sequences of up to FEW_MOST columns go to the kernel of 16-column tiles, and all
-// of a call do while rows x heads x max_kv stays small: its tiles fill the CUs
-// sooner.  us, 16-column / 128-column tiles, 16 heads on 8: 32 rows behind 500 keys
-// 11 / 29, 512 rows 20 / 26, 64 rows behind 4000 keys (4.2e6) 24 / 31, 1024 rows (17e6)
-// 44 / 37, 256 rows behind 4000 keys 60 / 47, 8 x 64 rows behind 1000 keys (8.7e6)
-// 40 / 35.
-constexpr int FEW_MOST = 16;
+// of a call do where none has more than FEW_ALL, or while rows x heads x max_kv stays
+// small: its tiles fill the CUs sooner.  us, 16-column / 128-column tiles, 16 heads on 8:
+// 32 rows behind 500 keys 11 / 29, 512 rows 20 / 26, 64 rows behind 4000 keys (4.2e6) 24
+// / 31, 1024 rows (17e6) 44 / 37, 256 rows behind 4000 keys 60 / 47, 8 x 64 rows behind
+// 1000 keys (8.7e6) 40 / 35.  8 sequences behind 4000 keys: of 16 rows (32 columns) 33 /
+// 47, 24 (48) 38 / 48, 32 (64) 45 / 48; 64 behind 2000, 64 heads on 8: of 4 rows (32)
+// 90 / 125, of 8 (64) 139 / 129.  Beside longer sequences only those of one tile: with
+// tiles for 48 columns 60 decoding rows and 4 chunks of 128 rows take 79 instead of 70.
+constexpr int FEW_MOST = 16, FEW_ALL = 48;
 constexpr int64_t FEW_PAIRS = 6 << 20;
 // Workgroups to split for: equal lists of pages 1024, sequences, whose lengths differ,
 // more (64 rows at 500 .. 4000 keys 1024: 62 us, 1536: 56, 2304: 56; 92 rows' lists 49, 53, 56).
@@ -1129,12 +1148,13 @@ Plan plan_attn(const SeqAttnArgs &a) {
   const int64_t g = a.heads / a.kv_heads, rows = a.seqs.rows, n_seq = a.seqs.n_seq;
   const int64_t cols = a.ids ? g : a.seqs.max_rows * g;  // of a sequence (listed pages: of a row), at most
   const bool small = rows * a.heads * a.seqs.max_kv <= FEW_PAIRS && n_seq * cdiv(cols, FEW_COLS) * a.kv_heads <= 8 * FEW_WANT;
-  p.any_wide = !a.ids && cols > FEW_MOST && !small;
+  p.any_wide = !a.ids && cols > FEW_ALL && !small;
   const int64_t few_cols = p.any_wide ? FEW_MOST : cols < 1 ? 1 : cols;
   p.few.most = static_cast<int>(few_cols);
   p.few.tiles = static_cast<int>(cdiv(few_cols, FEW_COLS));
   p.few.units = (a.ids ? rows : n_seq) * p.few.tiles;
-  plan_splits(p.few.units * a.kv_heads, a.ids ? int64_t(a.n_sel) * a.pool.page_tokens : a.seqs.max_kv,
+  p.few.each = static_cast<int>(cdiv(FEW_WANT, (n_seq < 1 ? 1 : n_seq) * a.kv_heads));
+  plan_splits((a.ids ? p.few.units : n_seq) * a.kv_heads, a.ids ? int64_t(a.n_sel) * a.pool.page_tokens : a.seqs.max_kv,
               a.ids ? LIST_WANT : FEW_WANT, FEW_STEP, FEW_LEAST, p.few.part);
   if (p.few.part.splits > 1) p.few.part.slots = a.ids ? rows * a.heads : n_seq * a.kv_heads * few_cols;
   if (p.any_wide) {

@@ -255,12 +255,12 @@ def test_attention_scales(cuda):
     assert (err <= bound).all(), float((err / bound).max())
 
 
-@pytest.mark.parametrize("kind", ["few", "many", "hole", "wide", "listed"])
+@pytest.mark.parametrize("kind", ["few", "short", "many", "hole", "wide", "listed"])
 def test_attention_unsplit(cuda, kind):
     """So many sequences (of the same pages) that their 17000 keys are not split: more
     blocks than are named at a time."""
     kvh, n_sel = 16, 300
-    n, rows = (100, 1) if kind in ("few", "listed") else (49, 17)
+    n, rows = {"few": (100, 1), "listed": (100, 1), "short": (49, 17)}.get(kind, (50, 49))
     b = Batch([(rows, 17000 - rows)], kvh, 32, seed=6)
     if kind == "hole":
         b.tables[0, 300:310] = 65535
@@ -302,6 +302,15 @@ def test_attention_loose_limits(cuda, lens, heads, kv_heads):
     out = torch.empty((b.rows, heads * 128), device="cuda")
     ops.attention_varlen_paged(dev(q8), dev(qs), pool, loose, out, qk_scale=QK)
     assert (np.abs(out.cpu().numpy() - want) <= attend_bound(mag, top, b.max_kv)).all()
+
+
+@pytest.mark.parametrize("lens,heads,kv_heads", [([(24, 4000)] * 8, 16, 8), ([(5, 3000), (1, 5000), (48, 700), (0, 9), (17, 0)] * 3, 8, 8),
+                                                 ([(4, 2000), (1, 3500), (6, 100)] * 4, 64, 8)])
+def test_attention_short_chunks(cuda, lens, heads, kv_heads):
+    """Up to 48 columns of every sequence: 16-column tiles alone, some of them split."""
+    b = Batch(lens, kv_heads, 32, seed=14)
+    assert b.rows * heads * b.max_kv > 6 << 20 and b.max_rows * heads // kv_heads <= 48
+    check_attention(b, heads)
 
 
 @pytest.mark.parametrize("kind", ["few", "many", "listed"])
