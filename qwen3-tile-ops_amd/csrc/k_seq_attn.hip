@@ -499,8 +499,8 @@ __device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, F
 // their own, integer scores read as floats.  A wave's step is some 700 cycles of vector
 // and 660 of matrix instructions and takes 1800 of its SIMD: what a step waits
 // beyond its issue is the barrier and the LDS reads.  Three prompts of 1700 rows, 32
-// heads on 8: 129 us, 0.40 of the rate of a large bf16 matrix product for the products
-// that the causal mask leaves.  Matrix and vector instructions set apart by hand, a
+// heads on 8: 128 to 138 us from run to run, 0.37 to 0.40 of the rate of a large bf16
+// matrix product for the products that the causal mask leaves.  Matrix and vector instructions set apart by hand, a
 // wave's priority over its products, 64 keys a step, eight waves that halve the keys
 // and a third workgroup a CU (spills) were not faster.
 //
