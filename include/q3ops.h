@@ -266,7 +266,7 @@ typedef struct q3_seqs {
   const int32_t *row_start; /* device [n_seq + 1]                            */
   const int32_t *kv_len;    /* device [n_seq]: cached tokens, new ones included */
   const uint16_t *tables;   /* device [n_seq][ld_table]                      */
-  uint32_t n_seq;           /* at most 65535                                 */
+  uint32_t n_seq;           /* at most 4096                                  */
   uint32_t ld_table;        /* logical pages of a table row                  */
   uint32_t n_pages;         /* pages in the pool                             */
   uint32_t max_rows;        /* no sequence has more new rows (<= rows)       */

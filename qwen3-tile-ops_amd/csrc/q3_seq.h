@@ -53,26 +53,37 @@ struct SeqRow {
   int seq, pos;
 };
 
-// Of the wave-uniform rows row0 .. row0 + ROWS - 1: each is in the sequence behind
-// as many as end at or before it.  64 sequences a step, one per lane, whose starts
-// and lengths come with their ends: one round trip to memory.
+// Of the wave-uniform rows row0 .. row0 + ROWS - 1: each is in the sequence behind as
+// many as end at or before it.  Of up to 64 sequences one per lane, whose starts and
+// lengths come with their ends: one round trip to memory for all rows.  Of more, each
+// row's 64 are found first, by the ends of 64 equal parts (starts do not decrease).
 template <int ROWS>
 __device__ __forceinline__ void rows_at(const Seqs &q, int row0, SeqRow (&at)[ROWS]) {
   const int lane = threadIdx.x & 63;
+  int lo = 0, n = q.n_seq, begin = 0, end = INT32_MAX, kv = 0;
+  auto load = [&]() {
+    const int j = lane < n ? lo + lane : 0;
+    begin = q.start[j], end = lane < n ? q.start[j + 1] : INT32_MAX, kv = q.kv_len[j];
+  };
+  if (n <= 64) load();
 #pragma unroll
-  for (int r = 0; r < ROWS; ++r) at[r] = {-1, 0};
-#pragma unroll 2
-  for (int b = 0; b < q.n_seq; b += 64) {
-    const int j = min(b + lane, q.n_seq - 1);
-    const int begin = q.start[j], end = b + lane < q.n_seq ? q.start[j + 1] : INT32_MAX, kv = q.kv_len[j];
-#pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
-      const int before = __popcll(__ballot(end <= row0 + r));
-      if (at[r].seq >= 0 || before >= 64 || b + before >= q.n_seq) continue;
-      const SeqSpan sp = seq_span(q, __builtin_amdgcn_readlane(begin, before), __builtin_amdgcn_readlane(end, before),
-                                  __builtin_amdgcn_readlane(kv, before));
-      if (row0 + r >= sp.r0 && row0 + r < sp.r0 + sp.n) at[r] = {b + before, sp.pos(row0 + r)};
+  for (int r = 0; r < ROWS; ++r) {
+    at[r] = {-1, 0};
+    const int row = row0 + r;
+    if (q.n_seq > 64) {
+      for (lo = 0, n = q.n_seq; n > 64;) {
+        const int part = (n + 63) / 64, last = min((lane + 1) * part, n) - 1;
+        const int skip = min(__popcll(__ballot(q.start[lo + last + 1] <= row)) * part, n);
+        lo += skip;
+        n = min(part, n - skip);
+      }
+      load();
     }
+    const int before = __popcll(__ballot(end <= row));
+    if (before >= n) continue;
+    const SeqSpan sp = seq_span(q, __builtin_amdgcn_readlane(begin, before), __builtin_amdgcn_readlane(end, before),
+                                __builtin_amdgcn_readlane(kv, before));
+    if (row >= sp.r0 && row < sp.r0 + sp.n) at[r] = {lo + before, sp.pos(row)};
   }
 }
 __device__ __forceinline__ SeqRow row_at(const Seqs &q, int row) {

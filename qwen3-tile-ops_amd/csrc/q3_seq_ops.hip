@@ -18,6 +18,7 @@ using q3::unsupported;
 constexpr uint32_t kMaxTokens = 1u << 30;  // positions are 32-bit on the device
 constexpr uint32_t kMaxRows = 1u << 21;    // rows x heads, and twice that, are 32-bit too
 constexpr int kMaxHeads = 512;
+constexpr uint32_t kMaxSeqs = 4096;  // a 128-column tile's workgroup looks through them all
 
 bool aligned(const void *p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
@@ -34,7 +35,7 @@ int seq_common(const q3_paged_kv *kv, const q3_seqs *q, uint32_t rows, int kv_he
     return Q3_ERR_VIEW;
   if (q->n_seq && (!q->row_start || !q->kv_len || !q->tables)) return Q3_ERR_ARG;
   if (!aligned(q->row_start, 4) || !aligned(q->kv_len, 4) || !aligned(q->tables, 2)) return Q3_ERR_VIEW;
-  if (q->n_seq > 65535 || rows > kMaxRows || q->max_kv > kMaxTokens || pt > kMaxTokens) return Q3_ERR_RANGE;
+  if (q->n_seq > kMaxSeqs || rows > kMaxRows || q->max_kv > kMaxTokens || pt > kMaxTokens) return Q3_ERR_RANGE;
   if (q->max_kv > q->ld_table * pt) return Q3_ERR_RANGE;  // keys behind the table
   if (q->max_rows > rows && q->n_seq) return Q3_ERR_RANGE;
   p = {static_cast<int8_t *>(kv->k), static_cast<int8_t *>(kv->v), static_cast<float *>(kv->ks), static_cast<float *>(kv->vs),
@@ -282,7 +283,7 @@ int q3_attention_pages(const q3_view *q8, const q3_view *q_scale, const q3_paged
 int q3_seqs_workspace(const q3_seqs *seqs, uint32_t rows, uint32_t page_tokens, int heads, int kv_heads, uint32_t n_sel,
                       uint64_t *bytes) {
   if (!seqs || !bytes || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads > kMaxHeads || page_tokens == 0) return Q3_ERR_ARG;
-  if (seqs->n_seq > 65535 || rows > kMaxRows || seqs->max_kv > kMaxTokens || seqs->max_rows > kMaxRows ||
+  if (seqs->n_seq > kMaxSeqs || rows > kMaxRows || seqs->max_kv > kMaxTokens || seqs->max_rows > kMaxRows ||
       page_tokens > kMaxTokens || n_sel > 65536)
     return Q3_ERR_RANGE;
   q3::SeqAttnArgs a{};

@@ -313,6 +313,26 @@ def test_attention_short_chunks(cuda, lens, heads, kv_heads):
     check_attention(b, heads)
 
 
+@pytest.mark.parametrize("n", [64, 65, 128, 129, 700, 4096])
+def test_many_sequences(cuda, n):
+    """More sequences than a wave has lanes, some without rows, rows around them all."""
+    lens = [((i * 7) % 3, (i * 13) % 40) for i in range(n)]
+    if n == 129:
+        lens[70] = (200, 700)  # 128-column tiles too
+    b = Batch(lens, 2, 32, seed=n, before=3, behind=2)
+    check_attention(b, 4)
+    append_case(Batch(lens, 2, 32, seed=n, before=3, behind=2), 4, 64, False, True)
+    bounds, scale, _ = bounds_on_host(b)
+    q8, qs = queries(b.rng, b.rows, 4)
+    pool, seqs = on_device(b)
+    ids = torch.full((b.rows, 2), 7, dtype=torch.int32, device="cuda")
+    ops.select_pages(dev(q8), dev(qs), pool, seqs, dev(bounds), dev(scale), ids, 1)
+    want = np.full((b.rows, 2), 7, np.int32)
+    for row, _, pos in b.row_positions():
+        want[row] = pos // 32
+    assert np.array_equal(ids.cpu().numpy(), want)
+
+
 @pytest.mark.parametrize("kind", ["few", "many", "listed"])
 def test_attention_nan(cuda, kind):
     """A NaN query, key or value scale reaches the results that it enters, whole rows of

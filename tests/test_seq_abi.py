@@ -43,7 +43,7 @@ BAD_POOL = [(dict(k=None), ARG), (dict(vs=None), ARG), (dict(page_tokens=0), UNS
             (dict(scale_page_bytes=32 * 8 - 4), VIEW), (dict(k=_ADDR + 8), VIEW), (dict(ks=_ADDR + 2), VIEW),
             (dict(page_tokens=1 << 31, page_bytes=0xFFFFFFFF), VIEW)]
 BAD_SEQS = [(dict(row_start=None), ARG), (dict(kv_len=None), ARG), (dict(tables=None), ARG), (dict(tables=_ADDR + 1), VIEW),
-            (dict(row_start=_ADDR + 2), VIEW), (dict(n_seq=65536), RANGE), (dict(max_kv=129), RANGE), (dict(ld_table=3), RANGE),
+            (dict(row_start=_ADDR + 2), VIEW), (dict(n_seq=65536), RANGE), (dict(n_seq=4097), RANGE), (dict(max_kv=129), RANGE), (dict(ld_table=3), RANGE),
             (dict(max_rows=ROWS + 1), RANGE), (dict(max_kv=(1 << 30) + 1, ld_table=1 << 30), RANGE)]
 PLACES = [(pool(**kw), seqs(), rc) for kw, rc in BAD_POOL] + [(pool(), seqs(**kw), rc) for kw, rc in BAD_SEQS] + \
          [(None, seqs(), ARG), (pool(), None, ARG)]
