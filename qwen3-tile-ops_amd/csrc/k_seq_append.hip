@@ -215,13 +215,17 @@ __global__ void __launch_bounds__(256, 8) seq_append_kernel(SeqAppendArgs a, int
 // A page written by this call has just left the caches' write path, so the 4 KiB
 // of a 32-token page and head come from L2.  781 rows of 7 sequences, 8 heads: 5.9 us, the
 // chain length -> table -> keys and two barriers.
-__global__ void __launch_bounds__(256) page_bounds_kernel(PageBoundsArgs a, int pages_per_seq) {
+__global__ void __launch_bounds__(256) page_bounds_kernel(PageBoundsArgs a, int per, bool named) {
   __shared__ float lo_s[4][HD], hi_s[4][HD];
   __shared__ float peak[2];
-  const int s = blockIdx.y;
-  const int head = blockIdx.x % a.kv_heads, nth = blockIdx.x / a.kv_heads;
-  const SeqSpan sp = seq_span(a.seqs, s);
+  const int head = blockIdx.x % a.kv_heads, unit = blockIdx.x / a.kv_heads;
   const int pt = a.pool.page_tokens;
+  const SeqPart at = !named ? SeqPart{unit / per, unit % per} : nth_part(a.seqs, unit, [&](const SeqSpan &sp) {
+    return sp.n == 0 || sp.kv == 0 ? 0 : (sp.kv - 1) / pt - max(sp.kv - sp.n, 0) / pt + 1;
+  });
+  if (at.seq < 0) return;
+  const int s = at.seq, nth = at.part;
+  const SeqSpan sp = seq_span(a.seqs, s);
   if (sp.n == 0 || sp.kv == 0) return;
   const int logical = max(sp.kv - sp.n, 0) / pt + nth;
   if (static_cast<int64_t>(logical) * pt >= sp.kv) return;
@@ -308,9 +312,15 @@ hipError_t launch_seq_append(const SeqAppendArgs &a, hipStream_t s) {
 hipError_t launch_page_bounds(const PageBoundsArgs &a, hipStream_t s) {
   if (a.seqs.rows == 0 || a.seqs.n_seq == 0) return hipSuccess;
   const int pt = a.pool.page_tokens;
-  const int per = (min(a.seqs.max_rows, a.seqs.max_kv) + pt - 2) / pt + 1;  // pages that max_rows tokens can lie in
-  if (static_cast<int64_t>(per) * a.kv_heads * a.seqs.n_seq > INT32_MAX / 256) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(page_bounds_kernel, dim3(static_cast<unsigned>(per * a.kv_heads), a.seqs.n_seq), dim3(256), 0, s, a, per);
+  const int64_t most = min(a.seqs.max_rows, a.seqs.max_kv), n_seq = a.seqs.n_seq;
+  const int64_t per = (most + pt - 2) / pt + 1;  // pages that max_rows tokens can lie in
+  // (of all rows: n lie in n / pt pages and two more at most)
+  const int64_t all = a.seqs.rows / pt + 2 * n_seq;
+  const bool named = name_parts(a.seqs, per) && all < n_seq * per;
+  const int64_t pages = named ? all : n_seq * per;
+  if (pages * a.kv_heads > INT32_MAX / 256) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(page_bounds_kernel, dim3(static_cast<unsigned>(pages * a.kv_heads)), dim3(256), 0, s, a,
+                     static_cast<int>(per), named);
   return hipGetLastError();
 }
 

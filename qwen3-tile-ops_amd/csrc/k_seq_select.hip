@@ -23,13 +23,16 @@ constexpr int PICK_MOST = 256 * PICK_REGS;
 // sequence has few rows: a wave has the 16 KiB of its 64 pages in flight at once,
 // and the workgroups of a long context fill the CUs.  One row over 1024 pages takes 7.6
 // us, 24 rows of 64 heads over 170 on average 7.7: the chain length -> table -> bounds.
-__global__ void __launch_bounds__(256) page_score_kernel(SelectArgs a, int tile_rows, int tiles) {
+__global__ void __launch_bounds__(256) page_score_kernel(SelectArgs a, int tile_rows, int tiles, bool named) {
   __shared__ __align__(16) uint32_t key_s[4][16][20];  // [column][page of a 16-page group]
   const int lane = threadIdx.x & 63, wave = wave_id();
   const int col = lane & 15, quarter = lane >> 4;
   const int g = a.heads / a.kv_heads;
   const int head = blockIdx.x % a.kv_heads, unit = blockIdx.x / a.kv_heads;
-  const int seq = unit / tiles, tile = unit % tiles;
+  const SeqPart at = !named ? SeqPart{unit / tiles, unit % tiles}
+                            : nth_part(a.seqs, unit, [&](const SeqSpan &sp) { return (sp.n + tile_rows - 1) / tile_rows; });
+  if (at.seq < 0) return;
+  const int seq = at.seq, tile = at.part;
   const SeqSpan sp = seq_span(a.seqs, seq);
   const int row0 = sp.r0 + tile * tile_rows;
   const int rows = min(sp.r0 + sp.n - row0, tile_rows);
@@ -212,11 +215,14 @@ hipError_t launch_select_pages(const SelectArgs &a, hipStream_t s) {
   if (pages > a.n_sel) {
     const int tile_rows = 16 * a.kv_heads / a.heads;
     const int tiles = (max(a.seqs.max_rows, 1) + tile_rows - 1) / tile_rows;
-    const int64_t units = static_cast<int64_t>(a.seqs.n_seq) * tiles * a.kv_heads;
+    // (row tiles of all sequences: at most)
+    const int64_t each = static_cast<int64_t>(a.seqs.n_seq) * tiles, all = a.seqs.rows / tile_rows + a.seqs.n_seq;
+    const bool named = name_parts(a.seqs, tiles) && all < each;
+    const int64_t units = (named ? all : each) * a.kv_heads;
     const int64_t chunks = (pages + SCORE_PAGES - 1) / SCORE_PAGES;
     if (units > INT32_MAX / 256 || chunks > 65535 || units * chunks > INT32_MAX / 256) return hipErrorInvalidValue;
     hipLaunchKernelGGL(page_score_kernel, dim3(static_cast<unsigned>(units), static_cast<unsigned>(chunks)), dim3(256), 0, s, a,
-                       tile_rows, tiles);
+                       tile_rows, tiles, named);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
   if (items > INT32_MAX / 256) return hipErrorInvalidValue;

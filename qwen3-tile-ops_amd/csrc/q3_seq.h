@@ -29,6 +29,13 @@ struct Seqs {
   int n_seq, rows, max_rows, max_kv;
 };
 
+// Whether a launch over parts of the sequences, `most` of one, names the parts one by
+// one (nth_part), or has workgroups for `most` parts of every sequence: naming them takes
+// a step per 64 sequences in every workgroup.  us, named / not: scores of 63 decoding
+// rows and a chunk of 512 with a max_kv of 131072, 64 parts, 56 / 286; bounds of the same,
+// 17 parts, 7.8 / 11.6; bounds of 2000 decoding rows and a prompt of 512 481 / 241.
+inline bool name_parts(const Seqs &q, int64_t most) { return most > 1 && q.n_seq <= 32 * most; }
+
 #if defined(__HIPCC__)
 
 // A sequence's rows [r0, r0 + n) and its cached keys.
@@ -90,6 +97,33 @@ __device__ __forceinline__ SeqRow row_at(const Seqs &q, int row) {
   SeqRow at[1];
   rows_at<1>(q, row, at);
   return at[0];
+}
+
+// The sequence, and which of its parts, of the unit-th of all sequences' parts
+// (parts(span) of each; seq -1 behind the last): a launch then needs no workgroups for as
+// many parts of every sequence as the longest may have.
+struct SeqPart {
+  int seq, part;
+};
+template <class Parts>
+__device__ __forceinline__ SeqPart nth_part(const Seqs &q, int unit, Parts parts) {
+  const int lane = threadIdx.x & 63;
+  for (int b = 0; b < q.n_seq; b += 64) {
+    const int mine = b + lane < q.n_seq ? parts(seq_span(q, b + lane)) : 0;
+    int upto = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int x = __shfl_up(upto, d);
+      if (lane >= d) upto += x;
+    }
+    const int total = __builtin_amdgcn_readlane(upto, 63);
+    if (unit < total) {
+      const int at = __popcll(__ballot(upto <= unit));
+      return {b + at, unit - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(mine, at))};
+    }
+    unit -= total;
+  }
+  return {-1, 0};
 }
 
 // Physical page of a sequence's logical page (0 <= logical * page_tokens <

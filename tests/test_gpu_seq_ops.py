@@ -834,6 +834,33 @@ def test_selection_on_two_streams(cuda):
             assert torch.equal(ids, sets[2][0][0]) and torch.equal(out, sets[2][0][1])
 
 
+@pytest.mark.parametrize("n", [3, 100, 700])
+def test_bounds_and_selection_of_unequal_sequences(cuda, n):
+    """One long chunk among sequences of a row or none: parts of the sequences named one
+    by one, and, of many sequences, not."""
+    kvh, heads, n_sel = 2, 8, 3
+    lens = [(int((i % 5) > 0), (i * 37) % 150) for i in range(n)]
+    lens[n // 2] = (300, 200)
+    b = Batch(lens, kvh, 32, seed=n, before=1, behind=2, smooth=True)
+    pool, seqs = on_device(b)
+    want, wscale, touched = bounds_on_host(b)
+    bounds = torch.full((b.n_pages * kvh, 256), 99, dtype=torch.int8, device="cuda")
+    scale = torch.full(wscale.shape, 7.5, device="cuda")
+    ops.page_bounds(pool, seqs, bounds, scale, b.rows)
+    got = bounds.cpu().numpy().reshape(b.n_pages, -1)
+    assert bits_equal(got[touched], want.reshape(b.n_pages, -1)[touched]) and (got[~touched] == 99).all()
+    assert bits_equal(scale.cpu().numpy()[touched], wscale[touched])
+    hb = b.rng.integers(-127, 128, (b.n_pages * kvh, 256)).astype(np.int8)
+    hs = b.rng.uniform(0.1, 1, (b.n_pages, kvh)).astype(F)
+    q8, qs = queries(b.rng, b.rows, heads)
+    ids = torch.full((b.rows, kvh * n_sel), 77, dtype=torch.int32, device="cuda")
+    ops.select_pages(dev(q8), dev(qs), pool, seqs, dev(hb), dev(hs), ids, n_sel)
+    mine = np.zeros(b.rows, bool)
+    mine[[r for r, _, _ in b.row_positions()]] = True
+    got = ids.cpu().numpy()
+    assert np.array_equal(got[mine], seqref.select(b, q8, qs, heads, hb, hs, n_sel)[mine]) and (got[~mine] == 77).all()
+
+
 def test_page_bounds_rows_given_or_not(cuda):
     """Row starts that do not begin at 0, with and without the call's row count."""
     b = Batch([(1, 40), (33, 31)], 2, 32, before=50)
