@@ -227,14 +227,16 @@ def sequences(pool: PagedKV, tables, row_start, kv_len, max_rows: int, max_kv: i
     n_seq = kv_len.shape[0]
     if kv_len.dim() != 1 or tables.dim() != 2 or tables.shape[0] != n_seq or row_start.shape != (n_seq + 1,):
         raise ValueError("tables are [n_seq, pages], row_start [n_seq + 1], kv_len [n_seq]")
+    index = pool.device.index
     for t in (tables, row_start, kv_len):
         if not t.is_contiguous():
             raise ValueError("tables, row_start and kv_len must be contiguous")
-        _on_device(t, pool)
+        if t.get_device() != index:
+            _on_device(t, pool)
     s = Seqs(row_start.data_ptr(), kv_len.data_ptr(), tables.data_ptr(), n_seq, tables.shape[1],
              pool.n_pages, max_rows, max_kv)
     s._keep = (tables, row_start, kv_len)
-    s.index = pool.device.index
+    s.index = index
     return s
 
 
