@@ -500,9 +500,9 @@ __device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, F
 // and 660 of matrix instructions and takes 1800 of its SIMD: what a step waits
 // beyond its issue is the barrier and the LDS reads.  Three prompts of 1700 rows, 32
 // heads on 8: 128 to 138 us from run to run, 0.37 to 0.40 of the rate of a large bf16
-// matrix product for the products that the causal mask leaves.  Matrix and vector instructions set apart by hand, a
-// wave's priority over its products, 64 keys a step, eight waves that halve the keys
-// and a third workgroup a CU (spills) were not faster.
+// matrix product for the products that the causal mask leaves.  Matrix and vector
+// instructions set apart by hand, a wave's priority over its products, 64 keys a step,
+// eight waves that halve the keys and a third workgroup a CU (spills) were not faster.
 //
 // P: where the split's V scales lie within a factor of 2^8 of each other p * vs fits
 // two f16 numbers, with a reference that puts the largest p times the largest vs at
@@ -1134,7 +1134,8 @@ void plan_splits(int64_t units, int64_t keys, int64_t want, int step, int least,
 constexpr int FEW_MOST = 16, FEW_ALL = 48;
 constexpr int64_t FEW_PAIRS = 6 << 20;
 // Workgroups to split for: equal lists of pages 1024, sequences, whose lengths differ,
-// more (64 rows at 500 .. 4000 keys 1024: 62 us, 1536: 56, 2304: 56; 92 rows' lists 49, 53, 56).
+// more (64 rows at 500 .. 4000 keys 1024: 62 us, 1536: 56, 2304: 56; 92 rows' lists 49,
+// 53, 56).  Splits of one length for all sequences, by the work of the batch: 57.
 constexpr int LIST_WANT = 1024, FEW_WANT = 1536, WIDE_WANT = 1536;
 
 struct Plan {
