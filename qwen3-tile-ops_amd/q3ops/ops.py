@@ -269,6 +269,13 @@ def _views(pool: PagedKV, tensors) -> list:
     return out
 
 
+def _heads(rows) -> int:
+    heads, rest = divmod(rows.shape[1], 128)
+    if rest:
+        raise ValueError(f"rows of {rows.shape[1]} columns are not heads of 128")
+    return heads
+
+
 def _launch_stream(pool: PagedKV, seqs: Seqs, stream) -> int:
     """The stream of a call on the pool's device, which has to be the current one
     (kernels launch there).  Sequences of another pool do as well (a layer's), if
@@ -285,7 +292,7 @@ def _launch_stream(pool: PagedKV, seqs: Seqs, stream) -> int:
     return stream.cuda_stream
 
 
-def rope_append_paged(q, k, v, pool: PagedKV, seqs: Seqs, q8=None, qs=None, nwq=None, nwk=None, inv_hd=0.0,
+def rope_append_paged(q, k, v, pool: PagedKV, seqs: Seqs, q8=None, qs=None, nwq=None, nwk=None, inv_hd=1 / 128,
                       cos=None, sin=None, rot_dim=128, interleaved=False, stream=None):
     """q3_rope_append_paged: new Q/K/V rows (f32 [rows, heads * 128]) of every
     sequence, normed (gains nwq / nwk), rotated at their positions (cos / sin
@@ -294,7 +301,7 @@ def rope_append_paged(q, k, v, pool: PagedKV, seqs: Seqs, q8=None, qs=None, nwq=
     vq, vk, vv, vnq, vnk, vc, vs, v8, vqs = _views(pool, (q, k, v, nwq, nwk, cos, sin, q8, qs))
     check(lib().q3_rope_append_paged(vq, vk, vv, vnq, vnk, inv_hd, vc, vs, rot_dim if cos is not None else 0,
                                      int(interleaved), v8, vqs, byref(pool), byref(seqs),
-                                     0 if q is None else q.shape[1] // 128, pool.kv_heads,
+                                     0 if q is None else _heads(q), pool.kv_heads,
                                      _launch_stream(pool, seqs, stream)), "rope_append_paged")
 
 
@@ -321,7 +328,7 @@ def _workspace_on(ws, stream, pool, seqs, q8, n_sel):
     """The caller's workspace tensor, or a new one (torch's allocator hands its
     memory out again in the order of the current stream)."""
     if ws is None:
-        n = seqs_workspace_bytes(pool, seqs, q8.shape[0], q8.shape[1] // 128, n_sel)
+        n = seqs_workspace_bytes(pool, seqs, q8.shape[0], _heads(q8), n_sel)
         if n == 0:
             return None, None, 0
         if stream is not None and stream != torch.cuda.current_stream(pool.device):
@@ -342,7 +349,7 @@ def attention_varlen_paged(q8, q_scale, pool: PagedKV, seqs: Seqs, out=None, o8=
     vq, vs, vo, v8, vos = _views(pool, (q8, q_scale, out, o8, os))
     st = _launch_stream(pool, seqs, stream)
     keep, ws, n = _workspace_on(workspace, stream, pool, seqs, q8, 0)
-    check(lib().q3_attention_varlen_paged(vq, vs, byref(pool), byref(seqs), vo, v8, vos, q8.shape[1] // 128,
+    check(lib().q3_attention_varlen_paged(vq, vs, byref(pool), byref(seqs), vo, v8, vos, _heads(q8),
                                           pool.kv_heads, 128, int(causal), qk_scale, ws, n, st),
           "attention_varlen_paged")
 
@@ -353,7 +360,7 @@ def select_pages(q8, q_scale, pool: PagedKV, seqs: Seqs, bounds, bscale, ids, n_
     vq, vs, vb, vbs, vi = _views(pool, (q8, q_scale, bounds, bscale, ids))
     st = _launch_stream(pool, seqs, stream)
     keep, ws, n = _workspace_on(workspace, stream, pool, seqs, q8, n_sel)
-    check(lib().q3_select_pages(vq, vs, byref(pool), byref(seqs), vb, vbs, vi, n_sel, q8.shape[1] // 128,
+    check(lib().q3_select_pages(vq, vs, byref(pool), byref(seqs), vb, vbs, vi, n_sel, _heads(q8),
                                 pool.kv_heads, ws, n, st), "select_pages")
 
 
@@ -364,7 +371,7 @@ def attention_pages(q8, q_scale, pool: PagedKV, seqs: Seqs, ids, n_sel, out=None
     vq, vs, vi, vo, v8, vos = _views(pool, (q8, q_scale, ids, out, o8, os))
     st = _launch_stream(pool, seqs, stream)
     keep, ws, n = _workspace_on(workspace, stream, pool, seqs, q8, n_sel)
-    check(lib().q3_attention_pages(vq, vs, byref(pool), byref(seqs), vi, n_sel, vo, v8, vos, q8.shape[1] // 128,
+    check(lib().q3_attention_pages(vq, vs, byref(pool), byref(seqs), vi, n_sel, vo, v8, vos, _heads(q8),
                                    pool.kv_heads, 128, qk_scale, ws, n, st), "attention_pages")
 
 

@@ -498,6 +498,19 @@ def test_append_rotations(cuda, rot, interleaved, fused):
     append_case(Batch([(7, 50), (1, 31), (1, 4000)], 2, 32, seed=rot), 4, rot, interleaved, rot % 4 == 0, fused, seed=rot)
 
 
+def test_append_norm_factor(cuda):
+    """The norm's factor is that of heads of 128 if none is given."""
+    b = Batch([(3, 30)], 2, 32)
+    x, w = torch.randn((3, 512), device="cuda"), torch.rand(128, device="cuda")
+    res = []
+    for kw in ({}, {"inv_hd": 1 / 128}):
+        pool, seqs = on_device(b)
+        q8, qs = torch.empty((3, 512), dtype=torch.int8, device="cuda"), torch.empty((3, 4), device="cuda")
+        ops.rope_append_paged(x, x[:, :256], x[:, 256:], pool, seqs, q8, qs, nwq=w, nwk=w, **kw)
+        res.append((q8, qs, *(t.nan_to_num() for t in pool._keep)))
+    assert all(torch.equal(s, t) for s, t in zip(*res))
+
+
 def test_append_bad_pages(cuda):
     b = Batch([(40, 20), (1, 64)], 2, 32)
     b.tables[0, 1] = b.n_pages
@@ -925,6 +938,11 @@ def test_refused_on_the_device(cuda):
         ops.kv_pool(*(t[:, :, ::2] for t in pool._keep))
     with pytest.raises(TypeError):
         ops.sequences(pool, seqs._keep[0].int(), *seqs._keep[1:], 1, 41)
+    wide = torch.empty((1, 520), device="cuda")
+    with pytest.raises(ValueError):
+        ops.attention_varlen_paged(wide.to(torch.int8), wide, pool, seqs, wide)
+    with pytest.raises(ValueError):
+        ops.rope_append_paged(wide, out[:, :256], out[:, :256], pool, seqs, q8, qs)
     fewer = ops.kv_pool(*(t[:-1] for t in pool._keep))  # not all pages that the tables may name
     with pytest.raises(ValueError):
         ops.attention_varlen_paged(q8, qs, fewer, seqs, out)
