@@ -519,7 +519,9 @@ constexpr int WIDE_KEYS = KB;      // of a step
 constexpr int WIDE_WAVES = 4;
 constexpr int WIDE_DEPTH = 4;      // steps whose K and V lie in LDS or on their way
 constexpr int WIDE_RING = 256;     // steps whose blocks' places lie in LDS
-constexpr int WIDE_LEAST = 512;    // keys of a split
+// Keys of a split at least: 256 rows behind 4000 keys 512: 45 us, 384: 41, 256: 39; 20
+// sequences of 1 .. 300 rows at up to 3000 keys 32, 32, 35.
+constexpr int WIDE_LEAST = 384;
 constexpr int WIDE_OROW = 32 + 4;  // floats of a column's row where the results turn
 constexpr float WIDE_ROOM = 4.0f;  // P may reach 2^4 of its reference before O is scaled down
 
@@ -546,7 +548,11 @@ __device__ __forceinline__ int wave_max(int x) {
 
 // The sequence of the unit-th tile of 128 columns, -1 behind the last, and which of
 // its tiles it is: tiles are counted 64 sequences at a time, one per lane.  *span:
-// the keys of a split, no fewer than the work for each of WIDE_SLOTS workgroups.
+// the keys of a split, no fewer than the work for each of WIDE_SLOTS workgroups and an
+// eighth, so that ragged tiles' splits are no more than the slots either: one more starts
+// only when another has ended (4 sequences of 300 rows behind 1000 keys, 32 heads on 8: 74
+// us without the eighth, a sixteenth 73, an eighth 67, a quarter 69; 2048 rows 68, 64, 60,
+// 56; 512 rows behind 16000 keys 129, 129, 135, 134).
 __device__ __forceinline__ int wide_tile(const SeqAttnArgs &a, const WidePlan &p, int unit, int *nth, int *span, SeqSpan *seq) {
   const int lane = threadIdx.x & 63;
   const int group_heads = a.heads / a.kv_heads;
@@ -585,8 +591,8 @@ __device__ __forceinline__ int wide_tile(const SeqAttnArgs &a, const WidePlan &p
   }
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) steps += __uint_as_float(lane_xor_m(__float_as_uint(steps), d));
-  const float each = steps * static_cast<float>(a.kv_heads) / WIDE_SLOTS;
-  const int even = static_cast<int>(fminf(each, static_cast<float>(1 << 25))) * WIDE_KEYS;
+  const float each = steps * static_cast<float>(a.kv_heads) * 1.125f / WIDE_SLOTS;
+  const int even = static_cast<int>(ceilf(fminf(each, static_cast<float>(1 << 25)))) * WIDE_KEYS;
   *span = __builtin_amdgcn_readfirstlane(max(split_span(found < 0 ? 0 : seq->kv, p.part.splits, WIDE_LEAST, WIDE_KEYS), even));
   return found;
 }
