@@ -1131,14 +1131,15 @@ void plan_splits(int64_t units, int64_t keys, int64_t want, int step, int least,
 // Sequences of up to FEW_MOST columns go to the kernel of 16-column tiles, and all
 // of a call do where none has more than FEW_ALL, or while rows x heads x max_kv stays
 // small: its tiles fill the CUs sooner.  us, 16-column / 128-column tiles, 16 heads on 8:
-// 32 rows behind 500 keys 11 / 29, 512 rows 20 / 26, 64 rows behind 4000 keys (4.2e6) 24
-// / 31, 1024 rows (17e6) 44 / 37, 256 rows behind 4000 keys 60 / 47, 8 x 64 rows behind
-// 1000 keys (8.7e6) 40 / 35.  8 sequences behind 4000 keys: of 16 rows (32 columns) 33 /
-// 47, 24 (48) 38 / 48, 32 (64) 45 / 48; 64 behind 2000, 64 heads on 8: of 4 rows (32)
-// 90 / 125, of 8 (64) 139 / 129.  Beside longer sequences only those of one tile: with
-// tiles for 48 columns 60 decoding rows and 4 chunks of 128 rows take 79 instead of 70.
+// 32 rows behind 500 keys 11 / 24, 512 rows (4.2e6) 18 / 26, 64 rows behind 4000 keys
+// (4.2e6) 24 / 29, 8 x 64 rows behind 1000 keys (8.7e6) 31 / 35, 1024 rows (17e6) 29 /
+// 34, 256 rows behind 4000 keys (17e6) 45 / 41.  8 sequences behind 4000 keys: of 16 rows
+// (32 columns) 32 / 47, 24 (48) 36 / 48, 32 (64) 43 / 48; 64 behind 2000, 64 heads on 8:
+// of 4 rows (32) 91 / 124, of 8 (64) 137 / 125.  Beside longer sequences only those of
+// one tile: with tiles for 48 columns 60 decoding rows and 4 chunks of 128 rows take 79
+// instead of 70.
 constexpr int FEW_MOST = 16, FEW_ALL = 48;
-constexpr int64_t FEW_PAIRS = 6 << 20;
+constexpr int64_t FEW_PAIRS = 12 << 20;
 // Workgroups to split for: equal lists of pages 1024, sequences, whose lengths differ,
 // more (64 rows at 500 .. 4000 keys 1024: 62 us, 1536: 56, 2304: 56; 92 rows' lists 49,
 // 53, 56).  Splits of one length for all sequences, by the work of the batch: 57.

@@ -92,17 +92,17 @@ def test_attention_not_causal(cuda, lens):
     check_attention(Batch(LENS[lens], 4, 32, seed=5), 8, causal=False)
 
 
-# more than 6 << 20 (row, head, key) triples: the 128-column tiles, beside 16-column
+# more than 12 << 20 (row, head, key) triples: the 128-column tiles, beside 16-column
 # ones for the sequences of few rows
 WIDE = {
-    "prompt": ([(640, 0), (1, 700)], 16, 8, 32),
-    "chunk": ([(600, 101)], 16, 8, 128),
-    "mixed": ([(1, 3000), (200, 51), (0, 5), (33, 900), (2, 40), (9, 0)], 16, 8, 32),
-    "group_of_three": ([(300, 3300), (43, 7)], 6, 2, 96),
-    "one_kv_head": ([(130, 3000), (1, 64)], 16, 1, 32),
-    "group_of_33": ([(70, 2800)], 33, 1, 64),
+    "prompt": ([(920, 0), (1, 900)], 16, 8, 32),
+    "chunk": ([(860, 101)], 16, 8, 128),
+    "mixed": ([(1, 3000), (240, 51), (0, 5), (33, 900), (2, 40), (9, 0)], 16, 8, 32),
+    "group_of_three": ([(420, 4200), (43, 7)], 6, 2, 96),
+    "one_kv_head": ([(200, 4000), (1, 64)], 16, 1, 32),
+    "group_of_33": ([(100, 4000)], 33, 1, 64),
     "negative_positions": ([(200, -150), (64, 6400), (40, -40)], 16, 2, 32),
-    "many_splits": ([(20, 9000)], 64, 2, 256),
+    "many_splits": ([(24, 9000)], 64, 2, 256),
     "no_groups": ([(700, 500), (17, 33)], 16, 16, 32),
 }
 
@@ -111,7 +111,7 @@ WIDE = {
 def test_attention_wide(cuda, name):
     lens, heads, kv_heads, page = WIDE[name]
     b = Batch(lens, kv_heads, page, seed=len(name), before=1, behind=2)
-    assert b.rows * heads * b.max_kv > 6 << 20
+    assert b.rows * heads * b.max_kv > 12 << 20
     check_attention(b, heads)
 
 
@@ -122,11 +122,11 @@ def test_attention_wide_not_causal(cuda, name):
 
 
 def test_attention_wide_bad_pages(cuda):
-    b = Batch([(300, 500), (250, 1000), (60, 1000)], 2, 32, seed=1)
+    b = Batch([(340, 500), (250, 1000), (60, 1000)], 2, 32, seed=1)
     b.tables[0, [0, 3, 24]] = [b.n_pages, 65535, b.n_pages + 7]
     b.tables[1, 4:30] = 65535
     b.tables[2] = 65535
-    assert b.rows * 16 * b.max_kv > 6 << 20
+    assert b.rows * 16 * b.max_kv > 12 << 20
     check_attention(b, 16)
 
 
@@ -134,8 +134,8 @@ def test_attention_wide_bad_pages(cuda):
 def test_attention_wide_scales(cuda, what):
     """V scales both sides of what the f16 terms take: a range of 2^8 and more, one of 2^7, zeros,
     near either end of the floats, negative; query scales of zero and below."""
-    b = Batch([(500, 300), (1, 40), (100, 700)], 2, 32, seed=3)
-    assert b.rows * 16 * b.max_kv > 6 << 20
+    b = Batch([(800, 300), (1, 40), (100, 700)], 2, 32, seed=3)
+    assert b.rows * 16 * b.max_kv > 12 << 20
     scale = {"wide": lambda u: np.exp2(np.floor(u * 9) - 4), "within": lambda u: np.exp2(np.floor(u * 7) - 3),
              "zeros": lambda u: np.where(u < 0.3, 0, 1), "tiny": lambda u: np.full_like(u, 2.0 ** -90),
              "huge": lambda u: np.full_like(u, 2.0 ** 90), "negative": lambda u: np.where(u < 0.5, -1, 1), "queries": np.ones_like}[what]
@@ -156,7 +156,7 @@ def test_attention_wide_scales(cuda, what):
 
 def test_attention_wide_strided(cuda):
     """Result rows that 16-byte words do not fit."""
-    b = Batch([(500, 300), (1, 40)], 2, 32, seed=3)
+    b = Batch([(800, 300), (1, 40)], 2, 32, seed=3)
     q8, qs = queries(b.rng, b.rows, 16)
     want, mag, top = attend(b, q8, qs, 16, QK)
     pool, seqs = on_device(b)
@@ -168,8 +168,8 @@ def test_attention_wide_strided(cuda):
 
 
 def test_attention_wide_bad_lengths(cuda):
-    b = Batch([(300, 900), (300, 500)], 2, 32, behind=4)
-    assert b.rows * 16 * b.max_kv > 6 << 20
+    b = Batch([(300, 1300), (300, 500)], 2, 32, behind=4)
+    assert b.rows * 16 * b.max_kv > 12 << 20
     q8, qs = queries(b.rng, b.rows, 16)
     want, mag, top = attend(b, q8, qs, 16, QK)
     pool, _ = on_device(b)
@@ -304,12 +304,12 @@ def test_attention_loose_limits(cuda, lens, heads, kv_heads):
     assert (np.abs(out.cpu().numpy() - want) <= attend_bound(mag, top, b.max_kv)).all()
 
 
-@pytest.mark.parametrize("lens,heads,kv_heads", [([(24, 4000)] * 8, 16, 8), ([(5, 3000), (1, 5000), (48, 700), (0, 9), (17, 0)] * 3, 8, 8),
-                                                 ([(4, 2000), (1, 3500), (6, 100)] * 4, 64, 8)])
+@pytest.mark.parametrize("lens,heads,kv_heads", [([(24, 4000)] * 10, 16, 8), ([(5, 3000), (1, 5000), (48, 700), (0, 9), (17, 0)] * 5, 8, 8),
+                                                 ([(4, 2000), (1, 3500), (6, 100)] * 6, 64, 8)])
 def test_attention_short_chunks(cuda, lens, heads, kv_heads):
     """Up to 48 columns of every sequence: 16-column tiles alone, some of them split."""
     b = Batch(lens, kv_heads, 32, seed=14)
-    assert b.rows * heads * b.max_kv > 6 << 20 and b.max_rows * heads // kv_heads <= 48
+    assert b.rows * heads * b.max_kv > 12 << 20 and b.max_rows * heads // kv_heads <= 48
     check_attention(b, heads)
 
 
@@ -318,7 +318,7 @@ def test_many_sequences(cuda, n):
     """More sequences than a wave has lanes, some without rows, rows around them all."""
     lens = [((i * 7) % 3, (i * 13) % 40) for i in range(n)]
     if n == 129:
-        lens[70] = (200, 700)  # 128-column tiles too
+        lens[70] = (2000, 700)  # 128-column tiles too
     b = Batch(lens, 2, 32, seed=n, before=3, behind=2)
     check_attention(b, 4)
     append_case(Batch(lens, 2, 32, seed=n, before=3, behind=2), 4, 64, False, True)
@@ -337,10 +337,10 @@ def test_many_sequences(cuda, n):
 def test_attention_nan(cuda, kind):
     """A NaN query, key or value scale reaches the results that it enters, whole rows of
     a head, and no other."""
-    lens, page = ([(500, 300), (1, 40), (100, 700)] if kind == "many" else [(5, 700), (1, 40), (3, 2)]), 32
+    lens, page = ([(800, 300), (1, 40), (100, 700)] if kind == "many" else [(5, 700), (1, 40), (3, 2)]), 32
     b = Batch(lens, 2, page, seed=4)
     heads = 16 if kind == "many" else 4
-    assert (b.rows * heads * b.max_kv > 6 << 20) == (kind == "many")
+    assert (b.rows * heads * b.max_kv > 12 << 20) == (kind == "many")
     q8, qs = queries(b.rng, b.rows, heads)
     n_sel = 4
     ids = np.tile(np.arange(n_sel, dtype=np.int32), (b.rows, 2))
@@ -735,12 +735,12 @@ def test_steps_together(cuda):
                 b.tables[s, (int(b.kv_len[s]) - 1) // page] = free.pop()
 
 
-@pytest.mark.parametrize("rows,context", [(1, 500), (33, 500), (200, 1600)])
+@pytest.mark.parametrize("rows,context", [(1, 500), (33, 500), (300, 1600)])
 def test_captured_and_replayed(cuda, rows, context):
     """A step captured once and replayed on other lengths, tables and rows, with
     eager calls of the same operators between the replays; two graphs that share
     a workspace, replayed in turn."""
-    heads, kvh, page, n_sel, n = 8, 4, 32, 4, 3  # (200 rows: the 128-column tiles too)
+    heads, kvh, page, n_sel, n = 8, 4, 32, 4, 3  # (300 rows: the 128-column tiles too)
     b = Batch([(rows, context)] * n, kvh, page, seed=30, smooth=True)
     pool, _ = on_device(b)
     tk, tv, tks, tvs = pool._keep
