@@ -206,23 +206,13 @@ def prepare(case, seed):
 # ---- the framework's operators ------------------------------------------------
 
 
-def _operators():
-    """The package's operator module, imported once."""
-    global _ops
-    if _ops is None:
-        pkg = str(Path.cwd() / "qwen3-tile-ops_amd")
-        if pkg not in sys.path:
-            sys.path.insert(0, pkg)
-        from q3ops import ops
-        _ops = ops
-    return _ops
-
-
-_ops = None
-
-
 def _run_own(s):
-    ops, c = _operators(), s["case"]
+    pkg = str(Path.cwd() / "qwen3-tile-ops_amd")
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
+    from q3ops import ops
+
+    c = s["case"]
     if "pool" not in s:  # the handle of the pool, made once
         s["pool"] = ops.kv_pool(s["k"], s["v"], s["ks"], s["vs"])
     pool = s["pool"]
