@@ -504,8 +504,8 @@ __device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, F
 // instructions set apart by hand, a wave's priority over its products, 64 keys a step,
 // eight waves that halve the keys and a third workgroup a CU (spills) were not faster.
 //
-// P: where the split's V scales lie within a factor of 2^8 of each other p * vs fits
-// two f16 numbers, with a reference that puts the largest p times the largest vs at
+// P: where the split's V scales lie within a factor of 2^8 of each other (none is zero,
+// or all are) p * vs fits two f16 numbers, with a reference that puts the largest p times the largest vs at
 // 2^10 .. 2^15, so the key of the largest p at 2^2 or above: 22 bits from 2^-3 up, and
 // below nothing is off by more than 2^-25, 2^-27 of that key.  Otherwise the three bf16
 // numbers of the 16-column kernel, with a third more time (three prompts of 1700 rows
@@ -676,8 +676,8 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
       lds_copy4((half ? a.pool.vs : a.pool.ks) + at.x * a.pool.spage + (at.y + n32) * a.pool.srow + kvh, lds.sc[step % (2 * WIDE_DEPTH)]);
   };
 
-  // The blocks' places, and the range of the V scales' magnitudes (as integers; zeros
-  // aside), 32 lanes a block: of the whole split, its start last, beside whose scales
+  // The blocks' places, and the range of the V scales' magnitudes (as integers), 32 lanes
+  // a block: of the whole split, its start last, beside whose scales
   // the first steps' copies are under way.
   bool missing = false;
   uint32_t most = 0, least = 0x7f800000u;
@@ -702,7 +702,7 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
       if (at.x >= 0 && first + (part + i) * KB + n32 < end) {
         const uint32_t v = __float_as_uint(a.pool.vs[at.x * a.pool.spage + (at.y + n32) * a.pool.srow + kvh]) & 0x7fffffffu;
         most = max(most, v);
-        if (v) least = min(least, v);
+        least = min(least, v);
       }
     }
     if (part == 0) break;
@@ -720,7 +720,9 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
   wait_copies<0>();
   lds_barrier();
   most = __builtin_amdgcn_readfirstlane(lds.range[0]), least = __builtin_amdgcn_readfirstlane(lds.range[1]);
-  // Narrow: within a factor of 2^8, and no closer to the ends than 2^64.
+  // Narrow: within a factor of 2^8, and no closer to the ends than 2^64, or all zeros.  A
+  // zero beside others is not: its key may have the largest score, far below which the
+  // others' products would leave f16.
   const int expo = static_cast<int>(most >> 23) - 127;
   const bool narrow = most == 0 || (expo >= -64 && expo <= 64 && least >= most - (8u << 23));
   // with p = 2^(x - base), base = the largest x less `lift`: p vs < 2^11 there
