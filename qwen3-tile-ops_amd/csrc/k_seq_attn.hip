@@ -281,10 +281,12 @@ __device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, F
   const int vmax = __builtin_amdgcn_readlane(sees, min(cols - tile * FEW_COLS, FEW_COLS) - 1);
 
   const int span_blocks = span / KB;
-  const int first = split * span_blocks;  // blocks from 0, or of the list
-  if constexpr (!LIST) {
-    if (split > 0 && first * KB >= vmax) return;  // behind the tile's last key: nobody joins this split
+  if constexpr (!LIST) {  // behind the tile's last key: nobody joins this split
+    // (64 bits: where a sequence takes fewer splits than are launched the others' starts lie
+    // at several times its length)
+    if (split > 0 && static_cast<int64_t>(split) * span >= vmax) return;
   }
+  const int first = split * span_blocks;  // blocks from 0, or of the list
 
   // Q as the B operand: column l % 16, 16 bytes of each 64-byte half
   v4i_d qf[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
