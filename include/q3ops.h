@@ -305,7 +305,9 @@ int q3_page_bounds(const q3_paged_kv *kv, const q3_seqs *seqs, uint32_t rows,
  * the row's position if causal: softmax(RN-f32 of q . k * ks * (qs * qk_scale))
  * . (vs * v) with f32 maxima, sums and products (no int8 P, unlike
  * q3_attention_heads_gqa_tokscale_paged; a key's p * vs is held to 22 bits, or
- * to 2^-27 of the largest key's).  A row without any key gets zeros.
+ * to 2^-27 of the largest key's).  A row without any key, or whose
+ * scores are all -inf, gets zeros; a score of NaN or inf, and a V scale of either,
+ * makes a head's row NaN.
  * The result goes to out f32 [rows][heads * 128], or quantised per head as by
  * q3_quant_rows_heads to o8 i8 [rows][heads * 128] / os f32 [rows][heads]; the
  * other form is NULL.  ws: device memory of q3_seqs_workspace's size, 16-byte

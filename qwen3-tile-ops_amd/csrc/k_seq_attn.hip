@@ -20,6 +20,7 @@
 // 2-norm: two numbers leave 2.3e-6, three 2e-7 at 2000 keys, where f32 sums in torch leave 6e-7;
 // one would leave 1.6e-3), V as bf16, which holds every int8.  bf16 because the
 // range of the V scales is the user's, which f16 does not hold.
+#include <cfloat>
 #include <type_traits>
 
 #include "q3_attn_v.h"
@@ -731,8 +732,9 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
   const float lift = narrow && most ? static_cast<float>(10 - expo) : 0.0f;
 
   // The softmax's reference (base 2), at most WIDE_ROOM short of the largest score
-  // less lift, so that O is scaled down a few times in all, not at every new maximum.
-  float base = -INFINITY, l = 0.0f;
+  // less lift, so that O is scaled down a few times in all, not at every new maximum.  Finite
+  // from the start: scores of -inf then have no weight, like keys that are not seen.
+  float base = -FLT_MAX, l = 0.0f;
   v16f o[4];
 #pragma unroll
   for (int t = 0; t < 4; ++t)
@@ -798,7 +800,7 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
   auto refer = [&](float top) {
     if (__ballot(top > base + WIDE_ROOM)) {
       const float to = fmaxf(top, base);
-      const float alpha = base == -INFINITY ? 0.0f : exp2_from(base, to);
+      const float alpha = exp2_from(base, to);
       l *= alpha;
 #pragma unroll
       for (int t = 0; t < 4; ++t) o[t] *= alpha;
@@ -920,7 +922,7 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
   const bool whole = tile_max <= span;
   const int64_t at = whole || !live ? 0 : ((static_cast<int64_t>(unit) * a.kv_heads + kvh) * WIDE_COLS + c - col0) * p.part.splits + split;
   if (whole) {
-    const float inv = base == -INFINITY ? 0.0f : 1.0f / l;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
     for (int t = 0; t < 4; ++t) o[t] *= inv;
   } else if (live && half == 0) {

@@ -50,3 +50,60 @@ def test_zero_values_under_the_largest_score(cuda, kind, margin):
     want, mag, top = attend(b, q8, qs, heads, qk)
     err, bound = np.abs(got - want), attend_bound(mag, top, b.max_kv)
     assert (err <= bound).all(), float((err / bound).max())
+
+
+def positive(kind, seed):
+    """Queries, keys and their scales above zero: a key's score has its scale's sign."""
+    b = Batch(KINDS[kind], 2, 32, seed=seed)
+    heads = 16 if kind == "many" else 4
+    b.k[:] = b.rng.integers(1, 128, b.k.shape)
+    q8, qs = queries(b.rng, b.rows, heads)
+    return b, heads, np.maximum(np.abs(q8), 1).astype(np.int8), qs
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("low", [-np.inf, -3e38])
+def test_scores_of_minus_infinity(cuda, kind, low):
+    """Keys whose scores are -inf (by their scale, or past the floats' range) have no
+    weight: rows that see none but such get zeros, the others what the other keys give."""
+    b, heads, q8, qs = positive(kind, 5)
+    n_sel = 20
+    ids = np.tile(np.arange(n_sel, dtype=np.int32), (b.rows, 2))
+    hidden = b.tables.copy()
+    for s, pages in ((0, range(15)), (1, range(2)), (2, range(1))):  # sequence 1: all its keys
+        for i in pages:
+            if i * 32 < b.kv_len[s]:
+                n = min(32, b.kv_len[s] - i * 32)
+                b.ks[b.tables[s, i], :n] = low
+                hidden[s, i] = 65535
+    got = run(kind, b, q8, qs, heads, ids, n_sel)
+    b.tables = hidden  # the same as pages outside the pool
+    want, mag, top = attend(b, q8, qs, heads, QK, True, ids if kind == "listed" else None, n_sel)
+    assert np.isfinite(got).all(), np.argwhere(~np.isfinite(got))[:4].tolist()
+    assert (np.abs(got - want) <= attend_bound(mag, top, b.max_kv)).all()
+    assert (got[int(b.start[1]):int(b.start[2])] == 0).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_scores_of_infinity(cuda, kind):
+    """A key whose score is inf makes the rows that see it NaN, whole rows of a head, and
+    no other; so does an infinite V scale."""
+    b, heads, q8, qs = positive(kind, 6)
+    n_sel = 4
+    ids = np.tile(np.arange(n_sel, dtype=np.int32), (b.rows, 2))
+    plain = run(kind, b, q8, qs, heads, ids, n_sel)
+    assert np.isfinite(plain).all()
+    _, mag, top = attend(b, q8, qs, heads, QK, True, ids if kind == "listed" else None, n_sel)
+    twice = 2 * attend_bound(mag, top, b.max_kv)
+    for name in ("ks", "vs"):
+        t = 33  # of sequence 0, KV head 1: the heads of the upper half
+        at = b.tables[0, t // 32], t % 32, 1
+        keep = getattr(b, name)[at]
+        getattr(b, name)[at] = np.inf
+        got, want = run(kind, b, q8, qs, heads, ids, n_sel), plain.copy()
+        getattr(b, name)[at] = keep
+        sees = [r for r, s, p in b.row_positions() if s == 0 and p >= t]
+        want[sees, heads * 64:] = np.nan
+        same = np.isnan(got) == np.isnan(want)
+        assert same.all(), (name, np.argwhere(~same)[:4].tolist())
+        assert (np.abs(got - want) <= twice)[~np.isnan(want)].all()
