@@ -20,7 +20,6 @@
 // 2-norm: two numbers leave 2.3e-6, three 2e-7 at 2000 keys, where f32 sums in torch leave 6e-7;
 // one would leave 1.6e-3), V as bf16, which holds every int8.  bf16 because the
 // range of the V scales is the user's, which f16 does not hold.
-#include <cfloat>
 #include <type_traits>
 
 #include "q3_attn_v.h"
@@ -728,13 +727,16 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
   // others' products would leave f16.
   const int expo = static_cast<int>(most >> 23) - 127;
   const bool narrow = most == 0 || (expo >= -64 && expo <= 64 && least >= most - (8u << 23));
-  // with p = 2^(x - base), base = the largest x less `lift`: p vs < 2^11 there
+  // with p = 2^(x - top + lift) p vs < 2^11 at the largest x
   const float lift = narrow && most ? static_cast<float>(10 - expo) : 0.0f;
 
-  // The softmax's reference (base 2), at most WIDE_ROOM short of the largest score
-  // less lift, so that O is scaled down a few times in all, not at every new maximum.  Finite
-  // from the start: scores of -inf then have no weight, like keys that are not seen.
-  float base = -FLT_MAX, l = 0.0f;
+  // The softmax's reference, a score but for the column's scale, at most WIDE_ROOM (base 2)
+  // short of the largest, so that O is scaled down a few times in all, not at every new
+  // maximum.  Scores are formed as their distance from it, by the FMA that multiplies by the
+  // key's scale: the largest's is then exact, however large it is (a difference of rounded
+  // products would be off by more than f16 or f32 hold from scores of 2^26 on).  room: -inf until
+  // there is a score; those of -inf never are the reference, and have no weight.
+  float ref = 0.0f, room = -INFINITY, l = 0.0f;
   v16f o[4];
 #pragma unroll
   for (int t = 0; t < 4; ++t)
@@ -761,26 +763,26 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
       kf[i] = *reinterpret_cast<const v4i_d *>(st.k[step % WIDE_DEPTH] + n32 * HD + 16 * ((2 * i + half) ^ (n32 & 7)));
   };
 
-  // Their scores but for the column's scale: register i is key 8 (i / 4) + 4 half +
-  // i % 4.  EDGE: some column does not see some key, or has a negative scale; `seen`
-  // keeps which, since nothing of that key may enter the sums, not even a scale's NaN.  Returns the
-  // column's largest score in base 2, less lift.
+  // Their scores' distances from ref, but for the column's scale: register i is key
+  // 8 (i / 4) + 4 half + i % 4.  EDGE: some column does not see some key, or has a negative
+  // scale; `seen` keeps which, since nothing of that key may enter the sums, not even a
+  // scale's NaN.  Returns the column's largest.
   float x[16];
   uint32_t seen = ~0u;
   auto scores = [&](int step, const v16i &s, auto edge_tag) {
     constexpr bool EDGE = decltype(edge_tag)::value;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const v4f ks = *reinterpret_cast<const v4f *>(lds.sc[step % (2 * WIDE_DEPTH)] + 8 * i + 4 * half);
+      v4f ks = *reinterpret_cast<const v4f *>(lds.sc[step % (2 * WIDE_DEPTH)] + 8 * i + 4 * half);
+      if constexpr (EDGE) {
+        if (turned) ks *= sign;
+      }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[4 * i + j] = (__int_as_float(s[4 * i + j]) - __int_as_float(kOnTop)) * ks[j];
+      for (int j = 0; j < 4; ++j)
+        x[4 * i + j] = __builtin_fmaf(__int_as_float(s[4 * i + j]) - __int_as_float(kOnTop), ks[j], -ref);
     }
     seen = ~0u;
     if constexpr (EDGE) {
-      if (turned) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] *= sign;
-      }
       seen = 0;
       const int limit = lds.block[step % WIDE_RING].x < 0 ? 0 : sees - (first + step * WIDE_KEYS + 4 * half);
 #pragma unroll
@@ -794,17 +796,20 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
 #pragma unroll
     for (int i = 1; i < 16; ++i) mb = fmaxf(mb, x[i]);
     const LanePair pr = lane_pair32(__float_as_uint(mb));
-    mb = fmaxf(__uint_as_float(pr.a), __uint_as_float(pr.b));
-    return mb == -INFINITY ? -INFINITY : mb * size - lift;
+    return fmaxf(__uint_as_float(pr.a), __uint_as_float(pr.b));
   };
   auto refer = [&](float top) {
-    if (__ballot(top > base + WIDE_ROOM)) {
-      const float to = fmaxf(top, base);
-      const float alpha = exp2_from(base, to);
+    const bool up = top > -INFINITY && !(top * size <= room);
+    if (__ballot(up)) {
+      const float by = up ? top : 0.0f;
+      const float alpha = room < 0.0f ? 0.0f : __builtin_amdgcn_exp2f(-by * size);
       l *= alpha;
 #pragma unroll
       for (int t = 0; t < 4; ++t) o[t] *= alpha;
-      base = to;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] -= by;
+      ref += by;
+      if (up) room = WIDE_ROOM;
     }
   };
 
@@ -817,7 +822,7 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
     float e[8], pv[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * r + j], size, -base));
+      e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * r + j], size, lift));
       const bool in = !EDGE || (seen >> (8 * r + j) & 1);
       if (!in) e[j] = 0.0f;
       pv[j] = e[j] * (j < 4 ? va[j] : vc[j - 4]);
@@ -921,13 +926,11 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
   }
   const bool whole = tile_max <= span;
   const int64_t at = whole || !live ? 0 : ((static_cast<int64_t>(unit) * a.kv_heads + kvh) * WIDE_COLS + c - col0) * p.part.splits + split;
-  if (whole) {
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  // (a partial result without its lift, a power of two that the other splits do not share)
+  const float inv = !whole ? __builtin_amdgcn_exp2f(-lift) : l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) o[t] *= inv;
-  } else if (live && half == 0) {
-    p.part.ml[at] = make_float2(base, l);
-  }
+  for (int t = 0; t < 4; ++t) o[t] *= inv;
+  if (!whole && live && half == 0) p.part.ml[at] = make_float2(room < 0.0f ? -INFINITY : ref * size, l * inv);
   if (whole && a.o8) {
     float pk = 0.0f;
 #pragma unroll

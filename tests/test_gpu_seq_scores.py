@@ -107,3 +107,30 @@ def test_scores_of_infinity(cuda, kind):
         same = np.isnan(got) == np.isnan(want)
         assert same.all(), (name, np.argwhere(~same)[:4].tolist())
         assert (np.abs(got - want) <= twice)[~np.isnan(want)].all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("size", [2.0 ** 18, 2.0 ** 24, 2.0 ** 27, 2.0 ** 32, 2.0 ** 60])
+def test_huge_scores(cuda, kind, size):
+    """Scores of millions and more: one key has all the weight of a row where the next
+    largest score lies further below than f32 roundings of both can move them."""
+    b, heads, q8, qs = positive(kind, 7)
+    b.ks *= F(size)
+    n_sel = 20
+    ids = np.tile(np.arange(n_sel, dtype=np.int32), (b.rows, 2))
+    got = run(kind, b, q8, qs, heads, ids, n_sel).reshape(b.rows, heads, 128)
+    assert np.isfinite(got).all()
+    checked = 0
+    for row, s, pos in b.row_positions():
+        for h in range(heads):
+            k, v, _ = b.keys(s, h // (heads // 2), np.arange(min(pos + 1, n_sel * 32) if kind == "listed" else pos + 1))
+            x = (k @ q8[row, h * 128:(h + 1) * 128].astype(np.float64)) * float(qs[row, h]) * QK
+            first = int(np.argmax(x))
+            # a score and its distance from the largest: ten roundings of 2^-24 each; e^-30 is none of the weight
+            if len(x) > 1 and x[first] - np.partition(x, -2)[-2] < 20 * 2.0 ** -24 * x[first] + 30:
+                continue
+            checked += 1
+            # the weight's products, P's terms (2^-22 each) and the division; 1100 other keys
+            # at most, of e^-30 and 127 * 0.03
+            assert (np.abs(got[row, h] - v[first]) <= 2.0 ** -20 * np.abs(v[first]) + 4e-10).all(), (row, h)
+    assert checked > b.rows * heads // 2
