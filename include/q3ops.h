@@ -343,9 +343,12 @@ int q3_attention_pages(const q3_view *q8, const q3_view *q_scale,
                        uint64_t ws_bytes, void *stream);
 
 /* Bytes of workspace that q3_attention_varlen_paged and, with n_sel > 0,
- * q3_select_pages and q3_attention_pages need for calls of these sizes: one
- * buffer serves them all in stream order.  Host only; of seqs the counts and
- * limits are read, not the arrays. */
+ * q3_select_pages and q3_attention_pages need for any calls whose rows, n_sel and
+ * seqs' n_seq, max_rows and max_kv are at most these (heads, kv_heads and
+ * page_tokens being these): one buffer, sized once for a serving loop's largest
+ * counts, serves them all in stream order.  At most 154 MB, or 4 bytes a row, KV head and
+ * logical page of max_kv for the selection's scores if that is more.  Host only; of seqs
+ * the counts and limits are read, not the arrays. */
 int q3_seqs_workspace(const q3_seqs *seqs, uint32_t rows, uint32_t page_tokens,
                       int heads, int kv_heads, uint32_t n_sel, uint64_t *bytes);
 

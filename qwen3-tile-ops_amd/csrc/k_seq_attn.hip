@@ -20,6 +20,7 @@
 // 2-norm: two numbers leave 2.3e-6, three 2e-7 at 2000 keys, where f32 sums in torch leave 6e-7;
 // one would leave 1.6e-3), V as bf16, which holds every int8.  bf16 because the
 // range of the V scales is the user's, which f16 does not hold.
+#include <algorithm>
 #include <type_traits>
 
 #include "q3_attn_v.h"
@@ -216,6 +217,7 @@ struct FewPlan {
   int tiles;
   int most;       // columns of a sequence that are taken here
   int each;       // workgroups of a sequence and KV head to aim at
+  int by_row;     // slots lie by (row, head) in memory: fewer, where row counts are far from equal
 };
 
 // The keys of a split of a sequence, whose tiles share its part of the workgroups (so a
@@ -472,8 +474,8 @@ __device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, F
     store_row8(a, jrow, jhead, d0, r);
     return;
   }
-  const int64_t slot = LIST ? static_cast<int64_t>(jrow) * a.heads + jhead
-                            : (static_cast<int64_t>(seq) * a.kv_heads + kvh) * p.most + cc;
+  const int64_t slot = LIST || p.by_row ? static_cast<int64_t>(jrow) * a.heads + jhead
+                                : (static_cast<int64_t>(seq) * a.kv_heads + kvh) * p.most + cc;
   const int64_t at = slot * p.part.splits + split;
   v4f *dst = reinterpret_cast<v4f *>(p.part.o + at * HD + d0);
   dst[0] = v4f{r[0], r[1], r[2], r[3]};
@@ -1044,7 +1046,11 @@ __device__ void join_slots(const SeqAttnArgs &a, const Plan &plan, int cell_cols
     const int sees = a.causal ? max(sp.pos(row) + 1, 0) : sp.kv;
     n = (sees + span - 1) / span;
   }
-  const int64_t at = (static_cast<int64_t>(cell) * cell_cols + c) * p.splits;
+  int64_t slot = static_cast<int64_t>(cell) * cell_cols + c;
+  if constexpr (!WIDE) {
+    if (plan.by_row) slot = static_cast<int64_t>(row) * a.heads + head;
+  }
+  const int64_t at = slot * p.splits;
   float top = -INFINITY;
   for (int s = threadIdx.x & 15; s < n; s += 16) top = fmaxf(top, p.ml[at + s].x);
   top = fmaxf(top, lane_xor<1>(top));
@@ -1158,6 +1164,7 @@ struct Plan {
   FewPlan few;
   WidePlan wide;
   bool any_wide;
+  int64_t few_held, wide_held;  // partial results
 };
 
 Plan plan_attn(const SeqAttnArgs &a) {
@@ -1173,32 +1180,64 @@ Plan plan_attn(const SeqAttnArgs &a) {
   p.few.each = static_cast<int>(cdiv(FEW_WANT, (n_seq < 1 ? 1 : n_seq) * a.kv_heads));
   plan_splits((a.ids ? p.few.units : n_seq) * a.kv_heads, a.ids ? int64_t(a.n_sel) * a.pool.page_tokens : a.seqs.max_kv,
               a.ids ? LIST_WANT : FEW_WANT, FEW_STEP, FEW_LEAST, p.few.part);
-  if (p.few.part.splits > 1) p.few.part.slots = a.ids ? rows * a.heads : n_seq * a.kv_heads * few_cols;
+  const int64_t by_row = rows * a.heads, by_col = n_seq * a.kv_heads * few_cols;
+  p.few.by_row = !a.ids && by_row < by_col;
+  if (p.few.part.splits > 1) {
+    p.few.part.slots = a.ids ? by_row : by_col;
+    p.few_held = std::min(p.few.part.slots, by_row) * p.few.part.splits;
+  }
   if (p.any_wide) {
     p.wide.least = FEW_MOST + 1;
     const int64_t wide_seqs = rows * g / p.wide.least;
     p.wide.tiles = rows * g / WIDE_COLS + (n_seq < wide_seqs ? n_seq : wide_seqs);
     plan_splits(p.wide.tiles * a.kv_heads, a.seqs.max_kv, WIDE_WANT, WIDE_KEYS, WIDE_LEAST, p.wide.part);
     if (p.wide.part.splits > 1) p.wide.part.slots = p.wide.tiles * a.kv_heads * WIDE_COLS;
+    p.wide_held = p.wide.part.slots * p.wide.part.splits;
   }
   return p;
 }
 
-int64_t partials(const Partials &p) { return p.slots * p.splits; }
+// The most that units x splits of plan_splits comes to, for up to so many units and keys
+// (0: no call of these sizes is split).
+int64_t most_splits(int64_t units, int64_t keys, int64_t want, int least) {
+  return keys <= least ? 0 : std::min(want, units * std::min<int64_t>(64, cdiv(keys, least)));
+}
+
+// The most partial results of any call whose counts are at most these.  Splits fall as
+// units grow, so a call's own number rises and falls with its counts.
+int64_t most_partials(const SeqAttnArgs &a) {
+  const int64_t g = a.heads / a.kv_heads, rows = a.seqs.rows, n_seq = a.seqs.n_seq;
+  if (a.ids) {  // units x splits x (heads of a tile)
+    const int64_t tiles = cdiv(g, FEW_COLS);
+    return cdiv(most_splits(rows * tiles * a.kv_heads, int64_t(a.n_sel) * a.pool.page_tokens, LIST_WANT, FEW_LEAST) * g, tiles);
+  }
+  const int64_t cols = std::max<int64_t>(1, a.seqs.max_rows * g), keys = a.seqs.max_kv;
+  int64_t few = most_splits(n_seq * a.kv_heads, keys, FEW_WANT, FEW_LEAST) * std::min<int64_t>(cols, FEW_ALL);
+  // Small calls of more columns, (row, head) slots at most: of more than FEW_LEAST keys, at
+  // most FEW_PAIRS / keys of them, each of at most 2 keys / FEW_LEAST splits.
+  if (cols > FEW_ALL && few > 0) few = std::max(few, 2 * FEW_PAIRS / FEW_LEAST);
+  few = std::min(few, most_splits(rows * a.heads, keys, INT64_MAX, FEW_LEAST));
+  const Plan p = plan_attn(a);  // (a call that is small, or of few columns, has none larger below it)
+  return few + (p.any_wide ? most_splits(p.wide.tiles * a.kv_heads, keys, WIDE_WANT, WIDE_LEAST) * WIDE_COLS : 0);
+}
+
+constexpr uint64_t kPartialBytes = HD * 4 + 8;
 
 }  // namespace
 
 uint64_t seq_attn_ws_bytes(const SeqAttnArgs &a) {
   const Plan p = plan_attn(a);
-  return static_cast<uint64_t>(partials(p.few.part) + partials(p.wide.part)) * (HD * 4 + 8);
+  return static_cast<uint64_t>(p.few_held + p.wide_held) * kPartialBytes;
 }
+
+uint64_t seq_attn_ws_most(const SeqAttnArgs &a) { return static_cast<uint64_t>(most_partials(a)) * kPartialBytes; }
 
 hipError_t launch_seq_attn(const SeqAttnArgs &args, hipStream_t s) {
   if (args.seqs.rows == 0 || args.seqs.n_seq == 0) return hipSuccess;
   SeqAttnArgs a = args;
   a.out_words = a.out && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && (a.ldo & 3) == 0;
   Plan p = plan_attn(a);
-  const int64_t nf = partials(p.few.part), nw = partials(p.wide.part);
+  const int64_t nf = p.few_held, nw = p.wide_held;
   p.few.part.o = static_cast<float *>(a.ws);
   p.wide.part.o = p.few.part.o + nf * HD;
   p.few.part.ml = reinterpret_cast<float2 *>(p.wide.part.o + nw * HD);

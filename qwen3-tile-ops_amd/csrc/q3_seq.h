@@ -188,7 +188,8 @@ struct SeqAttnArgs {
   Pool pool;
   Seqs seqs;
 };
-uint64_t seq_attn_ws_bytes(const SeqAttnArgs &a);
+uint64_t seq_attn_ws_bytes(const SeqAttnArgs &a);  // this call's
+uint64_t seq_attn_ws_most(const SeqAttnArgs &a);   // any call's of at most these counts
 hipError_t launch_seq_attn(const SeqAttnArgs &a, hipStream_t s);
 
 // ---- page selection (k_seq_select.hip) ----------------------------------------

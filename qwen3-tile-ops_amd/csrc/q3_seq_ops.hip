@@ -294,14 +294,14 @@ int q3_seqs_workspace(const q3_seqs *seqs, uint32_t rows, uint32_t page_tokens, 
   a.seqs.rows = static_cast<int>(rows);
   a.seqs.max_rows = static_cast<int>(seqs->max_rows);
   a.seqs.max_kv = static_cast<int>(seqs->max_kv);
-  uint64_t need = q3::seq_attn_ws_bytes(a);
+  uint64_t need = q3::seq_attn_ws_most(a);
   if (n_sel) {
     const int32_t any = 0;
     a.ids = &any;  // only its presence counts
     a.n_sel = static_cast<int>(n_sel);
-    const uint64_t pages = q3::seq_attn_ws_bytes(a);
+    const uint64_t pages = q3::seq_attn_ws_most(a);
     const int64_t ld_keys = score_ld(seqs, page_tokens);
-    const uint64_t scores = ld_keys > n_sel ? 4ull * rows * kv_heads * ld_keys : 0;
+    const uint64_t scores = ld_keys > 1 ? 4ull * rows * kv_heads * ld_keys : 0;
     need = need > pages ? need : pages;
     need = need > scores ? need : scores;
   }
