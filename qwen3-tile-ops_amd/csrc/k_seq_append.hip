@@ -64,7 +64,7 @@ __device__ __forceinline__ float ordered_sum4(float s, int lane) {
 // VEC: x rows may be read as 16-byte words; angles: so may a lane's angles (and its
 // four columns are rotated alike).
 template <bool VEC, int ROWS>
-__global__ void __launch_bounds__(256, 8) seq_append_kernel(SeqAppendArgs a, int groups, bool angles) {
+__global__ void __launch_bounds__(256, 8) seq_append_kernel(SeqAppendArgs a, bool angles) {
   __shared__ __align__(16) float ex[8][HD];
   const int lane = threadIdx.x & 63, wave = wave_id();
   const int row_blocks = (a.seqs.rows + ROWS - 1) / ROWS;
@@ -301,11 +301,11 @@ hipError_t launch_seq_append(const SeqAppendArgs &a, hipStream_t s) {
   if (wgs > INT32_MAX / 256) return hipErrorInvalidValue;
   const dim3 grid(static_cast<unsigned>(wgs));
   if (two)
-    hipLaunchKernelGGL((seq_append_kernel<true, 2>), grid, dim3(256), 0, s, a, groups, angles);
+    hipLaunchKernelGGL((seq_append_kernel<true, 2>), grid, dim3(256), 0, s, a, angles);
   else if (vec)
-    hipLaunchKernelGGL((seq_append_kernel<true, 1>), grid, dim3(256), 0, s, a, groups, angles);
+    hipLaunchKernelGGL((seq_append_kernel<true, 1>), grid, dim3(256), 0, s, a, angles);
   else
-    hipLaunchKernelGGL((seq_append_kernel<false, 1>), grid, dim3(256), 0, s, a, groups, angles);
+    hipLaunchKernelGGL((seq_append_kernel<false, 1>), grid, dim3(256), 0, s, a, angles);
   return hipGetLastError();
 }
 

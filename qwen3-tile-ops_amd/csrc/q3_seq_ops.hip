@@ -12,7 +12,6 @@ using q3::check_vec;
 using q3::check_view;
 using q3::hip_status;
 using q3::ld;
-using q3::no_data;
 using q3::unsupported;
 
 constexpr uint32_t kMaxTokens = 1u << 30;  // positions are 32-bit on the device
