@@ -255,13 +255,16 @@ int q3_argmax_logits(const q3_view *logits, int32_t *out_id, void *stream);
  * by the kernels alone, so a call may be captured into a graph and replayed on
  * other lengths, within max_rows and max_kv.  Rows before row_start[0] and from
  * row_start[n_seq] on are left as they are.  What the arrays may hold wrongly is
- * clamped: a sequence's rows to max_rows, kv_len to [0, max_kv] (limits well
- * above the lengths cost little time, but workspace); a page id
+ * clamped: a sequence's rows to max_rows, kv_len to [0, max_kv]; a page id
  * outside the pool is a page whose keys are never attended to or written.
  * row_start must not decrease.  At most 2^21 rows, 512 heads and max_kv 2^30
  * (Q3_ERR_RANGE / Q3_ERR_ARG), and no more work than one launch's grid holds
- * (Q3_ERR_HIP).  The same call gives the same bits; a row's last bits may hang on
- * what else the batch holds. */
+ * (Q3_ERR_HIP).  A max_kv well above the lengths costs little time but for the
+ * attention of a small call in which a sequence may have more than 48 (row, query
+ * head) pairs to a KV head: whether it is small goes by rows * heads * max_kv, and
+ * otherwise it takes up to 2.4 times as long (32 rows behind 500 keys: 11 us with a
+ * max_kv of 532, 26 with 131072).  The same call gives the same bits; a row's last
+ * bits may hang on what else the batch holds. */
 typedef struct q3_seqs {
   const int32_t *row_start; /* device [n_seq + 1]                            */
   const int32_t *kv_len;    /* device [n_seq]: cached tokens, new ones included */
@@ -305,7 +308,8 @@ int q3_page_bounds(const q3_paged_kv *kv, const q3_seqs *seqs, uint32_t rows,
  * the row's position if causal: softmax(RN-f32 of q . k * ks * (qs * qk_scale))
  * . (vs * v) with f32 maxima, sums and products (no int8 P, unlike
  * q3_attention_heads_gqa_tokscale_paged; a key's p * vs is held to 22 bits, or
- * to 2^-27 of the largest key's).  A row without any key, or whose
+ * to 2^-27 of the largest key's, so n keys' sum to n * 2^-27 of it at worst, an eighth
+ * of what f32 sums of n terms may lose).  A row without any key, or whose
  * scores are all -inf, gets zeros; a score of NaN or inf, and a V scale of either,
  * makes a head's row NaN.
  * The result goes to out f32 [rows][heads * 128], or quantised per head as by

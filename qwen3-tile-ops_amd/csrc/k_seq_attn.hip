@@ -208,7 +208,11 @@ constexpr int FEW_V = 0, FEW_S = KB * HD, FEW_STAGE = KB * HD + 2 * KB * 4;
 constexpr int FEW_K = FEW_STAGES * FEW_STAGE, FEW_WAVE = FEW_K + KB * HD;  // bytes of a wave
 constexpr int FEW_ROW = HD + 4;  // floats of a column's row where the waves join
 constexpr int FEW_BLOCKS = 64 * FEW_WAVES;  // named at a time, one by a lane of each wave
-constexpr int FEW_STEP = KB * FEW_WAVES, FEW_LEAST = 256;  // keys of a split: a multiple, at least
+// Keys of a split: a multiple of FEW_STEP, FEW_LEAST at least.  us with 128, 256, 512 and 1024
+// at least, with the join: one row at 543 keys 9.6, 10.8, 12.5, 10.2, at 2000 9.8, 11.0, 12.6, 17.3, at
+// 8000 13.7, 12.3, 13.5, 17.6; 24 sequences of 3 rows behind 1000 keys 23, 18, 20, 16; 64 rows
+// at 500 .. 4000 keys 66.8, 66.8, 67.0, 68.5, at 300 20, 18, 13, 12.
+constexpr int FEW_STEP = KB * FEW_WAVES, FEW_LEAST = 256;
 static_assert(FEW_WAVES * FEW_COLS * FEW_ROW * 4 <= FEW_WAVES * FEW_WAVE, "the join fits the stages");
 
 struct FewPlan {
@@ -221,7 +225,9 @@ struct FewPlan {
 };
 
 // The keys of a split of a sequence, whose tiles share its part of the workgroups (so a
-// decoding row beside short chunks is split as finely as among its like).
+// decoding row beside short chunks is split as finely as among its like).  The part is the
+// same for every sequence: one row at 131072 keys among 63 at 500 gets 3 splits a KV head,
+// of 64 launched for it alone, and takes 713 us instead of 60.
 __device__ __forceinline__ int few_span(const FewPlan &p, int keys, int cols) {
   const int tiles = (cols + FEW_COLS - 1) / FEW_COLS;
   return split_span(keys, clampi(p.each / max(tiles, 1), 1, p.part.splits), FEW_LEAST, FEW_STEP);
@@ -511,9 +517,10 @@ __device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, F
 // P: where the split's V scales lie within a factor of 2^8 of each other (none is zero,
 // or all are) p * vs fits two f16 numbers, with a reference that puts the largest p times the largest vs at
 // 2^10 .. 2^15, so the key of the largest p at 2^2 or above: 22 bits from 2^-3 up, and
-// below nothing is off by more than 2^-25, 2^-27 of that key.  Otherwise the three bf16
+// below nothing is off by more than 2^-25, 2^-27 of that key (n such keys by n 2^-27 in all;
+// sums of n f32 numbers may be off by n 2^-24).  Otherwise the three bf16
 // numbers of the 16-column kernel, with a third more time (three prompts of 1700 rows
-// 170 us).
+// 201 us instead of 150, captured, where int8 results take 142).
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef int v16i __attribute__((ext_vector_type(16)));
 

@@ -317,7 +317,7 @@ def page_bounds(pool: PagedKV, seqs: Seqs, bounds, bscale, rows: int | None = No
 
 def seqs_workspace_bytes(pool: PagedKV, seqs: Seqs, rows: int, heads: int, n_sel: int = 0) -> int:
     """q3_seqs_workspace: bytes for attention_varlen_paged and, with n_sel,
-    select_pages and attention_pages on these sizes."""
+    select_pages and attention_pages on these sizes, and on any smaller ones."""
     n = C.c_uint64()
     check(lib().q3_seqs_workspace(byref(seqs), rows, pool.page_tokens, heads, pool.kv_heads, n_sel, byref(n)),
           "seqs_workspace")

@@ -2,7 +2,8 @@
 
 Angles are computed in float64 and rounded once to float32, as
 tools/convert_pqwf.py:46-52 does for the plain tables; the context-extension
-scalings below are the published ones.
+scalings are position interpolation (linear), NTK-aware base scaling (ntk) and
+YaRN's interpolation by parts with its attention factor (yarn).
 """
 from __future__ import annotations
 
@@ -14,7 +15,7 @@ __all__ = ["rope_tables"]
 
 
 def _yarn_ramp(half: int, theta: float, original: int, beta_fast: float, beta_slow: float) -> np.ndarray:
-    """1 where a dimension turns more than beta_fast times over the original
+    """YaRN's ramp: 1 where a dimension turns more than beta_fast times over the original
     context (left as it is), 0 where less than beta_slow times (interpolated),
     linear in the dimension's index between."""
     def dim(turns: float) -> float:
