@@ -40,8 +40,8 @@ def rope_tables(positions: int, rot_dim: int = 128, theta: float = 1e6, scaling:
     attention_factor (0.1 ln factor + 1 if not given)."""
     if rot_dim <= 0 or rot_dim > 128 or rot_dim % 2:
         raise ValueError("rot_dim is even, from 2 to 128")
-    if positions < 0 or theta <= 0 or factor < 1.0:
-        raise ValueError("positions >= 0, theta > 0 and factor >= 1")
+    if positions < 0 or not 0 < theta < math.inf or not 1.0 <= factor < math.inf:
+        raise ValueError("positions >= 0, theta > 0 and factor >= 1, both finite")
     half = rot_dim // 2
     i = np.arange(half, dtype=np.float64)
     scale = 1.0
@@ -53,8 +53,10 @@ def rope_tables(positions: int, rot_dim: int = 128, theta: float = 1e6, scaling:
     if scaling == "linear":
         f = f / factor
     elif scaling == "yarn":
-        if original <= 0 or theta == 1.0:
-            raise ValueError("yarn scaling needs the original context length and theta != 1")
+        if original <= 0 or theta <= 1.0 or not 0 < beta_slow <= beta_fast < math.inf:
+            raise ValueError("yarn scaling needs the original context length, theta > 1 and beta_fast >= beta_slow > 0")
+        if attention_factor is not None and not math.isfinite(attention_factor):
+            raise ValueError("attention_factor must be finite")
         keep = _yarn_ramp(half, theta, original, beta_fast, beta_slow)
         f = f * keep + f / factor * (1.0 - keep)
         scale = 0.1 * math.log(factor) + 1.0 if attention_factor is None else attention_factor
