@@ -520,7 +520,7 @@ __device__ void few_columns(const SeqAttnArgs &a, const FewPlan &p, int block, F
 // below nothing is off by more than 2^-25, 2^-27 of that key (n such keys by n 2^-27 in all;
 // sums of n f32 numbers may be off by n 2^-24).  Otherwise the three bf16
 // numbers of the 16-column kernel, with a third more time (three prompts of 1700 rows
-// 201 us instead of 150, captured, where int8 results take 142).
+// 207 us instead of 151, captured, where int8 results take 144).
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef int v16i __attribute__((ext_vector_type(16)));
 
@@ -741,11 +741,14 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
 
   // The softmax's reference, a score but for the column's scale, at most WIDE_ROOM (base 2)
   // short of the largest, so that O is scaled down a few times in all, not at every new
-  // maximum.  Scores are formed as their distance from it, by the FMA that multiplies by the
-  // key's scale: the largest's is then exact, however large it is (a difference of rounded
-  // products would be off by more than f16 or f32 hold from scores of 2^26 on).  room: -inf until
-  // there is a score; those of -inf never are the reference, and have no weight.
-  float ref = 0.0f, room = -INFINITY, l = 0.0f;
+  // maximum.  Exponents are (x - ref) * size + lift: the reference's own is exactly lift,
+  // however large it is.  While no reference of the wave is beyond 2^10 (`far`) x * size + add
+  // is as good and an instruction less (three prompts of 1700 rows 134.5 us without it, 131.3
+  // with); add's rounding at 2^26 would be more than f16 has room for.
+  // room: the exponent at which ref moves, -inf until there is a score; those of -inf never are
+  // the reference, and have no weight.
+  float ref = 0.0f, room = -INFINITY, add = lift, l = 0.0f;
+  bool far = false;
   v16f o[4];
 #pragma unroll
   for (int t = 0; t < 4; ++t)
@@ -772,10 +775,10 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
       kf[i] = *reinterpret_cast<const v4i_d *>(st.k[step % WIDE_DEPTH] + n32 * HD + 16 * ((2 * i + half) ^ (n32 & 7)));
   };
 
-  // Their scores' distances from ref, but for the column's scale: register i is key
-  // 8 (i / 4) + 4 half + i % 4.  EDGE: some column does not see some key, or has a negative
-  // scale; `seen` keeps which, since nothing of that key may enter the sums, not even a
-  // scale's NaN.  Returns the column's largest.
+  // Their scores but for the column's scale: register i is key 8 (i / 4) + 4 half +
+  // i % 4.  EDGE: some column does not see some key, or has a negative scale; `seen`
+  // keeps which, since nothing of that key may enter the sums, not even a scale's NaN.  Returns the
+  // column's largest.
   float x[16];
   uint32_t seen = ~0u;
   auto scores = [&](int step, const v16i &s, auto edge_tag) {
@@ -787,8 +790,7 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
         if (turned) ks *= sign;
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        x[4 * i + j] = __builtin_fmaf(__int_as_float(s[4 * i + j]) - __int_as_float(kOnTop), ks[j], -ref);
+      for (int j = 0; j < 4; ++j) x[4 * i + j] = (__int_as_float(s[4 * i + j]) - __int_as_float(kOnTop)) * ks[j];
     }
     seen = ~0u;
     if constexpr (EDGE) {
@@ -807,18 +809,21 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
     const LanePair pr = lane_pair32(__float_as_uint(mb));
     return fmaxf(__uint_as_float(pr.a), __uint_as_float(pr.b));
   };
-  auto refer = [&](float top) {
-    const bool up = top > -INFINITY && !(top * size <= room);
+  auto exponent = [&](float score, auto edge_tag) {
+    return decltype(edge_tag)::value ? __builtin_fmaf(score - ref, size, lift) : __builtin_fmaf(score, size, add);
+  };
+  auto refer = [&](float top, auto edge_tag) {
+    const bool up = top > -INFINITY && !(exponent(top, edge_tag) <= room);
     if (__ballot(up)) {
-      const float by = up ? top : 0.0f;
-      const float alpha = room < 0.0f ? 0.0f : __builtin_amdgcn_exp2f(-by * size);
+      const float to = up ? top : ref;
+      const float alpha = room == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((ref - to) * size);
       l *= alpha;
 #pragma unroll
       for (int t = 0; t < 4; ++t) o[t] *= alpha;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] -= by;
-      ref += by;
-      if (up) room = WIDE_ROOM;
+      ref = to;
+      add = __builtin_fmaf(-ref, size, lift);
+      far = __ballot(!(fabsf(add) < 0x1p+10f)) != 0;
+      if (up) room = lift + WIDE_ROOM;
     }
   };
 
@@ -831,7 +836,7 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
     float e[8], pv[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * r + j], size, lift));
+      e[j] = __builtin_amdgcn_exp2f(exponent(x[8 * r + j], edge_tag));
       const bool in = !EDGE || (seen >> (8 * r + j) & 1);
       if (!in) e[j] = 0.0f;
       pv[j] = e[j] * (j < 4 ? va[j] : vc[j - 4]);
@@ -880,6 +885,7 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
   int step = 0;
   auto run = [&](int to, auto edge_tag, auto narrow_tag) {
     for (; step < to; ++step) {
+      if (!decltype(edge_tag)::value && far) break;  // (to the other loop)
       if (step % (WIDE_RING / 2) == 0 && step > 0) {  // the places after the next, over those gone by
         const int next = step + WIDE_RING / 2 + tid;
         if (tid < WIDE_RING / 2 && next < steps) lds.block[next % WIDE_RING] = place(next);
@@ -895,7 +901,7 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
       values(step, 0, p0);
       if (more) turn(step + 1, narrow_tag);
       values(step, 1, p1);
-      if (more) refer(scores(step + 1, s, edge_tag));
+      if (more) refer(scores(step + 1, s, edge_tag), edge_tag);
       // the step after next is needed now; those behind it may be on their way, as
       // many copies as a wave issues for them (fewer where a page is missing)
       if (missing || step + WIDE_DEPTH >= steps)
@@ -913,10 +919,10 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
     v4i_d kf[4];
     keys_of(0, kf);
     products(kf, s);
-    refer(scores(0, s, std::true_type{}));
+    refer(scores(0, s, std::true_type{}), std::true_type{});
     lds_barrier();
     // Steps that every column sees whole, then the others (all, where a page is
-    // missing or a scale negative): two loops, since one with both forms of a step
+    // missing, a scale negative or a score far from 0): two loops, since one with both forms of a step
     // keeps O twice.
     if constexpr (decltype(narrow_tag)::value)
       run(missing || turned ? 0 : clampi((tile_min - first) / WIDE_KEYS, 0, steps) - 1, std::false_type{}, narrow_tag);
@@ -939,7 +945,7 @@ __device__ void wide_columns(const SeqAttnArgs &a, const WidePlan &p, int block,
   const float inv = !whole ? __builtin_amdgcn_exp2f(-lift) : l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
   for (int t = 0; t < 4; ++t) o[t] *= inv;
-  if (!whole && live && half == 0) p.part.ml[at] = make_float2(room < 0.0f ? -INFINITY : ref * size, l * inv);
+  if (!whole && live && half == 0) p.part.ml[at] = make_float2(room == -INFINITY ? -INFINITY : ref * size, l * inv);
   if (whole && a.o8) {
     float pk = 0.0f;
 #pragma unroll

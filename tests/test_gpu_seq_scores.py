@@ -134,3 +134,37 @@ def test_huge_scores(cuda, kind, size):
             # at most, of e^-30 and 127 * 0.03
             assert (np.abs(got[row, h] - v[first]) <= 2.0 ** -20 * np.abs(v[first]) + 4e-10).all(), (row, h)
     assert checked > b.rows * heads // 2
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("low", [-1e4, -1e10, -1e20, -1e30])
+def test_scores_far_below_the_others(cuda, kind, low):
+    """Keys pushed far down by their scale, whole blocks of them in front of the others and
+    single ones between: the rest comes out as without them."""
+    b, heads, q8, qs = positive(kind, 8)
+    n_sel = 20
+    ids = np.tile(np.arange(n_sel, dtype=np.int32), (b.rows, 2))
+    hidden = b.tables.copy()
+    for i in (0, 1, 2, 3, 4, 6, 9):
+        b.ks[b.tables[0, i]] = low
+        hidden[0, i] = 65535
+    got = run(kind, b, q8, qs, heads, ids, n_sel)
+    b.tables = hidden  # the same as pages outside the pool: weights below 2^-1000
+    want, mag, top = attend(b, q8, qs, heads, QK, True, ids if kind == "listed" else None, n_sel)
+    sees = [r for r, s, p in b.row_positions() if s or p >= 5 * 32]
+    assert (np.abs(got - want) <= attend_bound(mag, top, b.max_kv))[sees].all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("size", [1.0, 2.0 ** 4, 2.0 ** 30, 2.0 ** 60])
+def test_equal_scores(cuda, kind, size):
+    """One key over and over: all have the same weight, however large their score."""
+    b, heads, q8, qs = positive(kind, 9)
+    b.k[:] = b.k[0, 0]
+    b.ks[:] = np.where(np.isnan(b.ks), np.nan, F(0.0217) * F(size))
+    n_sel = 20
+    ids = np.tile(np.arange(n_sel, dtype=np.int32), (b.rows, 2))
+    got = run(kind, b, q8, qs, heads, ids, n_sel)
+    b.ks[:] = np.where(np.isnan(b.ks), np.nan, 0)  # scores of no size: weights of 1
+    want, mag, _ = attend(b, q8, qs, heads, QK, True, ids if kind == "listed" else None, n_sel)
+    assert (np.abs(got - want) <= attend_bound(mag, 0, b.max_kv)).all()
